@@ -3,10 +3,10 @@
  *
  * This library replaces the reference's Objective-C++ nanobind module
  * `metal_backend` (src/metal_backend.mm:253-261). Every entry point returns an int
- * status: 0 = success, nonzero = failure, with the message available from
- * mt_last_error(). The Python layer raises RuntimeError on nonzero, matching the
- * reference's std::runtime_error -> RuntimeError behaviour (metal_backend.mm:78,
- * 192-207, 230-232).
+ * status: 0 = success, nonzero = failure (2 = an argument that does not fit, where an entry
+ * says so), with the message available from mt_last_error(). The Python layer raises
+ * RuntimeError on nonzero (ValueError on 2), matching the reference's
+ * std::runtime_error -> RuntimeError behaviour (metal_backend.mm:78, 192-207, 230-232).
  *
  * Threading: one CUDA stream per device; the buffer registry and kernel table are
  * mutex-guarded. Device work is stream ordered; reads synchronise the stream.
@@ -142,6 +142,71 @@ int mt_reduce_rows(int dev, uint64_t in_buf, uint64_t out_buf, uint64_t rows, ui
  * restored before returning. */
 int mt_reduce_rows_noalloc(int dev, const float* in, float* out, uint64_t rows, uint64_t cols, uint64_t ld,
                            int op, void* stream);
+
+/* ---- paged key-value cache ---------------------------------------------------
+ * No counterpart in the reference (its attention reads whole K and V tensors). These
+ * entry points take device arrays that the caller owns, allocate nothing and run on
+ * `stream` (a cudaStream_t of `dev`; NULL = this library's stream of `dev`) without
+ * waiting for it. They return 2 for an argument that does not fit (nothing was
+ * launched), 1 for a failed CUDA call. Calls may be captured into CUDA graphs. */
+
+enum {
+    MT_F32 = 0, MT_F16 = 1, MT_BF16 = 2,
+    MT_I8 = 3,    /* codes -127..127, value = code * scale */
+    MT_E4M3 = 4,  /* 8-bit floats (4 exponent, 3 fraction bits), value = code * scale */
+    MT_I32 = 5, MT_I64 = 6
+};
+
+/* A device array. Element (i0, i1, ..) is at ptr + dot(i, strides); strides count elements. */
+typedef struct mt_array {
+    void* ptr;
+    int32_t dtype;
+    int32_t ndim;
+    int64_t shape[4];
+    int64_t strides[4];
+} mt_array;
+
+/* A cache of `pages` pages of `page_size` tokens. k, v: [pages, page_size, kv_heads,
+ * head_dim] of one of MT_F32 .. MT_E4M3, head_dim at most 256, the last stride 1, the
+ * others free. The 8-bit types have k_scale, v_scale: MT_F32 [pages, page_size,
+ * kv_heads], any strides; for the others their ndim is 0. Slot s is token s % page_size
+ * of page s / page_size. */
+typedef struct mt_paged_cache {
+    mt_array k, v, k_scale, v_scale;
+} mt_paged_cache;
+
+/* Write rows k[i], v[i] ([tokens, kv_heads, head_dim], MT_F32 / MT_F16 / MT_BF16, last
+ * stride 1) into slot slots[i] ([tokens], MT_I32 or MT_I64). Rounds to the cache's type;
+ * for the 8-bit types each (token, head) row gets scale = fp32(largest |x| / 127 or 448)
+ * and codes nearest to x / scale, ties to even; a row that holds an infinity or a NaN
+ * gets scale NaN. Rows whose slot is outside [0, pages * page_size) are skipped. Slots
+ * must be distinct: one that is given twice is left with a mixture of its rows. */
+int mt_cache_write(int dev, const mt_array* k, const mt_array* v, const mt_paged_cache* cache,
+                   const mt_array* slots, void* stream);
+/* Read slot slots[i] back into k[i], v[i] (either may be NULL), converted to their type;
+ * a slot outside the cache reads as zeros. */
+int mt_cache_read(int dev, const mt_paged_cache* cache, const mt_array* slots, const mt_array* k,
+                  const mt_array* v, void* stream);
+
+/* Attention of one query token per sequence over the cache:
+ *   out[b, h] = softmax over t of (scale * q[b, h] . K[b, t, g]) times V[b, t, g],
+ * g = h / (heads / kv_heads), for the tokens t in [max(0, n - window), n) (window 0: from
+ * 0), n = lengths[b] clamped to the table's width; token t is in page
+ * tables[b, t / page_size]. Pages outside [0, pages) count as absent. A sequence without
+ * tokens gets zeros. q, out: [batch, heads, head_dim], last stride 1, of one type:
+ * MT_F32, or the cache's own 16-bit type, or any of the three on an 8-bit cache; an
+ * MT_F32 cache takes MT_F32. tables: MT_I32 [batch, width], last stride 1; lengths: MT_I32
+ * [batch]; lse (may be NULL): MT_F32 [batch, heads], the natural logarithm of the sum of
+ * exp(scores), -inf without tokens. Scores, sums and the output's accumulators are fp32.
+ * `workspace`: mt_paged_attention_workspace() bytes of device memory, 16-byte aligned,
+ * that no other call may use at the same time; its contents do not matter. */
+int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
+                       const mt_array* lengths, const mt_array* out, const mt_array* lse, double scale,
+                       int64_t window, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Bytes of workspace such a call needs (0: none). They depend on the shapes, the types
+ * and the device, not on the lengths. */
+int mt_paged_attention_workspace(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
+                                 uint64_t* bytes);
 
 /* ---- multi-GPU: combining sharded whole-tensor reductions -------------------
  * No counterpart in the reference (its Metal backend drives one GPU); a sharded

@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent.parent
@@ -29,15 +30,37 @@ def nvcc() -> str:
     return exe
 
 
+def sources() -> list[Path]:
+    return sorted((PKG / "csrc").glob("*.cu"))
+
+
 def build_backend(force: bool = False, verbose: bool = False) -> Path:
-    src = PKG / "csrc" / "cuda_backend.cu"
-    hdr = REPO / "include" / "metellus_b200.h"
+    """Compile every ``csrc/*.cu`` (in parallel, only what changed) and link them."""
+    headers = [REPO / "include" / "metellus_b200.h", *(PKG / "csrc").glob("*.h"),
+               *(PKG / "csrc" / "include").glob("*.cuh")]
+    newest_header = max(h.stat().st_mtime for h in headers)
     LIB_DIR.mkdir(exist_ok=True)
-    if not force and LIB.exists() and LIB.stat().st_mtime >= max(src.stat().st_mtime, hdr.stat().st_mtime):
+    newest = max(newest_header, *(s.stat().st_mtime for s in sources()))
+    if not force and LIB.exists() and LIB.stat().st_mtime >= newest:
         return LIB
+    obj_dir = PKG / "csrc" / "_build"
+    obj_dir.mkdir(exist_ok=True)
+
+    def compile_one(src: Path) -> Path:
+        obj = obj_dir / (src.stem + ".o")
+        if not force and obj.exists() and obj.stat().st_mtime >= max(newest_header, src.stat().st_mtime):
+            return obj
+        cmd = [nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-c",
+               "-I", str(REPO / "include"), "-o", str(obj), str(src)]
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.run(cmd, check=True)
+        return obj
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        objects = list(pool.map(compile_one, sources()))
     cmd = [
-        nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-        "-I", str(REPO / "include"), "-o", str(LIB), str(src),
+        nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(LIB), *map(str, objects),
         "-cudart", "static", "-L", str(CUDA_HOME / "lib64"), "-lnvrtc",
         f"-Xlinker=-rpath,{CUDA_HOME / 'lib64'}",
     ]

@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "../../include/metellus_b200.h"
+#include "mt_host.h"
 
 namespace {
 
@@ -41,23 +42,7 @@ struct DriverApi {
     bool ok = false;
 } g_drv;
 
-int fail(const char* fmt, ...) {
-    char buf[2048];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    g_err = buf;
-    return 1;
-}
-
-#define RT_CHECK(call)                                                               \
-    do {                                                                             \
-        cudaError_t e_ = (call);                                                     \
-        if (e_ != cudaSuccess)                                                       \
-            return fail("%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_),      \
-                        __FILE__, __LINE__);                                         \
-    } while (0)
+using mt::fail;
 
 #define DRV_CHECK(call)                                                              \
     do {                                                                             \
@@ -154,7 +139,58 @@ int get_func(KernelEntry* k, int dev, CUfunction* f) {
     return 0;
 }
 
+int g_sms[kMaxDev] = {};
+
 }  // namespace
+
+namespace mt {
+
+int fail(const char* fmt, ...) {
+    char buf[2048];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_err = buf;
+    return 1;
+}
+
+int bad_argument(const char* fmt, ...) {
+    char buf[2048];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_err = buf;
+    return 2;
+}
+
+int call_stream(int dev, void* stream, cudaStream_t* out) {
+    if (dev < 0 || dev >= kMaxDev) return bad_argument("device index %d out of range", dev);
+    if (stream) {
+        // a stream of another device is refused by the launch itself; asking for its
+        // device here would break a capture
+        *out = (cudaStream_t)stream;
+        return 0;
+    }
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (ensure_dev(dev)) return 1;
+    *out = g_dev[dev].stream;
+    return 0;
+}
+
+int sm_count(int dev, int* out) {
+    if (dev < 0 || dev >= kMaxDev) return bad_argument("device index %d out of range", dev);
+    if (!g_sms[dev]) {
+        int v = 0;
+        RT_CHECK(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev));
+        g_sms[dev] = v;  // the same value from every thread
+    }
+    *out = g_sms[dev];
+    return 0;
+}
+
+}  // namespace mt
 
 // ---- native split-row reduction ------------------------------------------------
 

@@ -1,0 +1,48 @@
+// What the backend's translation units share on the host: the error message behind
+// mt_last_error, the per-device stream, and checks of the arrays that callers describe.
+#ifndef METELLUS_MT_HOST_H
+#define METELLUS_MT_HOST_H
+
+#include <cuda_runtime.h>
+
+#include "../../include/metellus_b200.h"
+
+namespace mt {
+
+// Record the calling thread's error message; fail returns 1 (the call failed), bad_argument
+// 2 (nothing was done: an argument does not fit).
+int fail(const char* fmt, ...);
+int bad_argument(const char* fmt, ...);
+
+// The stream a call runs on: the caller's, or (NULL) the library's own stream of `dev`,
+// initialising the device at first use.
+int call_stream(int dev, void* stream, cudaStream_t* out);
+// Number of SMs of `dev` (looked up once per device).
+int sm_count(int dev, int* out);
+
+#define RT_CHECK(call)                                                               \
+    do {                                                                             \
+        cudaError_t e_ = (call);                                                     \
+        if (e_ != cudaSuccess)                                                       \
+            return mt::fail("%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_),  \
+                            __FILE__, __LINE__);                                     \
+    } while (0)
+
+// Makes `dev` current for a call and gives the caller its own device back.
+struct OnDevice {
+    int caller = -1;
+    cudaError_t enter(int dev) {
+        int now = -1;
+        cudaError_t e = cudaGetDevice(&now);
+        if (e != cudaSuccess || now == dev) return e;
+        caller = now;
+        return cudaSetDevice(dev);
+    }
+    ~OnDevice() {
+        if (caller >= 0) cudaSetDevice(caller);
+    }
+};
+
+}  // namespace mt
+
+#endif

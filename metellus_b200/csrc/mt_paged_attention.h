@@ -1,0 +1,31 @@
+// Paged attention: arguments after the checks, and the kernels' entry points.
+#ifndef METELLUS_MT_PAGED_ATTENTION_H
+#define METELLUS_MT_PAGED_ATTENTION_H
+
+#include "mt_paged.h"
+
+namespace mt {
+
+struct AttentionArgs {
+    const void* q;
+    int64_t q_seq, q_head;  // strides in elements
+    void* out;
+    int64_t out_seq, out_head;
+    float* lse;  // may be null
+    int64_t lse_seq, lse_head;
+    const int32_t* tables;
+    int64_t table_seq;
+    const int32_t* lengths;
+    int64_t length_seq;
+    CacheShape cache;
+    FastDiv page;
+    int q_type, batch, group, max_tokens, window;
+    float scale;
+};
+
+// Any head_dim and alignment: one warp a key row (attention_rows.cu).
+int attend_by_rows(const AttentionArgs& a, cudaStream_t st);
+
+}  // namespace mt
+
+#endif

@@ -1,0 +1,106 @@
+// Attention of one new token per sequence over a paged key-value cache
+// (mt_paged_attention): argument checks and the choice of the kernel.
+#include <cmath>
+
+#include "mt_paged_attention.h"
+
+namespace mt {
+
+namespace {
+
+int check_attention(const char* who, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
+                    AttentionArgs* a, int* batch, int* heads) {
+    CacheShape c;
+    if (int rc = check_cache(who, cache, false, &c)) return rc;
+    if (int rc = check_array(who, "q", q, 3, 1u << MT_F32 | 1u << MT_F16 | 1u << MT_BF16, true)) return rc;
+    if (q->shape[2] != c.head_dim)
+        return bad_argument("%s: q has head_dim %lld, the cache %d", who, (long long)q->shape[2], c.head_dim);
+    if (q->shape[1] < 1 || q->shape[1] % c.kv_heads)
+        return bad_argument("%s: %lld query heads are not a multiple of %d key-value heads", who,
+                            (long long)q->shape[1], c.kv_heads);
+    if (q->shape[1] > 65535 || q->shape[0] > 65535 * 32)
+        return bad_argument("%s: at most %d sequences of 65535 heads", who, 65535 * 32);
+    if (q->dtype != MT_F32 && !c.scaled() && q->dtype != c.dtype)
+        return bad_argument("%s: q of %s does not go with a cache of %s", who, dtype_name(q->dtype),
+                            dtype_name(c.dtype));
+    if (int rc = check_array(who, "tables", tables, 2, 1u << MT_I32, true)) return rc;
+    if (tables->shape[0] != q->shape[0])
+        return bad_argument("%s: tables has %lld rows, q %lld", who, (long long)tables->shape[0], (long long)q->shape[0]);
+    if (tables->shape[1] > INT32_MAX / c.page_size)
+        return bad_argument("%s: the tables' width allows over 2^31 - 1 tokens", who);
+    a->q = q->ptr;
+    a->q_seq = q->strides[0];
+    a->q_head = q->strides[1];
+    a->cache = c;
+    a->tables = (const int32_t*)tables->ptr;
+    a->table_seq = tables->strides[0];
+    a->max_tokens = (int)tables->shape[1] * c.page_size;
+    a->page = FastDiv((uint32_t)c.page_size);
+    a->group = (int)(q->shape[1] / c.kv_heads);
+    a->q_type = q->dtype;
+    *batch = (int)q->shape[0];
+    *heads = (int)q->shape[1];
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace mt
+
+using namespace mt;
+
+extern "C" {
+
+int mt_paged_attention_workspace(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
+                                 uint64_t* bytes) {
+    const char* who = "paged_attention_workspace";
+    AttentionArgs a{};
+    int batch, heads;
+    if (!bytes) return bad_argument("%s: bytes is missing", who);
+    if (int rc = check_attention(who, q, cache, tables, &a, &batch, &heads)) return rc;
+    *bytes = 0;
+    return 0;
+}
+
+int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
+                       const mt_array* lengths, const mt_array* out, const mt_array* lse, double scale,
+                       int64_t window, void* workspace, uint64_t workspace_bytes, void* stream) {
+    const char* who = "paged_attention";
+    AttentionArgs a{};
+    int batch, heads;
+    if (int rc = check_attention(who, q, cache, tables, &a, &batch, &heads)) return rc;
+    if (int rc = check_array(who, "lengths", lengths, 1, 1u << MT_I32, false)) return rc;
+    if (lengths->shape[0] != batch)
+        return bad_argument("%s: lengths has %lld entries, q %d sequences", who, (long long)lengths->shape[0], batch);
+    if (int rc = check_array(who, "out", out, 3, 1u << q->dtype, true)) return rc;
+    for (int i = 0; i < 3; ++i)
+        if (out->shape[i] != q->shape[i]) return bad_argument("%s: out must have q's shape", who);
+    if (int rc = check_written(who, "out", *out)) return rc;
+    if (lse) {
+        if (int rc = check_array(who, "lse", lse, 2, 1u << MT_F32, false)) return rc;
+        if (lse->shape[0] != batch || lse->shape[1] != heads)
+            return bad_argument("%s: lse must be [batch, heads]", who);
+        if (int rc = check_written(who, "lse", *lse)) return rc;
+        a.lse = (float*)lse->ptr;
+        a.lse_seq = lse->strides[0];
+        a.lse_head = lse->strides[1];
+    }
+    if (!std::isfinite(scale)) return bad_argument("%s: scale must be finite", who);
+    if (window < 0) return bad_argument("%s: window must not be negative", who);
+    if (batch == 0) return 0;
+    a.lengths = (const int32_t*)lengths->ptr;
+    a.length_seq = lengths->strides[0];
+    a.out = out->ptr;
+    a.out_seq = out->strides[0];
+    a.out_head = out->strides[1];
+    a.scale = (float)scale;
+    a.window = window == 0 || window > INT32_MAX ? INT32_MAX : (int)window;
+    a.batch = batch;
+    cudaStream_t st;
+    OnDevice on;
+    RT_CHECK(on.enter(dev));
+    if (int rc = call_stream(dev, stream, &st)) return rc;
+    return attend_by_rows(a, st);
+}
+
+}  // extern "C"

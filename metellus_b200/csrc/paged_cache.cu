@@ -1,0 +1,358 @@
+// Writing a paged key-value cache and reading it back (mt_cache_write, mt_cache_read).
+//
+// One warp a row (one token's head, of K or of V): the row stays in registers between
+// the pass that finds its largest magnitude and the one that stores its codes, so HBM
+// sees each element once each way.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "mt_paged.h"
+
+namespace mt {
+
+const char* dtype_name(int dtype) {
+    static const char* const names[] = {"float32", "float16", "bfloat16", "int8", "float8_e4m3", "int32", "int64"};
+    return dtype >= 0 && dtype <= MT_I64 ? names[dtype] : "unknown";
+}
+
+int64_t elements(const mt_array& a) {
+    int64_t n = 1;
+    for (int i = 0; i < a.ndim; ++i) n *= a.shape[i];
+    return n;
+}
+
+int check_array(const char* who, const char* name, const mt_array* a, int ndim, uint32_t dtypes, bool last1) {
+    if (!a) return bad_argument("%s: %s is missing", who, name);
+    if (a->ndim != ndim) return bad_argument("%s: %s must have %d dimensions, not %d", who, name, ndim, a->ndim);
+    if (a->dtype < 0 || a->dtype > MT_I64 || !(dtypes >> a->dtype & 1))
+        return bad_argument("%s: %s cannot be %s", who, name, dtype_name(a->dtype));
+    double bytes = bytes_of(a->dtype);
+    for (int i = 0; i < ndim; ++i) {
+        if (a->shape[i] < 0) return bad_argument("%s: %s has a negative extent", who, name);
+        if (a->shape[i] > 1 && a->strides[i] < 0) return bad_argument("%s: %s has a negative stride", who, name);
+        bytes *= (double)a->shape[i];
+    }
+    if (bytes > 4e18) return bad_argument("%s: %s is too large", who, name);
+    if (last1 && a->shape[ndim - 1] > 1 && a->strides[ndim - 1] != 1)
+        return bad_argument("%s: the last dimension of %s must be contiguous", who, name);
+    if (elements(*a) > 0) {
+        if (!a->ptr) return bad_argument("%s: %s has no memory", who, name);
+        if ((uintptr_t)a->ptr % bytes_of(a->dtype))
+            return bad_argument("%s: %s is not aligned to its elements", who, name);
+    }
+    return 0;
+}
+
+int check_written(const char* who, const char* name, const mt_array& a) {
+    if (elements(a) == 0) return 0;
+    for (int i = 0; i < a.ndim; ++i)
+        if (a.shape[i] > 1 && a.strides[i] == 0)
+            return bad_argument("%s: %s is written and must not be a broadcast (stride 0)", who, name);
+    return 0;
+}
+
+static bool same_shape(const mt_array& a, const mt_array& b, int n) {
+    for (int i = 0; i < n; ++i)
+        if (a.shape[i] != b.shape[i]) return false;
+    return true;
+}
+
+static CacheView view_of(const mt_array& a) {
+    CacheView v;
+    if (a.ndim < 3) return v;
+    v.ptr = a.ptr;
+    v.page = a.strides[0];
+    v.token = a.strides[1];
+    v.head = a.strides[2];
+    return v;
+}
+
+int check_cache(const char* who, const mt_paged_cache* c, bool written, CacheShape* out) {
+    if (!c) return bad_argument("%s: the cache is missing", who);
+    const uint32_t types = 1u << MT_F32 | 1u << MT_F16 | 1u << MT_BF16 | 1u << MT_I8 | 1u << MT_E4M3;
+    if (int rc = check_array(who, "k_cache", &c->k, 4, types, true)) return rc;
+    if (int rc = check_array(who, "v_cache", &c->v, 4, types, true)) return rc;
+    if (c->k.dtype != c->v.dtype) return bad_argument("%s: k_cache and v_cache must have one type", who);
+    if (!same_shape(c->k, c->v, 4)) return bad_argument("%s: k_cache and v_cache must have one shape", who);
+    const int64_t* s = c->k.shape;
+    if (s[1] < 1 || s[2] < 1 || s[3] < 1)
+        return bad_argument("%s: page_size, kv_heads and head_dim of the cache must be positive", who);
+    if (s[3] > kMaxHeadDim) return bad_argument("%s: head_dim %lld is over %d", who, (long long)s[3], kMaxHeadDim);
+    if (s[0] > INT32_MAX || s[1] > INT32_MAX || s[2] > 65535 || s[0] * s[1] > INT32_MAX)
+        return bad_argument("%s: a cache holds at most 2^31 - 1 tokens of 65535 heads", who);
+    const bool scaled = c->k.dtype == MT_I8 || c->k.dtype == MT_E4M3;
+    for (int i = 0; i < 2; ++i) {
+        const mt_array& z = i ? c->v_scale : c->k_scale;
+        const char* name = i ? "v_scale" : "k_scale";
+        if (!scaled) {
+            if (z.ndim) return bad_argument("%s: a cache of %s has no %s", who, dtype_name(c->k.dtype), name);
+            continue;
+        }
+        if (!z.ndim) return bad_argument("%s: a cache of %s needs %s", who, dtype_name(c->k.dtype), name);
+        if (int rc = check_array(who, name, &z, 3, 1u << MT_F32, false)) return rc;
+        if (!same_shape(z, c->k, 3))
+            return bad_argument("%s: %s must be [pages, page_size, kv_heads] of the cache", who, name);
+        if (written)
+            if (int rc = check_written(who, name, z)) return rc;
+    }
+    if (written) {
+        if (int rc = check_written(who, "k_cache", c->k)) return rc;
+        if (int rc = check_written(who, "v_cache", c->v)) return rc;
+    }
+    out->dtype = c->k.dtype;
+    out->pages = (int)s[0];
+    out->page_size = (int)s[1];
+    out->kv_heads = (int)s[2];
+    out->head_dim = (int)s[3];
+    out->k = view_of(c->k);
+    out->v = view_of(c->v);
+    if (scaled) {
+        out->k_scale = view_of(c->k_scale);
+        out->v_scale = view_of(c->v_scale);
+    }
+    return 0;
+}
+
+bool rows_aligned(const mt_array& a, int align) {
+    if ((uintptr_t)a.ptr % align) return false;
+    for (int i = 0; i + 1 < a.ndim; ++i)
+        if (a.shape[i] > 1 && a.strides[i] * bytes_of(a.dtype) % align) return false;
+    return true;
+}
+
+}  // namespace mt
+
+namespace {
+
+using namespace mt;
+
+// Rows outside the cache: [tokens, heads, head_dim], last stride 1.
+struct RowsView {
+    void* ptr;
+    int64_t token, head;
+};
+
+struct RowArgs {
+    RowsView rows[2];      // k, v
+    CacheView cache[2];
+    CacheView scale[2];
+    const void* slots;
+    int64_t slot_stride;
+    int slots64;
+    int total_slots, head_dim, first, count;  // which of k, v: first .. first + count - 1
+    int64_t row_count;                         // tokens * heads
+    FastDiv heads, page;
+};
+
+template <class T> __device__ inline float to_float(T x) { return (float)x; }
+template <> __device__ inline float to_float(__nv_fp8_e4m3 x) { return (float)x; }
+template <> __device__ inline float to_float(int8_t x) { return (float)x; }
+
+template <class T> __device__ inline T from_float(float x);
+template <> __device__ inline float from_float<float>(float x) { return x; }
+template <> __device__ inline __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <class C> struct Code;
+
+// The code nearest to x / s, ties to even. x / s in fp32 can be rounded onto a border
+// between two codes, so the nearest integer n to it is checked by the remainder
+// x - n s, which one fma gives exactly: more than half of s means the other neighbour.
+__device__ inline float nearest_multiple(float x, float s, float t) {
+    float n = rintf(t);
+    const float r = fmaf(-n, s, x), twice = 2.0f * fabsf(r);
+    if (twice > s || (twice == s && fmodf(n, 2.0f) != 0.0f)) n += copysignf(1.0f, r);
+    return n;
+}
+
+template <> struct Code<int8_t> {
+    static constexpr float kLargest = 127.0f;
+    static __device__ int8_t of(float x, float s) {
+        const float n = nearest_multiple(x, s, x / s);
+        return (int8_t)fminf(fmaxf(n, -127.0f), 127.0f);
+    }
+};
+template <> struct Code<__nv_fp8_e4m3> {
+    static constexpr float kLargest = 448.0f;
+    static __device__ __nv_fp8_e4m3 of(float x, float s) {
+        const float t = x / s;
+        // the spacing of e4m3 around t: 2^(exponent - 3), at least 2^-9
+        const int e = max((int)(__float_as_uint(t) >> 23 & 0xff) - 127, -6) - 3;
+        const float u = __uint_as_float((uint32_t)(e + 127) << 23);
+        const float per = __uint_as_float((uint32_t)(127 - e) << 23);
+        return __nv_fp8_e4m3(nearest_multiple(x, s * u, t * per) * u);
+    }
+};
+
+__device__ inline int64_t slot_of(const RowArgs& a, int64_t token) {
+    return a.slots64 ? ((const int64_t*)a.slots)[token * a.slot_stride]
+                     : (int64_t)((const int32_t*)a.slots)[token * a.slot_stride];
+}
+
+__device__ inline int64_t cache_offset(const CacheView& c, uint32_t page, uint32_t token, uint32_t head) {
+    return (int64_t)page * c.page + (int64_t)token * c.token + (int64_t)head * c.head;
+}
+
+constexpr int kRowThreads = 256;
+constexpr int kPerLane = kMaxHeadDim / 32;
+
+template <class X, class C, bool kScaled>
+__global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a) {
+    const int lane = threadIdx.x & 31, which = a.first + blockIdx.y;
+    const int64_t stride = (int64_t)gridDim.x * (kRowThreads / 32);
+    for (int64_t row = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5); row < a.row_count; row += stride) {
+        uint32_t head;
+        const uint32_t token = a.heads.div((uint32_t)row, &head);
+        const int64_t slot = slot_of(a, token);
+        if (slot < 0 || slot >= a.total_slots) continue;
+        uint32_t at;
+        const uint32_t page = a.page.div((uint32_t)slot, &at);
+        const X* x = (const X*)a.rows[which].ptr + (int64_t)token * a.rows[which].token + (int64_t)head * a.rows[which].head;
+        C* c = (C*)a.cache[which].ptr + cache_offset(a.cache[which], page, at, head);
+        float v[kPerLane];
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) v[i] = lane + 32 * i < a.head_dim ? to_float(x[lane + 32 * i]) : 0.0f;
+        if constexpr (kScaled) {
+            // as bits, magnitudes order like numbers, with infinities and NaN on top
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) top = max(top, __float_as_uint(fabsf(v[i])));
+            top = __reduce_max_sync(0xffffffffu, top);
+            const bool finite = top < 0x7f800000u;
+            const float s = finite ? __uint_as_float(top) / Code<C>::kLargest : __uint_as_float(0x7fc00000u);
+            if (lane == 0)
+                ((float*)a.scale[which].ptr)[cache_offset(a.scale[which], page, at, head)] = s;
+            const bool none = !finite || s == 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i)
+                if (lane + 32 * i < a.head_dim) c[lane + 32 * i] = none ? C(0.0f) : Code<C>::of(v[i], s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i)
+                if (lane + 32 * i < a.head_dim) c[lane + 32 * i] = from_float<C>(v[i]);
+        }
+    }
+}
+
+template <class X, class C, bool kScaled>
+__global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) {
+    const int lane = threadIdx.x & 31, which = a.first + blockIdx.y;
+    const int64_t stride = (int64_t)gridDim.x * (kRowThreads / 32);
+    for (int64_t row = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5); row < a.row_count; row += stride) {
+        uint32_t head;
+        const uint32_t token = a.heads.div((uint32_t)row, &head);
+        const int64_t slot = slot_of(a, token);
+        const bool there = slot >= 0 && slot < a.total_slots;
+        uint32_t at;
+        const uint32_t page = a.page.div(there ? (uint32_t)slot : 0u, &at);
+        X* x = (X*)a.rows[which].ptr + (int64_t)token * a.rows[which].token + (int64_t)head * a.rows[which].head;
+        const C* c = (const C*)a.cache[which].ptr + cache_offset(a.cache[which], page, at, head);
+        float s = 1.0f;
+        if constexpr (kScaled)
+            if (there) s = ((const float*)a.scale[which].ptr)[cache_offset(a.scale[which], page, at, head)];
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+            const int d = lane + 32 * i;
+            if (d < a.head_dim) x[d] = from_float<X>(there ? (kScaled ? to_float(c[d]) * s : to_float(c[d])) : 0.0f);
+        }
+    }
+}
+
+template <class X, class C>
+int launch_rows(bool write, const RowArgs& a, int blocks, cudaStream_t st) {
+    constexpr bool kScaled = sizeof(C) == 1;
+    const dim3 grid(blocks, a.count);
+    if (write)
+        cache_write_rows<X, C, kScaled><<<grid, kRowThreads, 0, st>>>(a);
+    else
+        cache_read_rows<X, C, kScaled><<<grid, kRowThreads, 0, st>>>(a);
+    RT_CHECK(cudaGetLastError());
+    return 0;
+}
+
+template <class X>
+int launch_cache_type(int dtype, bool write, const RowArgs& a, int blocks, cudaStream_t st) {
+    switch (dtype) {
+        case MT_F32: return launch_rows<X, float>(write, a, blocks, st);
+        case MT_F16: return launch_rows<X, __half>(write, a, blocks, st);
+        case MT_BF16: return launch_rows<X, __nv_bfloat16>(write, a, blocks, st);
+        case MT_I8: return launch_rows<X, int8_t>(write, a, blocks, st);
+        default: return launch_rows<X, __nv_fp8_e4m3>(write, a, blocks, st);
+    }
+}
+
+int move_rows(const char* who, bool write, int dev, const mt_array* k, const mt_array* v, const mt_paged_cache* cache,
+              const mt_array* slots, void* stream) {
+    CacheShape c;
+    if (int rc = check_cache(who, cache, write, &c)) return rc;
+    if (!k && !v) return bad_argument("%s: k and v are missing", who);
+    const uint32_t types = 1u << MT_F32 | 1u << MT_F16 | 1u << MT_BF16;
+    if (int rc = check_array(who, "slots", slots, 1, 1u << MT_I32 | 1u << MT_I64, false)) return rc;
+    RowArgs a{};
+    int dtype = -1;
+    for (int i = 0; i < 2; ++i) {
+        const mt_array* x = i ? v : k;
+        const char* name = i ? "v" : "k";
+        if (!x) continue;
+        if (int rc = check_array(who, name, x, 3, types, true)) return rc;
+        if (x->shape[1] != c.kv_heads || x->shape[2] != c.head_dim)
+            return bad_argument("%s: %s must be [tokens, %d, %d] as the cache's heads are", who, name, c.kv_heads, c.head_dim);
+        if (x->shape[0] != slots->shape[0])
+            return bad_argument("%s: %s has %lld tokens, slots %lld", who, name, (long long)x->shape[0],
+                                (long long)slots->shape[0]);
+        if (dtype >= 0 && dtype != x->dtype) return bad_argument("%s: k and v must have one type", who);
+        dtype = x->dtype;
+        if (!write)
+            if (int rc = check_written(who, name, *x)) return rc;
+        a.rows[i] = {x->ptr, x->strides[0], x->strides[1]};
+    }
+    a.first = k ? 0 : 1;
+    a.count = (k ? 1 : 0) + (v ? 1 : 0);
+    const int64_t tokens = slots->shape[0];
+    if (tokens > INT32_MAX / c.kv_heads) return bad_argument("%s: over 2^31 - 1 rows in one call", who);
+    if (tokens == 0) return 0;
+    if (c.pages == 0 && write) return 0;  // every slot is outside the cache
+    a.cache[0] = c.k;
+    a.cache[1] = c.v;
+    a.scale[0] = c.k_scale;
+    a.scale[1] = c.v_scale;
+    a.slots = slots->ptr;
+    a.slot_stride = slots->strides[0];
+    a.slots64 = slots->dtype == MT_I64;
+    a.total_slots = c.pages * c.page_size;
+    a.head_dim = c.head_dim;
+    a.row_count = tokens * c.kv_heads;
+    a.heads = FastDiv((uint32_t)c.kv_heads);
+    a.page = FastDiv((uint32_t)c.page_size);
+    cudaStream_t st;
+    OnDevice on;
+    RT_CHECK(on.enter(dev));
+    if (int rc = call_stream(dev, stream, &st)) return rc;
+    int sms;
+    if (int rc = sm_count(dev, &sms)) return rc;
+    const int64_t want = (a.row_count + kRowThreads / 32 - 1) / (kRowThreads / 32);
+    const int blocks = (int)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8);
+    switch (dtype) {
+        case MT_F32: return launch_cache_type<float>(c.dtype, write, a, blocks, st);
+        case MT_F16: return launch_cache_type<__half>(c.dtype, write, a, blocks, st);
+        default: return launch_cache_type<__nv_bfloat16>(c.dtype, write, a, blocks, st);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int mt_cache_write(int dev, const mt_array* k, const mt_array* v, const mt_paged_cache* cache, const mt_array* slots,
+                   void* stream) {
+    if (!k || !v) return bad_argument("cache_write: k and v are both needed");
+    return move_rows("cache_write", true, dev, k, v, cache, slots, stream);
+}
+
+int mt_cache_read(int dev, const mt_paged_cache* cache, const mt_array* slots, const mt_array* k, const mt_array* v,
+                  void* stream) {
+    return move_rows("cache_read", false, dev, k, v, cache, slots, stream);
+}
+
+}  // extern "C"

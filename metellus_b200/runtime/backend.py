@@ -51,6 +51,26 @@ class MtTmapSpec(ctypes.Structure):
     ]
 
 
+class MtArray(ctypes.Structure):
+    """``mt_array``: a device array as the paged-cache entry points take it."""
+
+    _fields_ = [
+        ("ptr", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("ndim", ctypes.c_int32),
+        ("shape", ctypes.c_int64 * 4),
+        ("strides", ctypes.c_int64 * 4),
+    ]
+
+
+class MtPagedCache(ctypes.Structure):
+    _fields_ = [("k", MtArray), ("v", MtArray), ("k_scale", MtArray), ("v_scale", MtArray)]
+
+
+# mt_array dtype codes
+ARRAY_DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3, "float8_e4m3fn": 4, "int32": 5, "int64": 6}
+
+
 EXPORTED = (
     "mt_last_error", "mt_device_count", "mt_init", "mt_device_attr", "mt_buffer_create",
     "mt_buffer_release", "mt_buffer_size", "mt_buffer_ptr", "mt_buffer_write", "mt_buffer_read",
@@ -60,6 +80,7 @@ EXPORTED = (
     "mt_event_create", "mt_event_record", "mt_event_elapsed", "mt_event_destroy",
     "mt_graph_begin", "mt_graph_end", "mt_graph_launch", "mt_graph_destroy", "mt_reduce_rows",
     "mt_reduce_rows_noalloc", "mt_nccl_unique_id", "mt_nccl_init", "mt_nccl_destroy", "mt_allreduce_f64",
+    "mt_cache_write", "mt_cache_read", "mt_paged_attention", "mt_paged_attention_workspace",
 )
 
 
@@ -120,6 +141,12 @@ def lib() -> ctypes.CDLL:
                 "mt_nccl_init": [i32, i32, i32, ctypes.c_char_p],
                 "mt_nccl_destroy": [i32],
                 "mt_allreduce_f64": [i32, u64, u64, i32, u64],
+                "mt_cache_write": [i32, P(MtArray), P(MtArray), P(MtPagedCache), P(MtArray), ctypes.c_void_p],
+                "mt_cache_read": [i32, P(MtPagedCache), P(MtArray), P(MtArray), P(MtArray), ctypes.c_void_p],
+                "mt_paged_attention": [i32, P(MtArray), P(MtPagedCache), P(MtArray), P(MtArray), P(MtArray),
+                                       P(MtArray), ctypes.c_double, ctypes.c_int64, ctypes.c_void_p, u64,
+                                       ctypes.c_void_p],
+                "mt_paged_attention_workspace": [i32, P(MtArray), P(MtPagedCache), P(MtArray), P(u64)],
             }
             for name, args in sig.items():
                 fn = getattr(L, name)
@@ -133,7 +160,8 @@ def _check(rc: int) -> None:
     if rc != 0:
         buf = ctypes.create_string_buffer(4096)
         lib().mt_last_error(buf, 4096)
-        raise RuntimeError(buf.value.decode(errors="replace"))
+        message = buf.value.decode(errors="replace")
+        raise ValueError(message) if rc == 2 else RuntimeError(message)
 
 
 # -- devices -----------------------------------------------------------------------
