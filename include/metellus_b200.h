@@ -193,7 +193,7 @@ int mt_cache_read(int dev, const mt_paged_cache* cache, const mt_array* slots, c
  * g = h / (heads / kv_heads), for the tokens t in [max(0, n - window), n) (window 0: from
  * 0), n = lengths[b] clamped to the table's width; token t is in page
  * tables[b, t / page_size]. Pages outside [0, pages) count as absent. A sequence without
- * tokens gets zeros. q, out: [batch, heads, head_dim], last stride 1, of one type:
+ * tokens (or whose scores are all -inf) gets zeros. q, out: [batch, heads, head_dim], last stride 1, of one type:
  * MT_F32, or the cache's own 16-bit type, or any of the three on an 8-bit cache; an
  * MT_F32 cache takes MT_F32. tables: MT_I32 [batch, width], last stride 1; lengths: MT_I32
  * [batch]; lse (may be NULL): MT_F32 [batch, heads], the natural logarithm of the sum of
@@ -203,10 +203,10 @@ int mt_cache_read(int dev, const mt_paged_cache* cache, const mt_array* slots, c
 int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
                        const mt_array* lengths, const mt_array* out, const mt_array* lse, double scale,
                        int64_t window, void* workspace, uint64_t workspace_bytes, void* stream);
-/* Bytes of workspace such a call needs (0: none). They depend on the shapes, the types
- * and the device, not on the lengths. */
+/* Bytes of workspace such a call needs (0: none). They depend on the shapes, the types, the
+ * window and the device, not on the lengths. */
 int mt_paged_attention_workspace(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
-                                 uint64_t* bytes);
+                                 int64_t window, uint64_t* bytes);
 
 /* ---- multi-GPU: combining sharded whole-tensor reductions -------------------
  * No counterpart in the reference (its Metal backend drives one GPU); a sharded

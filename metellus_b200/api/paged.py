@@ -161,7 +161,7 @@ def paged_attention(q, k_cache, v_cache, tables, lengths, *, k_scale=None, v_sca
         al = _array(lse, "lse", device)
     L = backend.lib()
     need = ctypes.c_uint64(0)
-    backend._check(L.mt_paged_attention_workspace(device.index, aq, cache, at, ctypes.byref(need)))
+    backend._check(L.mt_paged_attention_workspace(device.index, aq, cache, at, window, ctypes.byref(need)))
     space = q.new_empty(need.value, dtype=sys.modules["torch"].uint8) if need.value else None
     backend._check(L.mt_paged_attention(device.index, aq, cache, at, an, ao, al, scale, window,
                                         None if space is None else space.data_ptr(), need.value, _stream(device)))

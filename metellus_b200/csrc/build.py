@@ -36,7 +36,7 @@ def sources() -> list[Path]:
 
 def build_backend(force: bool = False, verbose: bool = False) -> Path:
     """Compile every ``csrc/*.cu`` (in parallel, only what changed) and link them."""
-    headers = [REPO / "include" / "metellus_b200.h", *(PKG / "csrc").glob("*.h"),
+    headers = [REPO / "include" / "metellus_b200.h", *(PKG / "csrc").glob("*.h"), *(PKG / "csrc").glob("*.cuh"),
                *(PKG / "csrc" / "include").glob("*.cuh")]
     newest_header = max(h.stat().st_mtime for h in headers)
     LIB_DIR.mkdir(exist_ok=True)

@@ -26,6 +26,15 @@ struct AttentionArgs {
 // Any head_dim and alignment: one warp a key row (attention_rows.cu).
 int attend_by_rows(const AttentionArgs& a, cudaStream_t st);
 
+// Rows of the cache that 16-byte copies can fetch: tiles on the matrix pipe
+// (attention_tiles.cuh), split over the sequences' lengths. `bytes`: the workspace needed;
+// with `workspace` null that is all that is found out.
+int attend_tiles_f32(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_f16(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_bf16(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_i8(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_e4m3(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+
 }  // namespace mt
 
 #endif

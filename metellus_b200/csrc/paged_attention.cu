@@ -9,7 +9,7 @@ namespace mt {
 namespace {
 
 int check_attention(const char* who, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
-                    AttentionArgs* a, int* batch, int* heads) {
+                    int64_t window, AttentionArgs* a, int* batch, int* heads, bool* tiled) {
     CacheShape c;
     if (int rc = check_cache(who, cache, false, &c)) return rc;
     if (int rc = check_array(who, "q", q, 3, 1u << MT_F32 | 1u << MT_F16 | 1u << MT_BF16, true)) return rc;
@@ -23,11 +23,13 @@ int check_attention(const char* who, const mt_array* q, const mt_paged_cache* ca
     if (q->dtype != MT_F32 && !c.scaled() && q->dtype != c.dtype)
         return bad_argument("%s: q of %s does not go with a cache of %s", who, dtype_name(q->dtype),
                             dtype_name(c.dtype));
+    if (window < 0) return bad_argument("%s: window must not be negative", who);
     if (int rc = check_array(who, "tables", tables, 2, 1u << MT_I32, true)) return rc;
     if (tables->shape[0] != q->shape[0])
         return bad_argument("%s: tables has %lld rows, q %lld", who, (long long)tables->shape[0], (long long)q->shape[0]);
-    if (tables->shape[1] > INT32_MAX / c.page_size)
-        return bad_argument("%s: the tables' width allows over 2^31 - 1 tokens", who);
+    // the kernels count tokens in int, up to a few hundred past the end
+    if (tables->shape[1] > (INT32_MAX - 1024) / c.page_size)
+        return bad_argument("%s: the tables' width allows over 2^31 - 1025 tokens", who);
     a->q = q->ptr;
     a->q_seq = q->strides[0];
     a->q_head = q->strides[1];
@@ -38,9 +40,21 @@ int check_attention(const char* who, const mt_array* q, const mt_paged_cache* ca
     a->page = FastDiv((uint32_t)c.page_size);
     a->group = (int)(q->shape[1] / c.kv_heads);
     a->q_type = q->dtype;
-    *batch = (int)q->shape[0];
+    *batch = a->batch = (int)q->shape[0];
     *heads = (int)q->shape[1];
+    a->window = window == 0 || window > INT32_MAX ? INT32_MAX : (int)window;
+    *tiled = c.head_dim * bytes_of(c.dtype) % 16 == 0 && rows_aligned(cache->k, 16) && rows_aligned(cache->v, 16);
     return 0;
+}
+
+int attend_tiles(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
+    switch (a.cache.dtype) {
+        case MT_F32: return attend_tiles_f32(a, workspace, bytes, dev, st);
+        case MT_F16: return attend_tiles_f16(a, workspace, bytes, dev, st);
+        case MT_BF16: return attend_tiles_bf16(a, workspace, bytes, dev, st);
+        case MT_I8: return attend_tiles_i8(a, workspace, bytes, dev, st);
+        default: return attend_tiles_e4m3(a, workspace, bytes, dev, st);
+    }
 }
 
 }  // namespace
@@ -52,14 +66,15 @@ using namespace mt;
 extern "C" {
 
 int mt_paged_attention_workspace(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
-                                 uint64_t* bytes) {
+                                 int64_t window, uint64_t* bytes) {
     const char* who = "paged_attention_workspace";
     AttentionArgs a{};
     int batch, heads;
+    bool tiled;
     if (!bytes) return bad_argument("%s: bytes is missing", who);
-    if (int rc = check_attention(who, q, cache, tables, &a, &batch, &heads)) return rc;
+    if (int rc = check_attention(who, q, cache, tables, window, &a, &batch, &heads, &tiled)) return rc;
     *bytes = 0;
-    return 0;
+    return batch == 0 || !tiled ? 0 : attend_tiles(a, nullptr, bytes, dev, nullptr);
 }
 
 int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
@@ -68,7 +83,8 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
     const char* who = "paged_attention";
     AttentionArgs a{};
     int batch, heads;
-    if (int rc = check_attention(who, q, cache, tables, &a, &batch, &heads)) return rc;
+    bool tiled;
+    if (int rc = check_attention(who, q, cache, tables, window, &a, &batch, &heads, &tiled)) return rc;
     if (int rc = check_array(who, "lengths", lengths, 1, 1u << MT_I32, false)) return rc;
     if (lengths->shape[0] != batch)
         return bad_argument("%s: lengths has %lld entries, q %d sequences", who, (long long)lengths->shape[0], batch);
@@ -86,7 +102,6 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
         a.lse_head = lse->strides[1];
     }
     if (!std::isfinite(scale)) return bad_argument("%s: scale must be finite", who);
-    if (window < 0) return bad_argument("%s: window must not be negative", who);
     if (batch == 0) return 0;
     a.lengths = (const int32_t*)lengths->ptr;
     a.length_seq = lengths->strides[0];
@@ -94,13 +109,18 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
     a.out_seq = out->strides[0];
     a.out_head = out->strides[1];
     a.scale = (float)scale;
-    a.window = window == 0 || window > INT32_MAX ? INT32_MAX : (int)window;
-    a.batch = batch;
     cudaStream_t st;
     OnDevice on;
     RT_CHECK(on.enter(dev));
     if (int rc = call_stream(dev, stream, &st)) return rc;
-    return attend_by_rows(a, st);
+    if (!tiled) return attend_by_rows(a, st);
+    uint64_t need = 0;
+    if (int rc = attend_tiles(a, nullptr, &need, dev, st)) return rc;
+    if (!workspace || workspace_bytes < need)
+        return bad_argument("%s: the workspace has %llu bytes, %llu are needed", who,
+                            (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)need);
+    if ((uintptr_t)workspace % 16) return bad_argument("%s: the workspace is not 16-byte aligned", who);
+    return attend_tiles(a, workspace, &need, dev, st);
 }
 
 }  // extern "C"

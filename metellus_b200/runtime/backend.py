@@ -146,7 +146,7 @@ def lib() -> ctypes.CDLL:
                 "mt_paged_attention": [i32, P(MtArray), P(MtPagedCache), P(MtArray), P(MtArray), P(MtArray),
                                        P(MtArray), ctypes.c_double, ctypes.c_int64, ctypes.c_void_p, u64,
                                        ctypes.c_void_p],
-                "mt_paged_attention_workspace": [i32, P(MtArray), P(MtPagedCache), P(MtArray), P(u64)],
+                "mt_paged_attention_workspace": [i32, P(MtArray), P(MtPagedCache), P(MtArray), ctypes.c_int64, P(u64)],
             }
             for name, args in sig.items():
                 fn = getattr(L, name)

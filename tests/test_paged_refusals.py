@@ -60,7 +60,7 @@ def attend(match, **other):
     ("too large", {"q": array("bfloat16", (2 ** 40, 2 ** 20, 64), (64, 64, 1))}),
     ("tables has 2 rows, q 3", {"tables": array("int32", (2, 5))}),
     ("tables cannot be int64", {"tables": array("int64", (3, 5))}),
-    ("over 2\\^31 - 1 tokens", {"tables": array("int32", (3, 2 ** 28))}),
+    ("over 2\\^31 - 1025 tokens", {"tables": array("int32", (3, 2 ** 28))}),
     ("lengths has 4 entries", {"lengths": array("int32", (4,))}),
     ("lengths is missing", {"lengths": None}),
     ("out cannot be float32", {"out": array("float32", (3, 4, 64))}),
@@ -127,7 +127,7 @@ def test_nothing_to_do_needs_no_device():
     q = array("bfloat16", (0, 4, 64), ptr=0)
     assert L.mt_paged_attention(0, q, cache(), array("int32", (0, 5), ptr=0), array("int32", (0,), ptr=0), q, None,
                                 0.125, 0, None, 0, None) == 0
-    assert L.mt_paged_attention_workspace(0, q, cache(), array("int32", (0, 5), ptr=0), ctypes.byref(need)) == 0
+    assert L.mt_paged_attention_workspace(0, q, cache(), array("int32", (0, 5), ptr=0), 0, ctypes.byref(need)) == 0
     assert need.value == 0
 
 
