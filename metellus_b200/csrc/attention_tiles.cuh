@@ -1,7 +1,7 @@
-// Paged attention of one token per sequence in tiles of 16 tokens a warp.
+// Paged attention of one token per sequence in tiles of 16 or 32 tokens a warp.
 //
-// For each sequence and key-value head: S^T = K Q^T (16 tokens x 8 query heads), the
-// softmax over the tokens in one pass (running maximum m, l = sum exp2(s - m), O = sum
+// For each sequence and key-value head: S^T = K Q^T (16 tokens x 8 query heads a product),
+// the softmax over the tokens in one pass (running maximum m, l = sum exp2(s - m), O = sum
 // exp2(s - m) v, rescaled when m grows), and O^T += V^T P^T. What bounds it is HBM: K and V
 // are read once and used by one token's query heads only (2 flops a query head for each
 // element), so everything here serves the loads:
@@ -10,13 +10,14 @@
 //   columns: a group of 4 or 8 query heads wastes little of them, and 16 columns (NT = 2)
 //   serve larger groups. K's fragments come by ldmatrix, V's by its transposing form; S^T's
 //   accumulators become P^T's operands by transposing 8 x 8 blocks in registers.
-// * Each warp streams its own 16 of a unit's tokens through a ring of S stages in shared
-//   memory (16-byte asynchronous copies, page by page), so no barrier stands between a
-//   copy and its use; warps meet only where a head's part ends.
-// * Units (64 tokens of one sequence and head) of all sequences lie on one line that is
-//   cut into equal ranges, one a block: a ragged batch or one long sequence keeps every SM
-//   at work. A head that a cut crosses leaves parts (m, l, O) in the workspace, and a second
-//   kernel joins them; it is launched early and waits for the first on the device.
+// * Every warp works alone, without barriers: it streams tiles through its own ring of S
+//   stages in shared memory (16-byte asynchronous copies, page by page), and while one
+//   waits where a head ends, the others of its SM go on.
+// * The tiles of all sequences lie on one line that is cut into equal ranges: a ragged batch
+//   or one long sequence keeps every SM at work. Neighbouring warps take the heads of one range,
+//   whose rows are neighbours in memory. A sequence that a cut crosses leaves parts (m, l, O) of
+//   its heads in the workspace, and a second kernel joins them; it is launched early and
+//   waits for the first on the device.
 //
 // 8-bit codes become fp16 in registers, exactly; K's scales multiply the scores, V's the
 // probabilities. 32-bit queries (and 32-bit caches) are split into pieces whose products
@@ -27,6 +28,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "mt_paged_attention.h"
 
 namespace mt {
@@ -36,17 +39,17 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct TileArgs {
     AttentionArgs a;
-    int items;       // per sequence: kv_heads * row blocks
-    int row_blocks;  // blocks of NT * 8 query heads in a group
+    int items;       // of a sequence: kv_heads * row blocks; warp w works on item w % items of range w / items
     int row_chunks;  // 16-byte pieces of a cache row
-    // workspace: two parts a block, (m, l) and O of NT * 8 rows each, and what they are of
-    int4* meta;
+    int q_chunks;    // 16-byte pieces of a query row, 0 where it cannot be copied in pieces
+    int out_quads;   // output rows can be written four elements at a time
+    int whole;       // a range a sequence: nothing is cut
+    FastDiv ranges, per_range, row_blocks;  // divisors: ranges, items, blocks of NT * 8 query heads in a group
+    // workspace: two parts a warp, (m, l) and O of NT * 8 rows each. Part 2 w belongs to a
+    // sequence that began before warp w's range, part 2 w + 1 to one that ends behind it.
     float2* part_ml;
     float* part_o;
 };
-
-// What a block's first part is (meta[block].z), for the join.
-enum { kNoPart = 0, kMiddle = 1, kEnd = 2, kIdle = 3 };
 
 // ---- instructions ------------------------------------------------------------------------
 
@@ -59,6 +62,7 @@ __device__ inline void copy4(uint32_t dst, const void* src, bool really) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(really ? 4 : 0));
 }
 __device__ inline void copies_commit() { asm volatile("cp.async.commit_group;"); }
+__device__ inline void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int N> __device__ inline void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ inline void load_matrices(uint32_t (&r)[4], uint32_t at) {
@@ -103,6 +107,16 @@ template <> __device__ inline float rounded<float>(float x) { return x; }
 template <> __device__ inline __half rounded<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ inline __nv_bfloat16 rounded<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+__device__ inline void store4(float* to, float4 y) { *(float4*)to = y; }
+__device__ inline void store4(__half* to, float4 y) {
+    *(__half2*)to = __floats2half2_rn(y.x, y.y);
+    *(__half2*)(to + 2) = __floats2half2_rn(y.z, y.w);
+}
+__device__ inline void store4(__nv_bfloat16* to, float4 y) {
+    *(__nv_bfloat162*)to = __floats2bfloat162_rn(y.x, y.y);
+    *(__nv_bfloat162*)(to + 2) = __floats2bfloat162_rn(y.z, y.w);
+}
+
 // Two floats as one register of 16-bit operands (bf16 for a bf16 cache, else fp16).
 template <bool kBf16> __device__ inline uint32_t pack(float lo, float hi) {
     if constexpr (kBf16) {
@@ -142,15 +156,14 @@ template <int CT, bool kQ32, int DP, int NT> struct Shape {
     static constexpr int EB = CT == MT_F32 ? 4 : CT == MT_F16 || CT == MT_BF16 ? 2 : 1;
     static constexpr bool kScaled = EB == 1, kBf16 = CT == MT_BF16;
     // The matrix pipe truncates what it adds to an accumulator, so a long chain of products
-    // drifts. For 32-bit outputs chains are short (4 steps of a score, 16 tokens of O) and
+    // drifts. For 32-bit outputs chains are short (4 steps of a score, one tile of O) and
     // are added up in fp32, rounded to nearest.
     static constexpr bool kExact = kQ32;
     static constexpr int ROW = DP * EB;               // bytes of a (padded) cache row
     static constexpr int CPR = ROW / 16;              // its 16-byte pieces
-    static constexpr int NW = ROW >= 1024 ? 2 : 4;    // warps a block
-    static constexpr int KT = 16 * NW;                // tokens a unit
-    static constexpr int STAGE = 32 * ROW + (kScaled ? 128 : 0);  // 16 rows of K, of V, their scales
-    static constexpr int S = ROW <= 128 ? 4 : 3;      // stages
+    // tokens a tile: 8-bit rows are short, and a tile's chain of instructions takes as long
+    static constexpr int TW = kScaled ? 32 : 16, TB = TW / 16;
+    static constexpr int STAGE = 2 * TW * ROW + (kScaled ? 2 * TW * 4 : 0);  // rows of K, of V, their scales
     static constexpr int KS = CT == MT_F32 ? DP / 8 : DP / 16;    // steps of K Q^T
     // pieces of a query: fp16 11 bits, bf16 8 bits, tf32 11 bits each
     static constexpr int QP = CT == MT_F32 ? 2 : !kQ32 ? 1 : kBf16 ? 3 : 2;
@@ -158,13 +171,21 @@ template <int CT, bool kQ32, int DP, int NT> struct Shape {
     static constexpr bool kNormed = CT != MT_F32 && !kBf16 && (kQ32 || kScaled);
     // fp16 probabilities are held times 2^15: the smallest, 2^-24, is 2^-39 of the largest
     static constexpr float kOffset = CT == MT_F16 || kScaled ? 15.0f : 0.0f;
-    static constexpr bool kQReg = KS * 2 * NT * QP <= 64;         // queries in registers, else in shared memory
+    // A part's queries come into shared memory as they are, while the part before is worked
+    // on; then they stay in registers as operands, or, where O leaves too few, in shared memory.
+    // Those that are operands as they are (one piece) need no second place, and come late.
+    static constexpr bool kQReg = KS * 2 * NT * QP + DP / 4 * NT <= 168, kQRaw = !kQReg && QP == 1 && !kNormed;
     static constexpr int ROWS = NT * 8;
-    static constexpr int Q_BYTES = KS * NT * QP * 256;
-    static constexpr int SMALL = NW * S * 16 + NW * ROWS * 8 + ROWS * 4 + 64;
-    static constexpr int SMEM = NW * S * STAGE + Q_BYTES + SMALL;
-    static constexpr int kFit = 227 * 1024 / (SMEM + 1024);
+    static constexpr int QROW = DP * (kQ32 ? 4 : 2) + 16;  // 8 rows' words of a column in different banks
+    static constexpr int Q_BYTES = ROWS * QROW + (kQReg || kQRaw ? 0 : KS * NT * QP * 256);
+    static constexpr int warp_bytes(int stages) { return stages * STAGE + (Q_BYTES + 127) / 128 * 128 + 128; }
+    static constexpr int kMost = 226 * 1024;          // of shared memory a block
+    static constexpr int NW = ROW < 1024 && 4 * warp_bytes(2) <= kMost ? 4 : 2;  // warps a block
+    static constexpr int S = ROW * TW <= 2048 ? 4 : NW * warp_bytes(3) <= kMost ? 3 : 2;  // stages
+    static constexpr int WARP = warp_bytes(S), SMEM = NW * WARP;
+    static constexpr int kFit = 228 * 1024 / (SMEM + 1024 + 256);  // with what the system and the scan take
     static constexpr int BLOCKS = kFit > 4 ? 4 : kFit < 1 ? 1 : kFit;  // resident blocks an SM
+    static_assert(SMEM <= kMost, "a block's shared memory");
 };
 
 // Where 16-byte piece c of row r lies, so that 8 rows' pieces of one column fall in
@@ -174,174 +195,245 @@ template <int CPR> __device__ inline int swizzled(int r, int c) {
     else return r * CPR + (c ^ (r / (8 / CPR) & (CPR - 1)));
 }
 
-// Where a block is on the line of units.
+// Where a warp is on the line of tiles.
 struct Cursor {
-    int b, begin, end, tiles, item, tile, next_length;
+    int b, begin, end, tiles, tile, next_length;
 };
 
-template <int KT> __device__ inline void enter_sequence(Cursor& c, const TileArgs& t, int length) {
-    const int n = min(max(length, 0), t.a.max_tokens);
-    c.end = n;
-    c.begin = n > t.a.window ? n - t.a.window : 0;
-    c.tiles = max(1, (n - c.begin + KT - 1) / KT);  // a sequence without tokens has one empty unit
-    c.next_length = c.b + 1 < t.a.batch ? t.a.lengths[(int64_t)(c.b + 1) * t.a.length_seq] : 0;
+// The tokens [begin, end) that a sequence of `length` shows, and its tiles (one, without
+// tokens, where there are none).
+template <int TW> __device__ inline void enter_sequence(Cursor& c, const TileArgs& t, int length) {
+    c.end = min(max(length, 0), t.a.max_tokens);
+    c.begin = c.end > t.a.window ? c.end - t.a.window : 0;
+    c.tiles = max(1, (c.end - c.begin + TW - 1) / TW);
+}
+__device__ inline int length_of(const TileArgs& t, int b) { return t.a.lengths[(int64_t)b * t.a.length_seq]; }
+
+// The cuts: every range gets tiles / ranges, the first ones one more.
+struct Ranges {
+    uint32_t base, more;
+    Ranges() = default;
+    __device__ Ranges(const TileArgs& t, int tiles) { base = t.ranges.div((uint32_t)tiles, &more); }
+    __device__ int first(uint32_t c) const { return (int)(c * base + min(c, more)); }
+    __device__ int owner(uint32_t u) const {
+        const uint32_t big = more * (base + 1);
+        return (int)(u < big ? u / (base + 1) : more + (u - big) / base);  // base is not 0 in the second
+    }
+};
+
+// Sums over the block of each thread's `mine`: all (total) and those of threads before it.
+template <int kThreads> __device__ inline int scan(int mine, int& total) {
+    __shared__ int sums[kThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int before = upto - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += sums[w];
+        total += sums[w];
+    }
+    return before;
+}
+
+// Finds the first tiles of ranges range_of(0) .. range_of(kCount - 1) (all threads of the block
+// call it): the caller's cursor is at the first tile of range_of(g). Returns how many tiles
+// that range has. Every thread sums some sequences' tiles; a scan over the sums finds the
+// sequence.
+template <int TW, int kThreads, int kCount, class RangeOf>
+__device__ inline int locate(const TileArgs& t, RangeOf range_of, int g, Cursor& c, Ranges& ranges) {
+    __shared__ int found[kCount][3];
+    const int per = (t.a.batch + kThreads - 1) / kThreads;
+    const int b0 = threadIdx.x * per, b1 = min(b0 + per, t.a.batch);
+    int mine = 0, length = 0, total;
+    for (int b = b0; b < b1; ++b) {
+        length = length_of(t, b);
+        enter_sequence<TW>(c, t, length);
+        mine += c.tiles;
+    }
+    const int before = scan<kThreads>(mine, total);
+    ranges = Ranges(t, total);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+        const int target = ranges.first(range_of(i));
+        int p = before;
+        if (p <= target && target < p + mine) {
+            int b = b0;
+            if (per > 1)
+                for (; b < b1; ++b) {
+                    length = length_of(t, b);
+                    enter_sequence<TW>(c, t, length);
+                    if (target < p + c.tiles) break;
+                    p += c.tiles;
+                }
+            found[i][0] = b;
+            found[i][1] = p;
+            found[i][2] = length;
+        }
+    }
+    __syncthreads();
+    const int u0 = ranges.first(range_of(g)), count = ranges.first(range_of(g) + 1) - u0;
+    if (count == 0) return 0;  // behind the end: nothing was found
+    c.b = found[g][0];
+    enter_sequence<TW>(c, t, found[g][2]);
+    c.tile = u0 - found[g][1];
+    return count;
 }
 
 template <int CT, class Q, int DP, int NT>
 __global__ void __launch_bounds__(Shape<CT, sizeof(Q) == 4, DP, NT>::NW * 32, Shape<CT, sizeof(Q) == 4, DP, NT>::BLOCKS)
 attention_tiles(const __grid_constant__ TileArgs t) {
     using Z = Shape<CT, sizeof(Q) == 4, DP, NT>;
-    constexpr int NW = Z::NW, KT = Z::KT, S = Z::S, CPR = Z::CPR, ROWS = Z::ROWS, QP = Z::QP, KS = Z::KS;
+    constexpr int NW = Z::NW, TW = Z::TW, TB = Z::TB, S = Z::S, CPR = Z::CPR, ROWS = Z::ROWS, QP = Z::QP, KS = Z::KS;
     constexpr bool kScaled = Z::kScaled, kBf16 = Z::kBf16;
     extern __shared__ __align__(128) unsigned char smem[];
     const AttentionArgs& a = t.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, oct = lane >> 2;
+    unsigned char* const ring = smem + warp * Z::WARP;
+    unsigned char* const sm_raw = ring + S * Z::STAGE;                    // queries as they are
+    uint2* const sm_q = (uint2*)(sm_raw + ROWS * Z::QROW);                // and as operands, where not in registers
+    int4* const sm_meta = (int4*)(ring + Z::WARP - 128);
 
-    unsigned char* const ring = smem + warp * (S * Z::STAGE);
-    uint2* const sm_q = (uint2*)(smem + NW * S * Z::STAGE);
-    int4* const sm_meta = (int4*)((unsigned char*)sm_q + Z::Q_BYTES) + warp * S;
-    float2* const sm_ml = (float2*)((unsigned char*)sm_q + Z::Q_BYTES + NW * S * 16);  // [NW][ROWS]
-    float* const sm_qscale = (float*)(sm_ml + NW * ROWS);
-    int64_t* const sm_start = (int64_t*)(sm_qscale + ROWS);  // total, prefix, sequence
-
-    asm volatile("griddepcontrol.launch_dependents;");
-
-    // -- this block's range of units: every thread sums some sequences' tiles, a scan finds
-    // the sequence that the range starts in
-    int64_t left;
+    const int me = blockIdx.x * NW + warp;
+    uint32_t item;
+    const int range = (int)t.per_range.div((uint32_t)me, &item);
+    uint32_t row_block;
+    const int kv_head = (int)t.row_blocks.div(item, &row_block);
+    const int head0 = kv_head * a.group + (int)row_block * ROWS, rows = min(ROWS, a.group - (int)row_block * ROWS);
     Cursor in;
-    {
-        const int per = (a.batch + NW * 32 - 1) / (NW * 32);
-        const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.batch);
-        int64_t mine = 0;
-        for (int b = b0; b < b1; ++b) {
-            const int n = min(max(a.lengths[(int64_t)b * a.length_seq], 0), a.max_tokens);
-            mine += max(1, (min(n, a.window) + KT - 1) / KT);
-        }
-        int64_t upto = mine;
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += o;
-        }
-        int64_t* const sums = (int64_t*)smem;  // per warp; the ring is not in use yet
-        if (lane == 31) sums[warp] = upto;
-        __syncthreads();
-        int64_t total = 0, before = 0;
-        for (int w = 0; w < NW; ++w) {
-            if (w < warp) before += sums[w];
-            total += sums[w];
-        }
-        const int64_t units = total * t.items;
-        const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-        left = u1 - u0;
-        int64_t p = before + upto - mine;
-        const int64_t target = u0 / t.items;
-        if (left > 0 && p <= target && target < p + mine) {
-            for (int b = b0; b < b1; ++b) {
-                const int n = min(max(a.lengths[(int64_t)b * a.length_seq], 0), a.max_tokens);
-                const int64_t tiles = max(1, (min(n, a.window) + KT - 1) / KT);
-                if (target < p + tiles) {
-                    sm_start[0] = p;
-                    sm_start[1] = b;
-                    break;
-                }
-                p += tiles;
-            }
-        }
-        __syncthreads();
-        if (left == 0) {
-            if (threadIdx.x == 0) t.meta[blockIdx.x] = make_int4(0, 0, kIdle, 0);
-            return;
-        }
-        in.b = (int)sm_start[1];
-        enter_sequence<KT>(in, t, a.lengths[(int64_t)in.b * a.length_seq]);
-        const int64_t within = u0 - sm_start[0] * t.items;
-        in.item = (int)(within / in.tiles);
-        in.tile = (int)(within % in.tiles);
+    int tiles;
+    if (t.whole) {
+        if (range >= a.batch) return;
+        in.b = range;
+        in.tile = 0;
+        enter_sequence<TW>(in, t, length_of(t, in.b));
+        tiles = in.tiles;
+    } else {
+        Ranges ranges;
+        tiles = locate<TW, NW * 32, NW>(t, [&](int i) { return t.per_range.div((uint32_t)(blockIdx.x * NW + i)); }, warp, in, ranges);
+        if (tiles <= 0 || range >= (int)t.ranges.d) return;
     }
-    const int units = (int)left;
+    in.next_length = in.b + 1 < a.batch ? length_of(t, in.b + 1) : 0;
 
-    // -- fetching: lane l < 16 finds token l's row of K, lane l + 16 its row of V
-    bool from_start = in.tile == 0, fresh = true;
-    int page_id = -1;
-    auto look_up = [&]() {
-        const int token = in.begin + in.tile * KT + warp * 16 + (lane & 15);
-        page_id = token < in.end ? a.tables[(int64_t)in.b * a.table_seq + a.page.div((uint32_t)token)] : -1;
+    // -- a tile to fetch. Lane l finds token l's rows of K and V (of 16 tokens, lane l + 16
+    // that of V).
+    struct Step {
+        int b, token, page, flags;  // page: -1 for no token
     };
-    look_up();
-    auto fetch = [&](int slot) {
-        unsigned char* const stage = ring + slot * Z::STAGE;
-        const uint32_t to = smem_address(stage);
-        const int token = in.begin + in.tile * KT + warp * 16 + (lane & 15);
-        const bool valid = token < in.end && page_id >= 0 && page_id < a.cache.pages;
-        const uint32_t mask = __ballot_sync(0xffffffffu, valid) & 0xffffu;
-        const int head = in.item / t.row_blocks;
-        uint32_t at = 0;
-        if (valid) a.page.div((uint32_t)token, &at);
-        const CacheView& c = lane < 16 ? a.cache.k : a.cache.v;
-        const unsigned char* row = (const unsigned char*)c.ptr;
-        if (valid) row += ((int64_t)page_id * c.page + (int64_t)at * c.token + (int64_t)head * c.head) * Z::EB;
-        if (lane == 0) {
-            const bool ends = in.tile + 1 == in.tiles, last = ends || left == 1;
-            sm_meta[slot] = make_int4(in.b, in.item, (int)mask, (fresh ? 1 : 0) | (last ? 2 : 0) | (from_start ? 4 : 0) | (ends ? 8 : 0));
+    constexpr int kFirst = 1, kLast = 2, kFromStart = 4, kEnds = 8, kMore = 16;  // of a part; its sequence's ends; parts follow
+    int left = tiles;
+    bool from_start = in.tile == 0, fresh = true;
+    auto look_up = [&]() {
+        Step s;
+        s.b = in.b;
+        s.token = in.begin + in.tile * TW + (lane & (TW - 1));
+        s.page = s.token < in.end ? a.tables[(int64_t)in.b * a.table_seq + a.page.div((uint32_t)s.token)] : -1;
+        const bool ends = in.tile + 1 == in.tiles;
+        s.flags = (fresh ? kFirst : 0) | (left > in.tiles - in.tile ? kMore : 0) | (ends || left == 1 ? kLast : 0) | (from_start ? kFromStart : 0) | (ends ? kEnds : 0);
+        --left;
+        fresh = false;
+        if (++in.tile == in.tiles) {
+            in.tile = 0;
+            fresh = from_start = true;
+            ++in.b;
+            enter_sequence<TW>(in, t, in.next_length);
+            in.next_length = in.b + 1 < a.batch ? length_of(t, in.b + 1) : 0;
         }
+        return s;
+    };
+    auto fetch = [&](const Step& s, int slot) {
+        const uint32_t to = smem_address(ring + slot * Z::STAGE);
+        const bool valid = s.page >= 0 && s.page < a.cache.pages;
+        const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+        uint32_t at = 0;
+        if (valid) a.page.div((uint32_t)s.token, &at);
+        auto row_of = [&](const CacheView& c, int bytes) {
+            const unsigned char* row = (const unsigned char*)c.ptr;
+            if (valid) row += ((int64_t)s.page * c.page + (int64_t)at * c.token + (int64_t)kv_head * c.head) * bytes;
+            return row;
+        };
+        const unsigned char *k_row, *v_row;
+        if constexpr (TW == 32) {
+            k_row = row_of(a.cache.k, Z::EB);
+            v_row = row_of(a.cache.v, Z::EB);
+        } else {
+            k_row = v_row = row_of(lane < 16 ? a.cache.k : a.cache.v, Z::EB);
+        }
+        if (lane == 0) sm_meta[slot] = make_int4(s.b, s.flags, (int)mask, 0);
         if constexpr (kScaled) {
-            const CacheView& z = lane < 16 ? a.cache.k_scale : a.cache.v_scale;
-            const float* s = (const float*)z.ptr;
-            if (valid) s += (int64_t)page_id * z.page + (int64_t)at * z.token + (int64_t)head * z.head;
-            copy4(to + 32 * Z::ROW + lane * 4, s, valid);
+            copy4(to + 2 * TW * Z::ROW + lane * 4, row_of(a.cache.k_scale, 4), valid);
+            copy4(to + 2 * TW * Z::ROW + (32 + lane) * 4, row_of(a.cache.v_scale, 4), valid);
         }
         if (mask) {
 #pragma unroll
             for (int which = 0; which < 2; ++which)
 #pragma unroll
-                for (int i = 0; i < 16 * CPR / 32; ++i) {
+                for (int i = 0; i < TW * CPR / 32; ++i) {
                     const int r = (i * 32 + lane) / CPR, piece = (i * 32 + lane) % CPR;
-                    const unsigned char* from =
-                        (const unsigned char*)__shfl_sync(0xffffffffu, (unsigned long long)row, r + 16 * which);
+                    const unsigned char* from = (const unsigned char*)__shfl_sync(
+                        0xffffffffu, (unsigned long long)(which ? v_row : k_row), r + (TW == 16 ? 16 * which : 0));
                     const bool real = piece < t.row_chunks, there = mask >> r & 1;
-                    const uint32_t dst = to + which * 16 * Z::ROW + swizzled<CPR>(r, piece) * 16;
+                    const uint32_t dst = to + which * TW * Z::ROW + swizzled<CPR>(r, piece) * 16;
                     // absent tokens: V must be zeros (their probability is 0, and 0 * NaN is not);
                     // K's scores are replaced. Padding: K must be zeros, V's columns are not used.
                     if (which == 0 ? (there || !real) : real) copy16(dst, from + (real ? piece * 16 : 0), real && there);
                 }
         }
-        // on to the next unit
-        --left;
-        fresh = false;
-        if (left > 0) {
-            if (++in.tile == in.tiles) {
-                in.tile = 0;
-                fresh = from_start = true;
-                if (++in.item == t.items) {
-                    in.item = 0;
-                    ++in.b;
-                    enter_sequence<KT>(in, t, in.next_length);
-                }
-            }
-            look_up();
-        }
     };
 
-    // -- queries of a part as operands, in the order that the products take them: warp nt
-    // holds rows nt * 8 .. + 7, four lanes a row
-    auto stage_queries = [&](int b, int item) {
-        if (warp >= NT) return;
-        const int r = warp * 8 + oct, in_group = (item % t.row_blocks) * ROWS + r, dim = a.cache.head_dim;
-        const bool there = in_group < a.group;
-        const Q* q = (const Q*)a.q + (int64_t)b * a.q_seq + (int64_t)(item / t.row_blocks * a.group + (there ? in_group : 0)) * a.q_head;
-        float x[KS][CT == MT_F32 ? 2 : 4], top = 0.0f;
+    // -- a part's queries: asked for early, taken when it begins
+    auto ask_queries = [&](int b) {
+        const Q* const q = (const Q*)a.q + (int64_t)b * a.q_seq + (int64_t)head0 * a.q_head;
+        const uint32_t to = smem_address(sm_raw);
+        if (t.q_chunks)
+            for (int i = lane; i < rows * t.q_chunks; i += 32) {
+                const int r = i / t.q_chunks, piece = i - r * t.q_chunks;
+                copy16(to + r * Z::QROW + piece * 16, (const unsigned char*)(q + (int64_t)r * a.q_head) + piece * 16, true);
+            }
+        else
+            for (int i = lane; i < rows * a.cache.head_dim; i += 32) {
+                const int r = i / a.cache.head_dim, d = i - r * a.cache.head_dim;
+                ((Q*)(sm_raw + r * Z::QROW))[d] = q[(int64_t)r * a.q_head + d];
+            }
+    };
+    // in the order that the products take them: four lanes a row
+    uint2 qf[Z::kQReg ? KS : 1][NT][QP];
+    float qscale[NT][2];
+    auto lay_out = [&](int n, const Q* row, int dim) {
+        constexpr int XS = CT == MT_F32 ? 2 : 4;
+        float x[KS][XS];
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int i = 0; i < (CT == MT_F32 ? 2 : 4); ++i) {
+            for (int i = 0; i < XS; i += XS / 2) {
                 const int d = CT == MT_F32 ? k * 8 + quad + i * 4
-                              : kScaled ? k * 16 + quad * 4 + i : k * 16 + quad * 2 + (i & 1) + (i >> 1) * 8;
-                x[k][i] = there && d < dim ? (float)q[d] : 0.0f;
-                top = fmaxf(top, fabsf(x[k][i]));
+                              : kScaled ? k * 16 + quad * 4 + i : k * 16 + quad * 2 + i * 4;
+                if constexpr (CT == MT_F32) {
+                    x[k][i] = d < dim ? (float)row[d] : 0.0f;
+                } else {  // head_dim is even here
+                    float2 v = make_float2(0.0f, 0.0f);
+                    if (d < dim) {
+                        if constexpr (sizeof(Q) == 4) v = *(const float2*)(row + d);
+                        else v = unpack<std::is_same<Q, __nv_bfloat16>::value>(*(const uint32_t*)(row + d));
+                    }
+                    x[k][i] = v.x;
+                    x[k][i + 1] = v.y;
+                }
             }
         float factor = a.scale * kLog2e;
         if constexpr (Z::kNormed) {
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int i = 0; i < XS; ++i) top = fmaxf(top, fabsf(x[k][i]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^-e with 2^e <= top: exponents of both within fp32's normal range
@@ -351,73 +443,113 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[k][i] *= down;
+                for (int i = 0; i < XS; ++i) x[k][i] *= down;
         }
-        if (quad == 0) sm_qscale[r] = factor;
+        // row oct's factor, to the lanes that hold column oct of a product
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            if constexpr (CT == MT_F32) {
-                const uint32_t h0 = upper(x[k][0]), h1 = upper(x[k][1]);
-                sm_q[((k * NT + warp) * QP + 0) * 32 + lane] = make_uint2(h0, h1);
-                sm_q[((k * NT + warp) * QP + 1) * 32 + lane] =
-                    make_uint2(__float_as_uint(x[k][0] - __uint_as_float(h0)), __float_as_uint(x[k][1] - __uint_as_float(h1)));
-            } else {
+        for (int i = 0; i < 2; ++i) qscale[n][i] = __shfl_sync(0xffffffffu, factor, (quad * 2 + i) * 4);
 #pragma unroll
-                for (int p = 0; p < QP; ++p) {
-                    const uint32_t y0 = pack<kBf16>(x[k][0], x[k][1]), y1 = pack<kBf16>(x[k][2], x[k][3]);
-                    sm_q[((k * NT + warp) * QP + p) * 32 + lane] = make_uint2(y0, y1);
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int p = 0; p < QP; ++p) {
+                uint2 y;
+                if constexpr (CT == MT_F32) {
+                    if (p == 0) {
+                        y = make_uint2(upper(x[k][0]), upper(x[k][1]));
+                        x[k][0] -= __uint_as_float(y.x);
+                        x[k][1] -= __uint_as_float(y.y);
+                    } else {
+                        y = make_uint2(__float_as_uint(x[k][0]), __float_as_uint(x[k][1]));
+                    }
+                } else {
+                    y = make_uint2(pack<kBf16>(x[k][0], x[k][1]), pack<kBf16>(x[k][2], x[k][3]));
                     if (p + 1 < QP) {
-                        const float2 g0 = unpack<kBf16>(y0), g1 = unpack<kBf16>(y1);
+                        const float2 g0 = unpack<kBf16>(y.x), g1 = unpack<kBf16>(y.y);
                         x[k][0] -= g0.x;
                         x[k][1] -= g0.y;
                         x[k][2] -= g1.x;
                         x[k][3] -= g1.y;
                     }
                 }
+                if constexpr (Z::kQReg) qf[k][n][p] = y;
+                else sm_q[((k * NT + n) * QP + p) * 32 + lane] = y;  // read back by this lane alone
+            }
+    };
+    auto take_queries = [&]() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            Q* const row = (Q*)(sm_raw + (n * 8 + oct) * Z::QROW);
+            const int dim = n * 8 + oct < rows ? a.cache.head_dim : 0;  // behind it: zeros
+            if constexpr (Z::kQRaw) {
+                // products read the rows themselves: zeros where nothing was copied
+                for (int d = dim + quad; d < DP; d += 4) row[d] = Q(0.0f);
+                qscale[n][0] = qscale[n][1] = a.scale * kLog2e;
+            } else {
+                lay_out(n, row, dim);
             }
         }
     };
-    stage_queries(in.b, in.item);
-    const int first_item = in.item, first_b = in.b;
-    int first_kind = kNoPart;
+    auto query = [&](int k, int n, int p) {
+        if constexpr (Z::kQReg) {
+            return qf[k][n][p];
+        } else if constexpr (Z::kQRaw) {
+            const uint32_t* const w = (const uint32_t*)(sm_raw + (n * 8 + oct) * Z::QROW) + k * 8 + quad;
+            return make_uint2(w[0], w[4]);
+        } else {
+            return sm_q[((k * NT + n) * QP + p) * 32 + lane];
+        }
+    };
 
+    ask_queries(in.b);
+    // the first tiles' pages are looked up together
+    Step ahead[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (s < tiles) ahead[s] = look_up();
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) {
-        if (left > 0) fetch(s);
+        if (s < tiles) fetch(ahead[s], s);
         copies_commit();
     }
-    __syncthreads();  // queries
+    Step next = ahead[S - 1];
 
-    uint2 qf[Z::kQReg ? KS : 1][NT][QP];
-    float o[DP / 16][NT][4], m[NT][2], l[NT][2], qscale[NT][2];
+    float o[DP / 16][NT][4], m[NT][2], l[NT][2];
     float v_unit = 0.0f;  // O is in units of this power of two (8-bit caches)
-
-    int slot = 0;
-    for (int unit = 0; unit < units; ++unit) {
+    int slot = 0, in_part = S;  // tiles of this part so far
+    for (int tile = 0; tile < tiles; ++tile) {
         __syncwarp();
-        if (left > 0) fetch(slot == 0 ? S - 1 : slot - 1);
+        if (tile + S - 1 < tiles) {
+            fetch(next, slot == 0 ? S - 1 : slot - 1);
+            if (left > 0) next = look_up();
+        } else {
+            asm volatile("griddepcontrol.launch_dependents;");
+        }
         copies_commit();
         copies_wait<S - 1>();
         __syncwarp();
+        ++in_part;
         const int4 meta = sm_meta[slot];
         const uint32_t mask = (uint32_t)meta.z;
         unsigned char* const stage = ring + slot * Z::STAGE;
-        const uint32_t k_at = smem_address(stage), v_at = k_at + 16 * Z::ROW;
-        if (meta.w & 1) {
-            if constexpr (Z::kQReg)
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int p = 0; p < QP; ++p) qf[k][n][p] = sm_q[((k * NT + n) * QP + p) * 32 + lane];
+        const uint32_t k_at = smem_address(stage), v_at = k_at + TW * Z::ROW;
+        if (meta.y & kFirst) {
+            if (tile > 0) {
+                // asked for when the last part began; that copy is among those waited for once S tiles
+                // have passed
+                if (Z::kQRaw) ask_queries(meta.x);
+                if (Z::kQRaw || in_part <= S) copies_wait_all();
+                __syncwarp();
+            }
+            take_queries();
+            __syncwarp();
+            if (!Z::kQRaw && (meta.y & kMore)) ask_queries(meta.x + 1);
+            in_part = 1;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     m[n][i] = -INFINITY;
                     l[n][i] = 0.0f;
-                    qscale[n][i] = sm_qscale[n * 8 + quad * 2 + i];
                 }
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d)
@@ -428,72 +560,77 @@ attention_tiles(const __grid_constant__ TileArgs t) {
             v_unit = 1.17549435e-38f;  // 2^-126
         }
         if (mask) {
-            // S^T: c[0], c[1] are token oct, heads quad * 2 + 0, 1; c[2], c[3] token oct + 8
-            float s[NT][4], part[NT][4];
+            // S^T: s[.][.][0], [1] are token oct, heads quad * 2 + 0, 1; [2], [3] token oct + 8. The
+            // largest pieces' products go into `part` first where they are kept apart.
+            float s[TB][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[n][i] = part[n][i] = 0.0f;
-            auto query = [&](int k, int n, int p) {
-                return Z::kQReg ? qf[Z::kQReg ? k : 0][n][p] : sm_q[((k * NT + n) * QP + p) * 32 + lane];
-            };
-            // the largest pieces' products go into `part`, the others into s
-            auto times_queries = [&](int k, const uint32_t (&x)[4]) {
+            for (int b = 0; b < TB; ++b) {
+                float part[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int p = 0; p < QP; ++p) {
-                        const uint2 q = query(k, n, p);
-                        product<CT>(p == 0 && Z::kExact ? part[n] : s[n], x, q.x, q.y);
+                    for (int i = 0; i < 4; ++i) s[b][n][i] = part[n][i] = 0.0f;
+                auto times_queries = [&](int k, const uint32_t (&x)[4]) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int p = 0; p < QP; ++p) {
+                            const uint2 q = query(k, n, p);
+                            product<CT>(p == 0 && Z::kExact ? part[n] : s[b][n], x, q.x, q.y);
+                        }
+                    if constexpr (Z::kExact) {
+                        if (k % 4 == 3 || k == KS - 1) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    s[b][n][i] += part[n][i];
+                                    part[n][i] = 0.0f;
+                                }
+                        }
                     }
-                if constexpr (Z::kExact) {
-                    if (k % 4 == 3 || k == KS - 1) {
+                };
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                for (int c = 0; c < CPR / 2; ++c) {
+                    uint32_t r[4];
+                    load_matrices(r, k_at + swizzled<CPR>(b * 16 + (lane & 15), 2 * c + (lane >> 4)) * 16);
+                    if constexpr (CT == MT_F32) {
+                        uint32_t hi[4], lo[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                s[n][i] += part[n][i];
-                                part[n][i] = 0.0f;
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            hi[i] = upper(__uint_as_float(r[i]));
+                            lo[i] = __float_as_uint(__uint_as_float(r[i]) - __uint_as_float(hi[i]));
+                        }
+                        times_queries(c, hi);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const uint2 q = query(c, n, 0);
+                            product<CT>(s[b][n], lo, q.x, q.y);
+                        }
+                    } else if constexpr (kScaled) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t x[4] = {decode<CT, 0, 1>(r[2 * h]), decode<CT, 0, 1>(r[2 * h + 1]),
+                                                   decode<CT, 2, 3>(r[2 * h]), decode<CT, 2, 3>(r[2 * h + 1])};
+                            times_queries(2 * c + h, x);
+                        }
+                    } else {
+                        times_queries(c, r);
                     }
-                }
-            };
-#pragma unroll
-            for (int c = 0; c < CPR / 2; ++c) {
-                uint32_t r[4];
-                load_matrices(r, k_at + swizzled<CPR>(lane & 15, 2 * c + (lane >> 4)) * 16);
-                if constexpr (CT == MT_F32) {
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        hi[i] = upper(__uint_as_float(r[i]));
-                        lo[i] = __float_as_uint(__uint_as_float(r[i]) - __uint_as_float(hi[i]));
-                    }
-                    times_queries(c, hi);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint2 q = query(c, n, 0);
-                        product<CT>(s[n], lo, q.x, q.y);
-                    }
-                } else if constexpr (kScaled) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t x[4] = {decode<CT, 0, 1>(r[2 * h]), decode<CT, 0, 1>(r[2 * h + 1]),
-                                               decode<CT, 2, 3>(r[2 * h]), decode<CT, 2, 3>(r[2 * h + 1])};
-                        times_queries(2 * c + h, x);
-                    }
-                } else {
-                    times_queries(c, r);
                 }
             }
-            float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f}, shrink = 1.0f;
+            float ks[TB][2], vs[TB][2], shrink = 1.0f;
             if constexpr (kScaled) {
-                const float* z = (const float*)(stage + 32 * Z::ROW);
-                ks[0] = z[oct];
-                ks[1] = z[oct + 8];
-                vs[0] = z[16 + oct];
-                vs[1] = z[16 + oct + 8];
-                float top = fmaxf(fabsf(vs[0]), fabsf(vs[1]));
+                const float* z = (const float*)(stage + 2 * TW * Z::ROW);
+                float top = 0.0f;
+#pragma unroll
+                for (int b = 0; b < TB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        ks[b][h] = z[b * 16 + h * 8 + oct];
+                        vs[b][h] = z[32 + b * 16 + h * 8 + oct];
+                        top = fmaxf(top, fabsf(vs[b][h]));
+                    }
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                 // the power of two above the largest scale so far
@@ -502,54 +639,72 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     shrink = v_unit / unit;
                     v_unit = unit;
                 }
-                const float per = 1.0f / v_unit;
-                vs[0] *= per;
-                vs[1] *= per;
+                const float per = __uint_as_float((254u << 23) - __float_as_uint(v_unit));  // 1 / v_unit
+#pragma unroll
+                for (int b = 0; b < TB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) vs[b][h] *= per;
             }
-            const bool seen[2] = {(mask >> oct & 1) != 0, (mask >> (oct + 8) & 1) != 0};
-            uint32_t pf[NT][CT == MT_F32 ? 4 : 2 * QP];
+            uint32_t pf[TB][NT][CT == MT_F32 ? 4 : 2 * QP];
             bool grown = shrink != 1.0f;
             float keep[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float s0 = seen[0] ? s[n][i] * (qscale[n][i] * ks[0]) : -INFINITY;
-                    const float s1 = seen[1] ? s[n][2 + i] * (qscale[n][i] * ks[1]) : -INFINITY;
-                    float top = fmaxf(s0, s1);
+                    float top = m[n][i];
+#pragma unroll
+                    for (int b = 0; b < TB; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float& x = s[b][n][2 * h + i];
+                            x *= kScaled ? qscale[n][i] * ks[b][h] : qscale[n][i];
+                            if (!(mask >> (b * 16 + h * 8 + oct) & 1)) x = -INFINITY;
+                            top = fmaxf(top, x);
+                        }
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    top = fmaxf(top, m[n][i]);
                     const float base = top == -INFINITY ? 0.0f : top;
                     keep[n][i] = exp2_fast(m[n][i] - base);
                     grown |= top > m[n][i];
                     m[n][i] = top;
-                    const float p0 = exp2_fast(s0 - base + Z::kOffset), p1 = exp2_fast(s1 - base + Z::kOffset);
-                    l[n][i] = l[n][i] * keep[n][i] + (p0 + p1);
-                    s[n][i] = kScaled ? p0 * vs[0] : p0;
-                    s[n][2 + i] = kScaled ? p1 * vs[1] : p1;
-                }
-                if constexpr (CT == MT_F32) {
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t x = __float_as_uint(s[n][2 * h]), y = __float_as_uint(s[n][2 * h + 1]);
-                        const uint32_t low = transpose8x8(__byte_perm(x, y, 0x5410)), high = transpose8x8(__byte_perm(x, y, 0x7632));
-                        pf[n][2 * h] = __byte_perm(low, high, 0x5410);
-                        pf[n][2 * h + 1] = __byte_perm(low, high, 0x7632);
-                    }
-                } else {
-#pragma unroll
-                    for (int p = 0; p < QP; ++p)
+                    for (int b = 0; b < TB; ++b)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t y = pack<kBf16>(s[n][2 * h], s[n][2 * h + 1]);
-                            pf[n][2 * p + h] = transpose8x8(y);
-                            if (p + 1 < QP) {
-                                const float2 g = unpack<kBf16>(y);
-                                s[n][2 * h] -= g.x;
-                                s[n][2 * h + 1] -= g.y;
-                            }
+                            float& x = s[b][n][2 * h + i];
+                            x = exp2_fast(x - base + Z::kOffset);
+                            sum += x;
+                            if constexpr (kScaled) x *= vs[b][h];
                         }
+                    l[n][i] = l[n][i] * keep[n][i] + sum;
+                    if constexpr (kScaled) keep[n][i] *= shrink;
+                }
+#pragma unroll
+                for (int b = 0; b < TB; ++b) {
+                    if constexpr (CT == MT_F32) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t x = __float_as_uint(s[b][n][2 * h]), y = __float_as_uint(s[b][n][2 * h + 1]);
+                            const uint32_t low = transpose8x8(__byte_perm(x, y, 0x5410)), high = transpose8x8(__byte_perm(x, y, 0x7632));
+                            pf[b][n][2 * h] = __byte_perm(low, high, 0x5410);
+                            pf[b][n][2 * h + 1] = __byte_perm(low, high, 0x7632);
+                        }
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < QP; ++p)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t y = pack<kBf16>(s[b][n][2 * h], s[b][n][2 * h + 1]);
+                                pf[b][n][2 * p + h] = transpose8x8(y);
+                                if (p + 1 < QP) {
+                                    const float2 g = unpack<kBf16>(y);
+                                    s[b][n][2 * h] -= g.x;
+                                    s[b][n][2 * h + 1] -= g.y;
+                                }
+                            }
+                    }
                 }
             }
             if (!Z::kExact && __any_sync(0xffffffffu, grown)) {
@@ -558,19 +713,19 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[d][n][i] *= kScaled ? keep[n][i & 1] * shrink : keep[n][i & 1];
+                        for (int i = 0; i < 4; ++i) o[d][n][i] *= keep[n][i & 1];
             }
-            // O^T: rows are 16 dims, columns heads as above
+            // O^T: rows are 16 dims, columns heads as above. Where chains are kept short, a tile's
+            // product is added to the rescaled O.
             auto add_up = [&](int d, int n, const float (&x)[4]) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    o[d][n][i] = o[d][n][i] * (kScaled ? keep[n][i & 1] * shrink : keep[n][i & 1]) + x[i];
+                for (int i = 0; i < 4; ++i) o[d][n][i] = o[d][n][i] * keep[n][i & 1] + x[i];
             };
             if constexpr (CT == MT_F32) {
-                const float* v = (const float*)(stage + 16 * Z::ROW);
+                const float* v = (const float*)(stage + TW * Z::ROW);
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d) {
-                    float x16[NT][4] = {};
+                    float tile_o[NT][4] = {};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         // operand column j is token 8 h + 2 j, column j + 4 the one after: free of bank
@@ -585,234 +740,251 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const float p0 = __uint_as_float(pf[n][2 * h]), p1 = __uint_as_float(pf[n][2 * h + 1]);
+                            const float p0 = __uint_as_float(pf[0][n][2 * h]), p1 = __uint_as_float(pf[0][n][2 * h + 1]);
                             const uint32_t h0 = upper(p0), h1 = upper(p1);
-                            product<CT>(x16[n], lo, h0, h1);
-                            product<CT>(x16[n], hi, __float_as_uint(p0 - __uint_as_float(h0)),
+                            product<CT>(tile_o[n], lo, h0, h1);
+                            product<CT>(tile_o[n], hi, __float_as_uint(p0 - __uint_as_float(h0)),
                                         __float_as_uint(p1 - __uint_as_float(h1)));
-                            product<CT>(x16[n], hi, h0, h1);
+                            product<CT>(tile_o[n], hi, h0, h1);
                         }
                     }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) add_up(d, n, x16[n]);
-                }
-            } else if constexpr (kScaled) {
-#pragma unroll
-                for (int c = 0; c < CPR / 2; ++c) {
-                    uint32_t r[4];
-                    load_transposed(r, v_at + swizzled<CPR>(lane & 15, 2 * c + (lane >> 4)) * 16);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        // bytes 0, 2 are two tokens' even dim, bytes 1, 3 their odd one
-                        const uint32_t x[4] = {decode<CT, 0, 2>(r[2 * h]), decode<CT, 1, 3>(r[2 * h]),
-                                               decode<CT, 0, 2>(r[2 * h + 1]), decode<CT, 1, 3>(r[2 * h + 1])};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float x16[4] = {};
-#pragma unroll
-                            for (int p = QP - 1; p >= 0; --p)
-                                product<CT>(Z::kExact ? x16 : o[2 * c + h][n], x, pf[n][2 * p], pf[n][2 * p + 1]);
-                            if constexpr (Z::kExact) add_up(2 * c + h, n, x16);
-                        }
-                    }
+                    for (int n = 0; n < NT; ++n) add_up(d, n, tile_o[n]);
                 }
             } else {
+                // 16 dims of 16-bit rows are two pieces, of 8-bit ones one
 #pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    uint32_t r[4];
-                    load_transposed(r, v_at + swizzled<CPR>((lane & 7) + (lane >> 4) * 8, 2 * d + (lane >> 3 & 1)) * 16);
+                for (int c = 0; c < CPR / 2; ++c) {
+                    uint32_t r[TB][4];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float x16[4] = {};
+                    for (int b = 0; b < TB; ++b)
+                        load_transposed(r[b], kScaled ? v_at + swizzled<CPR>(b * 16 + (lane & 15), 2 * c + (lane >> 4)) * 16
+                                                      : v_at + swizzled<CPR>((lane & 7) + (lane >> 4) * 8, 2 * c + (lane >> 3 & 1)) * 16);
 #pragma unroll
-                        for (int p = QP - 1; p >= 0; --p)
-                            product<CT>(Z::kExact ? x16 : o[d][n], r, pf[n][2 * p], pf[n][2 * p + 1]);
-                        if constexpr (Z::kExact) add_up(d, n, x16);
+                    for (int h = 0; h < (kScaled ? 2 : 1); ++h) {
+                        const int d = kScaled ? 2 * c + h : c;
+                        float tile_o[NT][4] = {};
+#pragma unroll
+                        for (int b = 0; b < TB; ++b) {
+                            // 8 bits: bytes 0, 2 are two tokens' even dim, bytes 1, 3 their odd one
+                            uint32_t x[4];
+                            if constexpr (kScaled) {
+                                x[0] = decode<CT, 0, 2>(r[b][2 * h]);
+                                x[1] = decode<CT, 1, 3>(r[b][2 * h]);
+                                x[2] = decode<CT, 0, 2>(r[b][2 * h + 1]);
+                                x[3] = decode<CT, 1, 3>(r[b][2 * h + 1]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) x[i] = r[b][i];
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int p = QP - 1; p >= 0; --p)
+                                    product<CT>(Z::kExact ? tile_o[n] : o[d][n], x, pf[b][n][2 * p], pf[b][n][2 * p + 1]);
+                        }
+                        if constexpr (Z::kExact)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) add_up(d, n, tile_o[n]);
                     }
                 }
             }
         }
-        if (meta.w & 2) {
-            // -- the part ends: join the warps' (m, l, O). Each warp's O goes to its own stage of this
-            // unit, which nothing will be fetched into before the last barrier below.
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float sum = l[n][i];
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                    if (oct == 0) sm_ml[warp * ROWS + n * 8 + quad * 2 + i] = make_float2(m[n][i], sum);
-                }
-            __syncthreads();
-            const int item = meta.y, head0 = item / t.row_blocks * a.group + item % t.row_blocks * ROWS;
-            const int rows = min(ROWS, a.group - item % t.row_blocks * ROWS), dim = a.cache.head_dim;
-            const bool whole = (meta.w & 12) == 12;
-            const int part = blockIdx.x * 2 + (meta.w & 4 ? 1 : 0);
-            if (!(meta.w & 4)) first_kind = meta.w & 8 ? kEnd : kMiddle;
+        if (meta.y & kLast) {
+            // -- the part ends: from the accumulators' layout to rows by way of this tile's stage, into which
+            // nothing will be fetched before the next tile
+            __syncwarp();
+            const int dim = a.cache.head_dim;
+            const bool whole = (meta.y & kFromStart) && (meta.y & kEnds);
+            const int64_t part = (int64_t)me * 2 + (meta.y & kFromStart ? 1 : 0);
+            Q* const out = (Q*)a.out + (int64_t)meta.x * a.out_seq + (int64_t)head0 * a.out_head;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 if (n * 8 >= rows) break;
                 float* const mine = (float*)stage;  // [8][DP]
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int r = quad * 2 + i;
-                    float top = -INFINITY;
+                    float sum = l[n][i];
 #pragma unroll
-                    for (int w = 0; w < NW; ++w) top = fmaxf(top, sm_ml[w * ROWS + n * 8 + r].x);
-                    float f = m[n][i] == -INFINITY ? 0.0f : exp2_fast(m[n][i] - top);
+                    for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                    const bool none = m[n][i] == -INFINITY && sum == 0.0f;
+                    const int r = quad * 2 + i, row = n * 8 + r;
+                    float f = whole ? 1.0f / sum : 1.0f;
                     if constexpr (kScaled) f *= v_unit;
 #pragma unroll
                     for (int d = 0; d < DP / 16; ++d) {
                         const int d0 = 16 * d + (kScaled ? 2 * oct : oct), d1 = d0 + (kScaled ? 1 : 8);
-                        mine[r * DP + (d0 ^ quad * 8)] = o[d][n][i] * f;
-                        mine[r * DP + (d1 ^ quad * 8)] = o[d][n][2 + i] * f;
+                        mine[r * DP + (d0 ^ quad * 8)] = none ? 0.0f : o[d][n][i] * f;
+                        mine[r * DP + (d1 ^ quad * 8)] = none ? 0.0f : o[d][n][2 + i] * f;
                     }
-                }
-                __syncthreads();
-                for (int r = warp; r < 8 && n * 8 + r < rows; r += NW) {
-                    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < NW; ++w) top = fmaxf(top, sm_ml[w * ROWS + n * 8 + r].x);
-#pragma unroll
-                    for (int w = 0; w < NW; ++w) {
-                        const float2 ml = sm_ml[w * ROWS + n * 8 + r];
-                        sum += ml.x == -INFINITY ? ml.y : ml.y * exp2_fast(ml.x - top);
-                    }
-                    const bool none = top == -INFINITY && sum == 0.0f;
-                    const float per = none ? 0.0f : 1.0f / sum;
-                    for (int d = lane; d < dim; d += 32) {
-                        float x = 0.0f;
-#pragma unroll
-                        for (int w = 0; w < NW; ++w)
-                            x += ((const float*)(smem + w * (S * Z::STAGE) + slot * Z::STAGE))[r * DP + (d ^ (r >> 1) * 8)];
-                        if (whole)
-                            ((Q*)a.out)[(int64_t)meta.x * a.out_seq + (int64_t)(head0 + n * 8 + r) * a.out_head + d] =
-                                rounded<Q>(none ? 0.0f : x * per);
-                        else
-                            t.part_o[((int64_t)part * ROWS + n * 8 + r) * DP + d] = x;
-                    }
-                    if (lane == 0) {
+                    if (oct == 0 && row < rows) {
                         if (!whole)
-                            t.part_ml[(int64_t)part * ROWS + n * 8 + r] = make_float2(top, sum);
+                            t.part_ml[part * ROWS + row] = make_float2(m[n][i], sum);
                         else if (a.lse)
-                            a.lse[(int64_t)meta.x * a.lse_seq + (int64_t)(head0 + n * 8 + r) * a.lse_head] =
-                                (top + log2f(sum) - Z::kOffset) * kLn2;
+                            a.lse[(int64_t)meta.x * a.lse_seq + (int64_t)(head0 + row) * a.lse_head] =
+                                (m[n][i] + log2f(sum) - Z::kOffset) * kLn2;
                     }
                 }
-                if (n == NT - 1 || (n + 1) * 8 >= rows) {
-                    if (unit + 1 < units) {
-                        const int4 next = sm_meta[slot + 1 == S ? 0 : slot + 1];
-                        stage_queries(next.x, next.y);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8 * DP / 128; ++i) {
+                    const int r = (i * 32 + lane) / (DP / 4), d = (i * 32 + lane) % (DP / 4) * 4;
+                    if (n * 8 + r < rows) {
+                        const float4 y = *(const float4*)(mine + r * DP + (d ^ (r >> 1) * 8));
+                        if (!whole) {
+                            *(float4*)(t.part_o + (part * ROWS + n * 8 + r) * DP + d) = y;
+                        } else if (d < dim) {
+                            Q* const to = out + (int64_t)(n * 8 + r) * a.out_head + d;
+                            if (t.out_quads) {
+                                store4(to, y);
+                            } else {
+                                to[0] = rounded<Q>(y.x);
+                                if (d + 1 < dim) to[1] = rounded<Q>(y.y);
+                                if (d + 2 < dim) to[2] = rounded<Q>(y.z);
+                                if (d + 3 < dim) to[3] = rounded<Q>(y.w);
+                            }
+                        }
                     }
                 }
-                __syncthreads();
+                __syncwarp();
             }
         }
         if (++slot == S) slot = 0;
     }
-    copies_wait<0>();
-    if (threadIdx.x == 0) t.meta[blockIdx.x] = make_int4(first_b, first_item, first_kind, 0);
+    copies_wait_all();
 }
 
-// Joins the parts of heads that cuts crossed. Block (c, r): if the part that block c of
-// attention_tiles started in ended there, it is the last of a chain that goes back to the
-// block where that head began; row r of the chain's (m, l, O) becomes the output.
-constexpr int kJoinThreads = 128;
-
-template <class Q, int DP, int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) join_parts(const __grid_constant__ TileArgs t, float offset) {
-    extern __shared__ float weight[];  // of each part of the chain, then the first one's place
-    __shared__ float red[2][kJoinThreads / 32];
-    __shared__ int sm_first;
+// Joins the parts of sequences that cuts crossed: block (x, r) row r of an item whose tiles lie
+// in several ranges. Which ones is known from the lengths, so it is found out while
+// attention_tiles still runs. x / items is a sequence, or, where there are fewer ranges
+// than sequences, a range: it stands for the sequence that it starts in the middle of, if
+// that ends in it.
+template <class Q, int DP, int ROWS, int TW>
+__global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ TileArgs t, float offset, int by_sequence) {
+    constexpr int kLanes = DP / 4, kSide = 8, kJoinThreads = kLanes * kSide;  // threads a part, parts at a time
+    __shared__ float4 sm_o[kSide][kLanes];
+    __shared__ float2 sm_ml[kSide];
     const AttentionArgs& a = t.a;
-    const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r = blockIdx.y;
+    uint32_t item, row_block;
+    const int x = (int)t.per_range.div(blockIdx.x, &item);
+    const int head = (int)t.row_blocks.div(item, &row_block) * a.group + (int)row_block * ROWS + r;
+    if ((int)row_block * ROWS + r >= a.group) return;
+    int b, first, count;
+    Cursor c;
+    if (by_sequence) {
+        b = x;
+        int all = 0, before = 0;
+        for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) {
+            enter_sequence<TW>(c, t, length_of(t, i));
+            all += c.tiles;
+            if (i < b) before += c.tiles;
+        }
+        int total, begin;
+        scan<kJoinThreads>(all, total);
+        __syncthreads();
+        scan<kJoinThreads>(before, begin);
+        enter_sequence<TW>(c, t, length_of(t, b));
+        const Ranges ranges(t, total);
+        first = ranges.owner(begin);
+        count = ranges.owner(begin + c.tiles - 1) - first + 1;
+        if (count == 1) return;
+    } else {
+        Ranges ranges;
+        const int tiles = locate<TW, kJoinThreads, 1>(t, [&](int) { return x; }, 0, c, ranges);
+        if (tiles == 0 || c.tile == 0 || c.tiles - c.tile > tiles) return;
+        b = c.b;
+        first = ranges.owner(ranges.first(x) - c.tile);
+        count = x - first + 1;
+    }
+    const int lane = threadIdx.x % kLanes, side = threadIdx.x / kLanes;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 end = t.meta[c];
-    const int r = blockIdx.y, row_block = end.y % t.row_blocks;
-    if (end.z != kEnd || row_block * ROWS + r >= a.group) return;
-    // back to the block whose last part began the head
-    int first = -1;
-    for (int hi = c - 1; first < 0 && hi >= 0; hi -= kJoinThreads) {
-        const int p = hi - (int)threadIdx.x;
-        const int kind = p >= 0 ? t.meta[p].z : kMiddle;
-        if (threadIdx.x == 0) sm_first = -1;
-        __syncthreads();
-        if (kind == kNoPart || kind == kEnd) atomicMax(&sm_first, p);
-        __syncthreads();
-        first = sm_first;
-        __syncthreads();
-    }
-    if (first < 0) return;  // not reached: the first block's first part begins a head
-    const int count = c - first + 1;
-    auto place = [&](int i) { return (int64_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * ROWS + r; };
-    float top = -INFINITY;
-    for (int i = threadIdx.x; i < count; i += kJoinThreads)
-        if (i == 0 || t.meta[first + i].z != kIdle) top = fmaxf(top, t.part_ml[place(i)].x);
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) red[0][warp] = top;
-    __syncthreads();
+    // every side takes every kSide-th part, four at a time
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto take = [&](float2 ml, float4 x) {
+        const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2_fast(m - base), f = exp2_fast(ml.x - base);
+        // NaN scores leave m at -inf and l, o NaN: 0 * NaN passes them on
+        m = top;
+        l = l * keep + ml.y * f;
+        o.x = o.x * keep + x.x * f;
+        o.y = o.y * keep + x.y * f;
+        o.z = o.z * keep + x.z * f;
+        o.w = o.w * keep + x.w * f;
+    };
+    for (int i = side; i < count; i += 4 * kSide) {
+        float2 ml[4];
+        float4 x[4];
 #pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[0][w]);
-    float sum = 0.0f;
-    for (int i = threadIdx.x; i < count; i += kJoinThreads) {
-        float f = 0.0f;
-        if (i == 0 || t.meta[first + i].z != kIdle) {
-            const float2 ml = t.part_ml[place(i)];
-            f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : exp2_fast(ml.x - top);
-            sum += ml.y * f;
-        } else {
-            f = -1.0f;  // an idle block: its memory holds nothing
+        for (int j = 0; j < 4; ++j) {
+            const int part = i + j * kSide;
+            if (part < count) {
+                const int64_t row = (((int64_t)(first + part) * t.items + item) * 2 + (part == 0 ? 1 : 0)) * ROWS + r;
+                ml[j] = t.part_ml[row];
+                x[j] = *(const float4*)(t.part_o + row * DP + lane * 4);
+            }
         }
-        weight[i] = f;
-    }
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) red[1][warp] = sum;
-    __syncthreads();
-    sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[1][w];
-    const int head = end.y / t.row_blocks * a.group + row_block * ROWS + r;
-    const bool none = top == -INFINITY && sum == 0.0f;
-    const float per = none ? 0.0f : 1.0f / sum;
-    for (int d = threadIdx.x; d < a.cache.head_dim; d += kJoinThreads) {
-        float x = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < count; ++i) {
-            const float f = weight[i];
-            if (f >= 0.0f || f != f) x += f * t.part_o[place(i) * DP + d];
-        }
-        ((Q*)a.out)[(int64_t)end.x * a.out_seq + (int64_t)head * a.out_head + d] = rounded<Q>(none ? 0.0f : x * per);
+        for (int j = 0; j < 4; ++j)
+            if (i + j * kSide < count) take(ml[j], x[j]);
     }
-    if (threadIdx.x == 0 && a.lse)
-        a.lse[(int64_t)end.x * a.lse_seq + (int64_t)head * a.lse_head] = (top + log2f(sum) - offset) * kLn2;
+    sm_o[side][lane] = o;
+    if (lane == 0) sm_ml[side] = make_float2(m, l);
+    __syncthreads();
+    if (side != 0) return;
+#pragma unroll
+    for (int w = 1; w < kSide; ++w) take(sm_ml[w], sm_o[w][lane]);
+    const bool none = m == -INFINITY && l == 0.0f;
+    const float per = 1.0f / l;
+    const float y[4] = {o.x, o.y, o.z, o.w};
+    Q* out = (Q*)a.out + (int64_t)b * a.out_seq + (int64_t)head * a.out_head + lane * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (lane * 4 + i < a.cache.head_dim) out[i] = rounded<Q>(none ? 0.0f : y[i] * per);
+    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.lse_seq + (int64_t)head * a.lse_head] = (m + log2f(l) - offset) * kLn2;
 }
 
 // ---- launch ------------------------------------------------------------------------------------
 
 constexpr int kMaxDevices = 16;
+constexpr int kWholeTiles = 6;
 
 template <int CT, class Q, int DP, int NT>
-int launch(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
+int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
     using Z = Shape<CT, sizeof(Q) == 4, DP, NT>;
     TileArgs t;
     t.a = a;
-    t.row_blocks = (a.group + Z::ROWS - 1) / Z::ROWS;
-    t.items = a.cache.kv_heads * t.row_blocks;
+    const int row_blocks = (a.group + Z::ROWS - 1) / Z::ROWS;
+    t.row_blocks = FastDiv((uint32_t)row_blocks);
+    t.items = a.cache.kv_heads * row_blocks;
+    t.per_range = FastDiv((uint32_t)t.items);
     t.row_chunks = a.cache.head_dim * Z::EB / 16;
+    const int64_t q16 = 16 / (int)sizeof(Q);
+    t.q_chunks = a.cache.head_dim % q16 == 0 && (uintptr_t)a.q % 16 == 0 && a.q_seq % q16 == 0 && a.q_head % q16 == 0
+                     ? (int)(a.cache.head_dim / q16) : 0;
+    t.out_quads = a.cache.head_dim % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(Q)) == 0 && a.out_seq % 4 == 0 && a.out_head % 4 == 0;
     int sms;
     if (int rc = sm_count(dev, &sms)) return rc;
-    // as many blocks as fit the GPU at once, or fewer where there cannot be as many units
     const int64_t tokens = a.max_tokens < a.window ? a.max_tokens : a.window;
-    const int64_t most = (tokens + Z::KT - 1) / Z::KT, resident = (int64_t)sms * Z::BLOCKS;
-    int64_t blocks = (int64_t)a.batch * t.items * (most > 0 ? most : 1);
-    if (blocks > resident) blocks = resident;
-    const uint64_t meta_bytes = (uint64_t)blocks * 16, ml_bytes = (uint64_t)blocks * 2 * Z::ROWS * 8;
-    *bytes = meta_bytes + ml_bytes + (uint64_t)blocks * 2 * Z::ROWS * DP * 4;
-    if (!workspace) return 0;
-    t.meta = (int4*)workspace;
-    t.part_ml = (float2*)((char*)workspace + meta_bytes);
-    t.part_o = (float*)((char*)workspace + meta_bytes + ml_bytes);
+    const int64_t most = tokens > 0 ? (tokens + Z::TW - 1) / Z::TW : 1;
+    if (a.batch * most > INT32_MAX || (int64_t)a.batch * t.items > INT32_MAX - 64)
+        return bad_argument("paged_attention: the tables' width allows over 2^31 - 1 tiles of %d tokens", Z::TW);
+    // A range a sequence where none has more than a few tiles: that costs less than a join.
+    // Otherwise as many ranges as the warps that fit the GPU at once can take the heads of, or
+    // fewer where there cannot be as many tiles.
+    t.whole = most <= kWholeTiles;
+    int64_t ranges = (int64_t)sms * Z::BLOCKS * Z::NW / t.items;
+    if (ranges < 1) ranges = 1;
+    if (ranges > a.batch * most) ranges = a.batch * most;
+    if (t.whole) ranges = a.batch;
+    const int64_t warps = ranges * t.items, blocks = (warps + Z::NW - 1) / Z::NW;
+    const uint64_t ml_bytes = (uint64_t)warps * 2 * Z::ROWS * 8;
+    *bytes = t.whole ? 0 : ml_bytes + (uint64_t)warps * 2 * Z::ROWS * DP * 4;
+    if (!run) return 0;
+    t.ranges = FastDiv((uint32_t)ranges);
+    t.part_ml = (float2*)workspace;
+    t.part_o = (float*)((char*)workspace + ml_bytes);
     auto kernel = attention_tiles<CT, Q, DP, NT>;
     static bool ready[kMaxDevices] = {};
     if (!ready[dev]) {
@@ -821,26 +993,27 @@ int launch(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cu
     }
     kernel<<<(unsigned)blocks, Z::NW * 32, Z::SMEM, st>>>(t);
     RT_CHECK(cudaGetLastError());
+    if (t.whole) return 0;
+    const bool by_sequence = a.batch <= ranges;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks, a.group < Z::ROWS ? a.group : Z::ROWS);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.dynamicSmemBytes = (size_t)blocks * 4;
+    cfg.gridDim = dim3((unsigned)((by_sequence ? a.batch : ranges) * t.items), a.group < Z::ROWS ? a.group : Z::ROWS);
+    cfg.blockDim = dim3(DP * 2);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    RT_CHECK(cudaLaunchKernelEx(&cfg, join_parts<Q, DP, Z::ROWS>, (const TileArgs)t, Z::kOffset));
+    RT_CHECK(cudaLaunchKernelEx(&cfg, join_parts<Q, DP, Z::ROWS, Z::TW>, (const TileArgs)t, Z::kOffset, (int)by_sequence));
     return 0;
 }
 
-template <int CT, class Q> int by_shape(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
+template <int CT, class Q> int by_shape(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
     const int dim = a.cache.head_dim;
     const bool wide = a.group > 8;
-    if (dim <= 64) return wide ? launch<CT, Q, 64, 2>(a, workspace, bytes, dev, st) : launch<CT, Q, 64, 1>(a, workspace, bytes, dev, st);
-    if (dim <= 128) return wide ? launch<CT, Q, 128, 2>(a, workspace, bytes, dev, st) : launch<CT, Q, 128, 1>(a, workspace, bytes, dev, st);
-    return wide ? launch<CT, Q, 256, 2>(a, workspace, bytes, dev, st) : launch<CT, Q, 256, 1>(a, workspace, bytes, dev, st);
+    if (dim <= 64) return wide ? launch<CT, Q, 64, 2>(a, run, workspace, bytes, dev, st) : launch<CT, Q, 64, 1>(a, run, workspace, bytes, dev, st);
+    if (dim <= 128) return wide ? launch<CT, Q, 128, 2>(a, run, workspace, bytes, dev, st) : launch<CT, Q, 128, 1>(a, run, workspace, bytes, dev, st);
+    return wide ? launch<CT, Q, 256, 2>(a, run, workspace, bytes, dev, st) : launch<CT, Q, 256, 1>(a, run, workspace, bytes, dev, st);
 }
 
 }  // namespace tiles

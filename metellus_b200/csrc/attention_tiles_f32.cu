@@ -3,8 +3,8 @@
 
 namespace mt {
 
-int attend_tiles_f32(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
-    return tiles::by_shape<MT_F32, float>(a, workspace, bytes, dev, st);
+int attend_tiles_f32(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
+    return tiles::by_shape<MT_F32, float>(a, run, workspace, bytes, dev, st);
 }
 
 }  // namespace mt

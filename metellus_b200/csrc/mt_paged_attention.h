@@ -27,13 +27,13 @@ struct AttentionArgs {
 int attend_by_rows(const AttentionArgs& a, cudaStream_t st);
 
 // Rows of the cache that 16-byte copies can fetch: tiles on the matrix pipe
-// (attention_tiles.cuh), split over the sequences' lengths. `bytes`: the workspace needed;
-// with `workspace` null that is all that is found out.
-int attend_tiles_f32(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
-int attend_tiles_f16(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
-int attend_tiles_bf16(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
-int attend_tiles_i8(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
-int attend_tiles_e4m3(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+// (attention_tiles.cuh), split over the sequences' lengths. `bytes`: the workspace needed,
+// which is all that is found out unless `run`.
+int attend_tiles_f32(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_f16(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_bf16(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_i8(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
+int attend_tiles_e4m3(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st);
 
 }  // namespace mt
 

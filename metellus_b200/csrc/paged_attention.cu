@@ -47,13 +47,13 @@ int check_attention(const char* who, const mt_array* q, const mt_paged_cache* ca
     return 0;
 }
 
-int attend_tiles(const AttentionArgs& a, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
+int attend_tiles(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
     switch (a.cache.dtype) {
-        case MT_F32: return attend_tiles_f32(a, workspace, bytes, dev, st);
-        case MT_F16: return attend_tiles_f16(a, workspace, bytes, dev, st);
-        case MT_BF16: return attend_tiles_bf16(a, workspace, bytes, dev, st);
-        case MT_I8: return attend_tiles_i8(a, workspace, bytes, dev, st);
-        default: return attend_tiles_e4m3(a, workspace, bytes, dev, st);
+        case MT_F32: return attend_tiles_f32(a, run, workspace, bytes, dev, st);
+        case MT_F16: return attend_tiles_f16(a, run, workspace, bytes, dev, st);
+        case MT_BF16: return attend_tiles_bf16(a, run, workspace, bytes, dev, st);
+        case MT_I8: return attend_tiles_i8(a, run, workspace, bytes, dev, st);
+        default: return attend_tiles_e4m3(a, run, workspace, bytes, dev, st);
     }
 }
 
@@ -74,7 +74,7 @@ int mt_paged_attention_workspace(int dev, const mt_array* q, const mt_paged_cach
     if (!bytes) return bad_argument("%s: bytes is missing", who);
     if (int rc = check_attention(who, q, cache, tables, window, &a, &batch, &heads, &tiled)) return rc;
     *bytes = 0;
-    return batch == 0 || !tiled ? 0 : attend_tiles(a, nullptr, bytes, dev, nullptr);
+    return batch == 0 || !tiled ? 0 : attend_tiles(a, false, nullptr, bytes, dev, nullptr);
 }
 
 int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
@@ -115,12 +115,12 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
     if (int rc = call_stream(dev, stream, &st)) return rc;
     if (!tiled) return attend_by_rows(a, st);
     uint64_t need = 0;
-    if (int rc = attend_tiles(a, nullptr, &need, dev, st)) return rc;
-    if (!workspace || workspace_bytes < need)
+    if (int rc = attend_tiles(a, false, nullptr, &need, dev, st)) return rc;
+    if (need && (!workspace || workspace_bytes < need))
         return bad_argument("%s: the workspace has %llu bytes, %llu are needed", who,
                             (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)need);
     if ((uintptr_t)workspace % 16) return bad_argument("%s: the workspace is not 16-byte aligned", who);
-    return attend_tiles(a, workspace, &need, dev, st);
+    return attend_tiles(a, true, workspace, &need, dev, st);
 }
 
 }  // extern "C"

@@ -192,6 +192,16 @@ def test_attention(q_type, dtype, lengths, heads, kv_heads, dim, ps):
     compare(*make(lengths, heads, kv_heads, dim, ps, q_type, dtype))
 
 
+@pytest.mark.parametrize("q_type,dtype", [(F32, F32), (BF16, BF16), (BF16, I8), (F16, F16)])
+@pytest.mark.parametrize("batch,longest,extra_width", [(300, 400, 2), (700, 40, 0), (700, 40, 900), (1, 40000, 0), (1, 300, 5000),
+                                                       (2, 70, 20)])
+def test_attention_batches(q_type, dtype, batch, longest, extra_width):
+    """More sequences than threads, more items than blocks, fewer units than blocks."""
+    lengths = torch.randint(0, longest + 1, (batch,)).tolist()
+    lengths[0] = longest
+    compare(*make(lengths, 6, 3, 64, 16, q_type, dtype, extra_width=extra_width))
+
+
 @pytest.mark.parametrize("q_type,dtype", [(F32, F32), (BF16, BF16), (F32, I8), (F16, E4M3)])
 @pytest.mark.parametrize("dim", [1, 7, 36, 100, 200, 250])
 def test_attention_odd_head_dims(q_type, dtype, dim):
