@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -19,6 +20,7 @@ PKG = Path(__file__).resolve().parent.parent
 REPO = PKG.parent
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libmetellus_cuda.so"
+PAGED = LIB_DIR / "_metellus_paged.so"   # the Python binding of the paged cache's operators
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -42,6 +44,7 @@ def build_backend(force: bool = False, verbose: bool = False) -> Path:
     LIB_DIR.mkdir(exist_ok=True)
     newest = max(newest_header, *(s.stat().st_mtime for s in sources()))
     if not force and LIB.exists() and LIB.stat().st_mtime >= newest:
+        build_binding(force, verbose)
         return LIB
     obj_dir = PKG / "csrc" / "_build"
     obj_dir.mkdir(exist_ok=True)
@@ -67,7 +70,22 @@ def build_backend(force: bool = False, verbose: bool = False) -> Path:
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
+    build_binding(force, verbose)
     return LIB
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """The CPython extension over the library's paged-cache entry points."""
+    src, header = PKG / "csrc" / "python_paged.cpp", REPO / "include" / "metellus_b200.h"
+    if not force and PAGED.exists() and PAGED.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+        return PAGED
+    cmd = [nvcc(), "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-I", str(REPO / "include"),
+           "-I", sysconfig.get_paths()["include"], "-o", str(PAGED), str(src), "-cudart", "none",
+           "-L", str(LIB_DIR), "-lmetellus_cuda", "-Xlinker=-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    return PAGED
 
 
 if __name__ == "__main__":
