@@ -152,7 +152,8 @@ template <int CT, int kLo, int kHi> __device__ inline uint32_t decode(uint32_t x
 
 // ---- shapes --------------------------------------------------------------------------------
 
-template <int CT, bool kQ32, int DP, int NT> struct Shape {
+template <int CT, class Q, int DP, int NT> struct Shape {
+    static constexpr bool kQ32 = sizeof(Q) == 4;
     static constexpr int EB = CT == MT_F32 ? 4 : CT == MT_F16 || CT == MT_BF16 ? 2 : 1;
     static constexpr bool kScaled = EB == 1, kBf16 = CT == MT_BF16;
     // The matrix pipe truncates what it adds to an accumulator, so a long chain of products
@@ -167,6 +168,8 @@ template <int CT, bool kQ32, int DP, int NT> struct Shape {
     static constexpr int KS = CT == MT_F32 ? DP / 8 : DP / 16;    // steps of K Q^T
     // pieces of a query: fp16 11 bits, bf16 8 bits, tf32 11 bits each
     static constexpr int QP = CT == MT_F32 ? 2 : !kQ32 ? 1 : kBf16 ? 3 : 2;
+    // pieces of a probability: enough that the output's own rounding is what shows
+    static constexpr int PP = CT == MT_F32 ? 2 : kQ32 ? QP : kScaled && std::is_same<Q, __nv_bfloat16>::value ? 1 : 2;
     // queries that fp16 may not hold are divided by a power of two per row
     static constexpr bool kNormed = CT != MT_F32 && !kBf16 && (kQ32 || kScaled);
     // fp16 probabilities are held times 2^15: the smallest, 2^-24, is 2^-39 of the largest
@@ -288,10 +291,10 @@ __device__ inline int locate(const TileArgs& t, RangeOf range_of, int g, Cursor&
 }
 
 template <int CT, class Q, int DP, int NT>
-__global__ void __launch_bounds__(Shape<CT, sizeof(Q) == 4, DP, NT>::NW * 32, Shape<CT, sizeof(Q) == 4, DP, NT>::BLOCKS)
+__global__ void __launch_bounds__(Shape<CT, Q, DP, NT>::NW * 32, Shape<CT, Q, DP, NT>::BLOCKS)
 attention_tiles(const __grid_constant__ TileArgs t) {
-    using Z = Shape<CT, sizeof(Q) == 4, DP, NT>;
-    constexpr int NW = Z::NW, TW = Z::TW, TB = Z::TB, S = Z::S, CPR = Z::CPR, ROWS = Z::ROWS, QP = Z::QP, KS = Z::KS;
+    using Z = Shape<CT, Q, DP, NT>;
+    constexpr int NW = Z::NW, TW = Z::TW, TB = Z::TB, S = Z::S, CPR = Z::CPR, ROWS = Z::ROWS, QP = Z::QP, PP = Z::PP, KS = Z::KS;
     constexpr bool kScaled = Z::kScaled, kBf16 = Z::kBf16;
     extern __shared__ __align__(128) unsigned char smem[];
     const AttentionArgs& a = t.a;
@@ -645,7 +648,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) vs[b][h] *= per;
             }
-            uint32_t pf[TB][NT][CT == MT_F32 ? 4 : 2 * QP];
+            uint32_t pf[TB][NT][2 * PP];
             bool grown = shrink != 1.0f;
             float keep[NT][2];
 #pragma unroll
@@ -693,12 +696,12 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         }
                     } else {
 #pragma unroll
-                        for (int p = 0; p < QP; ++p)
+                        for (int p = 0; p < PP; ++p)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const uint32_t y = pack<kBf16>(s[b][n][2 * h], s[b][n][2 * h + 1]);
                                 pf[b][n][2 * p + h] = transpose8x8(y);
-                                if (p + 1 < QP) {
+                                if (p + 1 < PP) {
                                     const float2 g = unpack<kBf16>(y);
                                     s[b][n][2 * h] -= g.x;
                                     s[b][n][2 * h + 1] -= g.y;
@@ -780,7 +783,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int p = QP - 1; p >= 0; --p)
+                                for (int p = PP - 1; p >= 0; --p)
                                     product<CT>(Z::kExact ? tile_o[n] : o[d][n], x, pf[b][n][2 * p], pf[b][n][2 * p + 1]);
                         }
                         if constexpr (Z::kExact)
@@ -952,7 +955,7 @@ constexpr int kWholeTiles = 6;
 
 template <int CT, class Q, int DP, int NT>
 int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
-    using Z = Shape<CT, sizeof(Q) == 4, DP, NT>;
+    using Z = Shape<CT, Q, DP, NT>;
     TileArgs t;
     t.a = a;
     const int row_blocks = (a.group + Z::ROWS - 1) / Z::ROWS;

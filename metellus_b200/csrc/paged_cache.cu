@@ -1,8 +1,9 @@
 // Writing a paged key-value cache and reading it back (mt_cache_write, mt_cache_read).
 //
-// One warp a row (one token's head, of K or of V): the row stays in registers between
-// the pass that finds its largest magnitude and the one that stores its codes, so HBM
-// sees each element once each way.
+// HBM alone bounds both: each element is read once and written once, and between the two a
+// row (one token's head, of K or of V) stays in registers: 8 elements a thread, head_dim / 8
+// threads a row, two rows at a time so that enough loads are in flight. Rows that cannot be
+// moved in pieces of 8 elements take a warp each, element by element.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -141,6 +142,7 @@ struct RowArgs {
     int64_t slot_stride;
     int slots64;
     int total_slots, head_dim, first, count;  // which of k, v: first .. first + count - 1
+    int pieces;                               // rows can be moved 8 elements at a time
     int64_t row_count;                         // tokens * heads
     FastDiv heads, page;
 };
@@ -154,36 +156,117 @@ template <> __device__ inline float from_float<float>(float x) { return x; }
 template <> __device__ inline __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-template <class C> struct Code;
-
-// The code nearest to x / s, ties to even. x / s in fp32 can be rounded onto a border
-// between two codes, so the nearest integer n to it is checked by the remainder
-// x - n s, which one fma gives exactly: more than half of s means the other neighbour.
+// The multiple of s nearest to x, ties to even, from t, which is x / s up to a few ulps (|t| <
+// 2^21). The remainder x - n s is exact in one fma, so it tells whether n is the nearest: a
+// quotient in fp32 alone can be rounded onto, or over, the border between two codes.
 __device__ inline float nearest_multiple(float x, float s, float t) {
-    float n = rintf(t);
-    const float r = fmaf(-n, s, x), twice = 2.0f * fabsf(r);
-    if (twice > s || (twice == s && fmodf(n, 2.0f) != 0.0f)) n += copysignf(1.0f, r);
-    return n;
+    const float big = 12582912.0f;  // 1.5 * 2^23: its ulp is 1
+    const float shifted = t + big, n = shifted - big, r = fmaf(-n, s, x), twice = 2.0f * fabsf(r);
+    const bool odd = __float_as_uint(shifted) & 1;
+    return twice > s || (twice == s && odd) ? n + copysignf(1.0f, r) : n;
 }
 
+// Codes of a row whose scale is s (not 0): `per` is 1 / s, or 0 where s is so small that this
+// is no number (then x / s is taken as it is).
+template <class C> struct Code;
 template <> struct Code<int8_t> {
     static constexpr float kLargest = 127.0f;
-    static __device__ int8_t of(float x, float s) {
-        const float n = nearest_multiple(x, s, x / s);
-        return (int8_t)fminf(fmaxf(n, -127.0f), 127.0f);
+    static __device__ int number(float x, float s, float per) {
+        const float n = nearest_multiple(x, s, per != 0.0f ? x * per : x / s);
+        return (int)fminf(fmaxf(n, -127.0f), 127.0f);
+    }
+    static __device__ int8_t of(float x, float s, float per) { return (int8_t)number(x, s, per); }
+    static __device__ uint2 pack8(const float* x, float s, float per) {
+        int n[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n[i] = number(x[i], s, per);
+        uint2 y;
+        y.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+        y.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
+        return y;
+    }
+    static __device__ void unpack8(uint2 y, float* x) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // 2^23 + (code + 128), less 2^23 + 128
+            const uint32_t w = (i < 4 ? y.x : y.y) ^ 0x80808080u;
+            x[i] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 | i % 4)) - 8388736.0f;
+        }
     }
 };
 template <> struct Code<__nv_fp8_e4m3> {
     static constexpr float kLargest = 448.0f;
-    static __device__ __nv_fp8_e4m3 of(float x, float s) {
-        const float t = x / s;
+    static __device__ float number(float x, float s, float per) {
+        const float t = per != 0.0f ? x * per : x / s;
         // the spacing of e4m3 around t: 2^(exponent - 3), at least 2^-9
-        const int e = max((int)(__float_as_uint(t) >> 23 & 0xff) - 127, -6) - 3;
-        const float u = __uint_as_float((uint32_t)(e + 127) << 23);
-        const float per = __uint_as_float((uint32_t)(127 - e) << 23);
-        return __nv_fp8_e4m3(nearest_multiple(x, s * u, t * per) * u);
+        const int e = max((int)(__float_as_uint(t) >> 23 & 0xff), 121) - 3;
+        const float u = __uint_as_float((uint32_t)e << 23), inverse = __uint_as_float((uint32_t)(254 - e) << 23);
+        return nearest_multiple(x, s * u, t * inverse) * u;
+    }
+    static __device__ __nv_fp8_e4m3 of(float x, float s, float per) { return __nv_fp8_e4m3(number(x, s, per)); }
+    static __device__ uint2 pack8(const float* x, float s, float per) {
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            h[i] = __nv_cvt_float2_to_fp8x2(make_float2(number(x[2 * i], s, per), number(x[2 * i + 1], s, per)),
+                                            __NV_SATFINITE, __NV_E4M3);
+        return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+    static __device__ void unpack8(uint2 y, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? y.x : y.y) >> (i % 2 * 16)), __NV_E4M3);
+            const float2 f = __half22float2(*(const __half2*)&h);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
     }
 };
+
+// A row's scale from the bits of its largest magnitude (as bits, magnitudes order like
+// numbers, with infinities and NaN on top), and its reciprocal.
+template <class C> __device__ inline float scale_of(uint32_t top, float* per) {
+    const float s = top < 0x7f800000u ? __uint_as_float(top) / Code<C>::kLargest : __uint_as_float(0x7fc00000u);
+    *per = s > 1e-30f ? 1.0f / s : 0.0f;
+    return s;
+}
+
+// 8 elements from and to memory
+__device__ inline void load8(const float* p, float* x) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ inline void load8(const __half* p, float* x) {
+    const uint4 a = *(const uint4*)p;
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*(const __half2*)&w[i]);
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+}
+__device__ inline void load8(const __nv_bfloat16* p, float* x) {
+    const uint4 a = *(const uint4*)p;
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ inline void store8(float* p, const float* x) {
+    *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+    *(float4*)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ inline void store8(__half* p, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(__half2*)&w[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ inline void store8(__nv_bfloat16* p, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(__nv_bfloat162*)&w[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 __device__ inline int64_t slot_of(const RowArgs& a, int64_t token) {
     return a.slots64 ? ((const int64_t*)a.slots)[token * a.slot_stride]
@@ -197,8 +280,9 @@ __device__ inline int64_t cache_offset(const CacheView& c, uint32_t page, uint32
 constexpr int kRowThreads = 256;
 constexpr int kPerLane = kMaxHeadDim / 32;
 
-template <class X, class C, bool kScaled>
+template <class X, class C>
 __global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a) {
+    constexpr bool kScaled = sizeof(C) == 1;
     const int lane = threadIdx.x & 31, which = a.first + blockIdx.y;
     const int64_t stride = (int64_t)gridDim.x * (kRowThreads / 32);
     for (int64_t row = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5); row < a.row_count; row += stride) {
@@ -214,19 +298,18 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a)
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) v[i] = lane + 32 * i < a.head_dim ? to_float(x[lane + 32 * i]) : 0.0f;
         if constexpr (kScaled) {
-            // as bits, magnitudes order like numbers, with infinities and NaN on top
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i) top = max(top, __float_as_uint(fabsf(v[i])));
             top = __reduce_max_sync(0xffffffffu, top);
-            const bool finite = top < 0x7f800000u;
-            const float s = finite ? __uint_as_float(top) / Code<C>::kLargest : __uint_as_float(0x7fc00000u);
+            float per;
+            const float s = scale_of<C>(top, &per);
             if (lane == 0)
                 ((float*)a.scale[which].ptr)[cache_offset(a.scale[which], page, at, head)] = s;
-            const bool none = !finite || s == 0.0f;
+            const bool none = !(s > 0.0f);
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i)
-                if (lane + 32 * i < a.head_dim) c[lane + 32 * i] = none ? C(0.0f) : Code<C>::of(v[i], s);
+                if (lane + 32 * i < a.head_dim) c[lane + 32 * i] = none ? C(0.0f) : Code<C>::of(v[i], s, per);
         } else {
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i)
@@ -235,8 +318,9 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a)
     }
 }
 
-template <class X, class C, bool kScaled>
+template <class X, class C>
 __global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) {
+    constexpr bool kScaled = sizeof(C) == 1;
     const int lane = threadIdx.x & 31, which = a.first + blockIdx.y;
     const int64_t stride = (int64_t)gridDim.x * (kRowThreads / 32);
     for (int64_t row = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5); row < a.row_count; row += stride) {
@@ -259,26 +343,134 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) 
     }
 }
 
-template <class X, class C>
-int launch_rows(bool write, const RowArgs& a, int blocks, cudaStream_t st) {
+// The same in pieces of 8 elements: kThreads threads (a power of two) a row, the first
+// head_dim / 8 of them with a piece.
+constexpr int kAtOnce = 2;  // rows
+
+template <class X, class C, int kThreads>
+__global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs a) {
     constexpr bool kScaled = sizeof(C) == 1;
-    const dim3 grid(blocks, a.count);
+    constexpr int kGroups = kRowThreads / kThreads;
+    const int which = a.first + blockIdx.y, piece = threadIdx.x % kThreads, d = piece * 8;
+    const bool mine = d < a.head_dim;
+    const uint32_t step = gridDim.x * kGroups, count = (uint32_t)a.row_count;
+    const X* const rows = (const X*)a.rows[which].ptr + d;
+    // every thread of a warp takes every turn: rows' threads exchange their largest elements
+    for (uint32_t base = blockIdx.x * kGroups; base < count; base += kAtOnce * step) {
+        float x[kAtOnce][8];
+        uint32_t token[kAtOnce], head[kAtOnce];
+        int64_t slot[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const uint32_t row = base + i * step + threadIdx.x / kThreads;
+            const bool there = row < count;
+            token[i] = a.heads.div(there ? row : 0, &head[i]);
+            slot[i] = there ? slot_of(a, token[i]) : -1;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
+            if (there && mine) load8(rows + (int64_t)token[i] * a.rows[which].token + (int64_t)head[i] * a.rows[which].head, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const bool there = slot[i] >= 0 && slot[i] < a.total_slots;
+            uint32_t at;
+            const uint32_t page = a.page.div(there ? (uint32_t)slot[i] : 0, &at);
+            C* const c = (C*)a.cache[which].ptr + cache_offset(a.cache[which], page, at, head[i]) + d;
+            if constexpr (kScaled) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(fabsf(x[i][k])));
+#pragma unroll
+                for (int k = 1; k < kThreads; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+                float per;
+                const float s = scale_of<C>(top, &per);
+                if (there && piece == 0) ((float*)a.scale[which].ptr)[cache_offset(a.scale[which], page, at, head[i])] = s;
+                if (there && mine) *(uint2*)c = s > 0.0f ? Code<C>::pack8(x[i], s, per) : make_uint2(0, 0);
+            } else {
+                if (there && mine) store8(c, x[i]);
+            }
+        }
+    }
+}
+
+template <class X, class C, int kThreads>
+__global__ void __launch_bounds__(kRowThreads) cache_read_pieces(const RowArgs a) {
+    constexpr bool kScaled = sizeof(C) == 1;
+    constexpr int kGroups = kRowThreads / kThreads;
+    const int which = a.first + blockIdx.y, d = (int)(threadIdx.x % kThreads) * 8;
+    if (d >= a.head_dim) return;
+    const uint32_t step = gridDim.x * kGroups, count = (uint32_t)a.row_count;
+    for (uint32_t base = blockIdx.x * kGroups + threadIdx.x / kThreads; base < count; base += kAtOnce * step) {
+        uint32_t token[kAtOnce], head[kAtOnce], at[kAtOnce], page[kAtOnce];
+        bool there[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const uint32_t row = base + i * step;
+            token[i] = a.heads.div(row < count ? row : 0, &head[i]);
+            const int64_t slot = slot_of(a, token[i]);
+            there[i] = row < count && slot >= 0 && slot < a.total_slots;
+            page[i] = a.page.div(there[i] ? (uint32_t)slot : 0, &at[i]);
+        }
+        float x[kAtOnce][8];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
+            if (!there[i]) continue;
+            const C* const c = (const C*)a.cache[which].ptr + cache_offset(a.cache[which], page[i], at[i], head[i]) + d;
+            if constexpr (kScaled) {
+                const float s = ((const float*)a.scale[which].ptr)[cache_offset(a.scale[which], page[i], at[i], head[i])];
+                Code<C>::unpack8(*(const uint2*)c, x[i]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[i][k] *= s;
+            } else {
+                load8(c, x[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (base + i * step < count)
+                store8((X*)a.rows[which].ptr + (int64_t)token[i] * a.rows[which].token + (int64_t)head[i] * a.rows[which].head + d, x[i]);
+    }
+}
+
+template <class X, class C, int kThreads>
+int launch_pieces(bool write, const RowArgs& a, int sms, cudaStream_t st) {
+    const int64_t groups = kRowThreads / kThreads, want = (a.row_count + groups - 1) / groups;
+    const dim3 grid((unsigned)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8), a.count);
     if (write)
-        cache_write_rows<X, C, kScaled><<<grid, kRowThreads, 0, st>>>(a);
+        cache_write_pieces<X, C, kThreads><<<grid, kRowThreads, 0, st>>>(a);
     else
-        cache_read_rows<X, C, kScaled><<<grid, kRowThreads, 0, st>>>(a);
+        cache_read_pieces<X, C, kThreads><<<grid, kRowThreads, 0, st>>>(a);
+    RT_CHECK(cudaGetLastError());
+    return 0;
+}
+
+template <class X, class C>
+int launch_rows(bool write, const RowArgs& a, int sms, cudaStream_t st) {
+    if (a.pieces) {
+        if (a.head_dim <= 64) return launch_pieces<X, C, 8>(write, a, sms, st);
+        if (a.head_dim <= 128) return launch_pieces<X, C, 16>(write, a, sms, st);
+        return launch_pieces<X, C, 32>(write, a, sms, st);
+    }
+    const int64_t want = (a.row_count + kRowThreads / 32 - 1) / (kRowThreads / 32);
+    const dim3 grid((unsigned)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8), a.count);
+    if (write)
+        cache_write_rows<X, C><<<grid, kRowThreads, 0, st>>>(a);
+    else
+        cache_read_rows<X, C><<<grid, kRowThreads, 0, st>>>(a);
     RT_CHECK(cudaGetLastError());
     return 0;
 }
 
 template <class X>
-int launch_cache_type(int dtype, bool write, const RowArgs& a, int blocks, cudaStream_t st) {
+int launch_cache_type(int dtype, bool write, const RowArgs& a, int sms, cudaStream_t st) {
     switch (dtype) {
-        case MT_F32: return launch_rows<X, float>(write, a, blocks, st);
-        case MT_F16: return launch_rows<X, __half>(write, a, blocks, st);
-        case MT_BF16: return launch_rows<X, __nv_bfloat16>(write, a, blocks, st);
-        case MT_I8: return launch_rows<X, int8_t>(write, a, blocks, st);
-        default: return launch_rows<X, __nv_fp8_e4m3>(write, a, blocks, st);
+        case MT_F32: return launch_rows<X, float>(write, a, sms, st);
+        case MT_F16: return launch_rows<X, __half>(write, a, sms, st);
+        case MT_BF16: return launch_rows<X, __nv_bfloat16>(write, a, sms, st);
+        case MT_I8: return launch_rows<X, int8_t>(write, a, sms, st);
+        default: return launch_rows<X, __nv_fp8_e4m3>(write, a, sms, st);
     }
 }
 
@@ -291,6 +483,7 @@ int move_rows(const char* who, bool write, int dev, const mt_array* k, const mt_
     if (int rc = check_array(who, "slots", slots, 1, 1u << MT_I32 | 1u << MT_I64, false)) return rc;
     RowArgs a{};
     int dtype = -1;
+    bool pieces = c.head_dim % 8 == 0;
     for (int i = 0; i < 2; ++i) {
         const mt_array* x = i ? v : k;
         const char* name = i ? "v" : "k";
@@ -306,7 +499,10 @@ int move_rows(const char* who, bool write, int dev, const mt_array* k, const mt_
         if (!write)
             if (int rc = check_written(who, name, *x)) return rc;
         a.rows[i] = {x->ptr, x->strides[0], x->strides[1]};
+        const int align = 8 * bytes_of(c.dtype) < 16 ? 8 : 16;
+        pieces = pieces && rows_aligned(*x, 16) && rows_aligned(i ? cache->v : cache->k, align);
     }
+    a.pieces = pieces;
     a.first = k ? 0 : 1;
     a.count = (k ? 1 : 0) + (v ? 1 : 0);
     const int64_t tokens = slots->shape[0];
@@ -331,12 +527,10 @@ int move_rows(const char* who, bool write, int dev, const mt_array* k, const mt_
     if (int rc = call_stream(dev, stream, &st)) return rc;
     int sms;
     if (int rc = sm_count(dev, &sms)) return rc;
-    const int64_t want = (a.row_count + kRowThreads / 32 - 1) / (kRowThreads / 32);
-    const int blocks = (int)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8);
     switch (dtype) {
-        case MT_F32: return launch_cache_type<float>(c.dtype, write, a, blocks, st);
-        case MT_F16: return launch_cache_type<__half>(c.dtype, write, a, blocks, st);
-        default: return launch_cache_type<__nv_bfloat16>(c.dtype, write, a, blocks, st);
+        case MT_F32: return launch_cache_type<float>(c.dtype, write, a, sms, st);
+        case MT_F16: return launch_cache_type<__half>(c.dtype, write, a, sms, st);
+        default: return launch_cache_type<__nv_bfloat16>(c.dtype, write, a, sms, st);
     }
 }
 
