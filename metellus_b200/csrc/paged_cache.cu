@@ -1,12 +1,14 @@
 // Writing a paged key-value cache and reading it back (mt_cache_write, mt_cache_read).
 //
 // HBM alone bounds both: each element is read once and written once, and between the two a
-// row (one token's head, of K or of V) stays in registers: 8 elements a thread, head_dim / 8
-// threads a row, two rows at a time so that enough loads are in flight. Rows that cannot be
-// moved in pieces of 8 elements take a warp each, element by element.
+// token's head stays in registers, its rows of K and of V together: 16 elements a thread,
+// head_dim / 16 threads a row, so that a row's addresses cost little beside its elements. Rows that
+// cannot be moved 8 elements at a time take a warp each, element by element.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "mt_paged.h"
 
@@ -142,7 +144,7 @@ struct RowArgs {
     int64_t slot_stride;
     int slots64;
     int total_slots, head_dim, first, count;  // which of k, v: first .. first + count - 1
-    int pieces;                               // rows can be moved 8 elements at a time
+    int pieces;                               // rows can be moved 8 elements at a time (cache_*_pieces)
     int64_t row_count;                         // tokens * heads
     FastDiv heads, page;
 };
@@ -156,18 +158,24 @@ template <> __device__ inline float from_float<float>(float x) { return x; }
 template <> __device__ inline __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// The multiple of s nearest to x, ties to even, from t, which is x / s up to a few ulps (|t| <
-// 2^21). The remainder x - n s is exact in one fma, so it tells whether n is the nearest: a
-// quotient in fp32 alone can be rounded onto, or over, the border between two codes.
+// A row's codes. x / s in fp32 can be rounded onto, or over, the border between two codes, so
+// the nearest code is found in two ways:
+//
+// * quick(): from t = x * per, which is x / s up to a few ulps, unless t is next to a border (a part
+//   in 2^13 or less of all values): then `close` is set.
+// * number(): from the remainder x - n s of the candidate n, which one fma gives exactly. More than
+//   half of s, or half of it and n odd: the other neighbour is nearer, or even.
+//
+// `per` is 1 / s, or 0 where s is so small that this may not be a number; then x / s is taken as
+// it is. s is not 0.
+constexpr float kBig = 12582912.0f;  // 1.5 * 2^23: its ulp is 1, so adding it rounds to whole numbers
+
 __device__ inline float nearest_multiple(float x, float s, float t) {
-    const float big = 12582912.0f;  // 1.5 * 2^23: its ulp is 1
-    const float shifted = t + big, n = shifted - big, r = fmaf(-n, s, x), twice = 2.0f * fabsf(r);
+    const float shifted = t + kBig, n = shifted - kBig, r = fmaf(-n, s, x), twice = 2.0f * fabsf(r);
     const bool odd = __float_as_uint(shifted) & 1;
     return twice > s || (twice == s && odd) ? n + copysignf(1.0f, r) : n;
 }
 
-// Codes of a row whose scale is s (not 0): `per` is 1 / s, or 0 where s is so small that this
-// is no number (then x / s is taken as it is).
 template <class C> struct Code;
 template <> struct Code<int8_t> {
     static constexpr float kLargest = 127.0f;
@@ -176,22 +184,27 @@ template <> struct Code<int8_t> {
         return (int)fminf(fmaxf(n, -127.0f), 127.0f);
     }
     static __device__ int8_t of(float x, float s, float per) { return (int8_t)number(x, s, per); }
-    static __device__ uint2 pack8(const float* x, float s, float per) {
-        int n[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) n[i] = number(x[i], s, per);
-        uint2 y;
-        y.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
-        y.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
-        return y;
+    static __device__ uint32_t bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
     }
-    static __device__ void unpack8(uint2 y, float* x) {
+    static __device__ uint32_t quick4(const float* x, float per, bool& close) {
+        uint32_t y[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // 2^23 + (code + 128), less 2^23 + 128
-            const uint32_t w = (i < 4 ? y.x : y.y) ^ 0x80808080u;
-            x[i] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 | i % 4)) - 8388736.0f;
+        for (int i = 0; i < 4; ++i) {
+            const float shifted = fmaf(x[i], per, kBig), n = shifted - kBig;
+            // |t| < 128: t and this distance are good to 2^-15
+            close |= fabsf(fmaf(x[i], per, -n)) > 0.5f - 0x1p-14f;
+            y[i] = __float_as_uint(shifted);  // its low byte is n's
         }
+        return bytes(y[0], y[1], y[2], y[3]);
+    }
+    static __device__ uint32_t pack4(const float* x, float s, float per) {
+        return bytes(number(x[0], s, per), number(x[1], s, per), number(x[2], s, per), number(x[3], s, per));
+    }
+    static __device__ void unpack4(uint32_t y, float* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // 2^23 + (code + 128), less 2^23 + 128
+            x[i] = __uint_as_float(__byte_perm(y ^ 0x80808080u, 0x4B000000u, 0x7540 | i)) - 8388736.0f;
     }
 };
 template <> struct Code<__nv_fp8_e4m3> {
@@ -204,18 +217,30 @@ template <> struct Code<__nv_fp8_e4m3> {
         return nearest_multiple(x, s * u, t * inverse) * u;
     }
     static __device__ __nv_fp8_e4m3 of(float x, float s, float per) { return __nv_fp8_e4m3(number(x, s, per)); }
-    static __device__ uint2 pack8(const float* x, float s, float per) {
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            h[i] = __nv_cvt_float2_to_fp8x2(make_float2(number(x[2 * i], s, per), number(x[2 * i + 1], s, per)),
-                                            __NV_SATFINITE, __NV_E4M3);
-        return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    static __device__ uint32_t codes(const float* t) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[0], t[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[2], t[3]), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
     }
-    static __device__ void unpack8(uint2 y, float* x) {
+    static __device__ uint32_t quick4(const float* x, float per, bool& close) {
+        float t[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? y.x : y.y) >> (i % 2 * 16)), __NV_E4M3);
+            t[i] = x[i] * per;
+            // a border of normal codes has its 20 bits behind the third fraction bit at 0x80000; t
+            // is good to 4 ulps. Below 2^-6 the spacing is another, and 0 needs no look.
+            close |= ((__float_as_uint(t[i]) + (4u - 0x80000u)) & 0xfffffu) <= 8u || (fabsf(t[i]) < 0x1p-6f && t[i] != 0.0f);
+        }
+        return codes(t);
+    }
+    static __device__ uint32_t pack4(const float* x, float s, float per) {
+        const float t[4] = {number(x[0], s, per), number(x[1], s, per), number(x[2], s, per), number(x[3], s, per)};
+        return codes(t);
+    }
+    static __device__ void unpack4(uint32_t y, float* x) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(y >> (i * 16)), __NV_E4M3);
             const float2 f = __half22float2(*(const __half2*)&h);
             x[2 * i] = f.x;
             x[2 * i + 1] = f.y;
@@ -231,42 +256,110 @@ template <class C> __device__ inline float scale_of(uint32_t top, float* per) {
     return s;
 }
 
-// 8 elements from and to memory
-__device__ inline void load8(const float* p, float* x) {
-    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-__device__ inline void load8(const __half* p, float* x) {
-    const uint4 a = *(const uint4*)p;
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*(const __half2*)&w[i]);
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+// Two 16-bit elements as a word.
+template <class T> __device__ inline uint32_t word(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return reinterpret_cast<const uint32_t&>(v);
+    } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return reinterpret_cast<const uint32_t&>(v);
     }
 }
-__device__ inline void load8(const __nv_bfloat16* p, float* x) {
-    const uint4 a = *(const uint4*)p;
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+template <class T> __device__ inline float2 floats(uint32_t w) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(reinterpret_cast<const __half2&>(w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// A thread's 16 elements of a row, from and to memory, in runs whose neighbours belong to the
+// next thread, so that a warp's accesses are of whole lines: runs of 4 where that fills 16
+// bytes on one side, else of 8.
+constexpr int kElements = 16;
+
+template <int kThreads, int kRun> struct Piece {
+    static constexpr int kRuns = kElements / kRun;
+    int lane;
+    __device__ int at(int run) const { return (run * kThreads + lane) * kRun; }
+
+    __device__ void load(const float* p, int dim, float* x) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-}
-__device__ inline void store8(float* p, const float* x) {
-    *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
-    *(float4*)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ inline void store8(__half* p, const float* x) {
-    uint32_t w[4];
+        for (int i = 0; i < kRuns; ++i)
+            if (at(i) < dim) {
+                const float4 a = *(const float4*)(p + at(i));
+                x[4 * i] = a.x, x[4 * i + 1] = a.y, x[4 * i + 2] = a.z, x[4 * i + 3] = a.w;
+            }
+    }
+    __device__ void store(float* p, int dim, const float* x) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *(__half2*)&w[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ inline void store8(__nv_bfloat16* p, const float* x) {
-    uint32_t w[4];
+        for (int i = 0; i < kRuns; ++i)
+            if (at(i) < dim) *(float4*)(p + at(i)) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    }
+    // 16-bit elements: two to a word
+    template <class T> __device__ void load(const T* p, int dim, float* x) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *(__nv_bfloat162*)&w[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
-}
+        for (int i = 0; i < kRuns; ++i)
+            if (at(i) < dim) {
+                uint32_t w[kRun / 2];
+                if constexpr (kRun == 4) {
+                    const uint2 a = *(const uint2*)(p + at(i));
+                    w[0] = a.x, w[1] = a.y;
+                } else {
+                    const uint4 a = *(const uint4*)(p + at(i));
+                    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+                }
+#pragma unroll
+                for (int k = 0; k < kRun / 2; ++k) {
+                    const float2 f = floats<T>(w[k]);
+                    x[kRun * i + 2 * k] = f.x, x[kRun * i + 2 * k + 1] = f.y;
+                }
+            }
+    }
+    template <class T> __device__ void store(T* p, int dim, const float* x) const {
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+            if (at(i) < dim) {
+                uint32_t w[kRun / 2];
+#pragma unroll
+                for (int k = 0; k < kRun / 2; ++k) w[k] = word<T>(x[kRun * i + 2 * k], x[kRun * i + 2 * k + 1]);
+                if constexpr (kRun == 4) *(uint2*)(p + at(i)) = make_uint2(w[0], w[1]);
+                else *(uint4*)(p + at(i)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+    }
+    template <class C> __device__ void store_codes(C* p, int dim, const float* x, float s, float per) const {
+        uint32_t w[kElements / 4] = {};
+        if (s > 0.0f) {
+            bool close = per == 0.0f;
+#pragma unroll
+            for (int k = 0; k < kElements / 4; ++k) w[k] = Code<C>::quick4(x + 4 * k, per, close);
+            if (close) {
+#pragma unroll
+                for (int k = 0; k < kElements / 4; ++k) w[k] = Code<C>::pack4(x + 4 * k, s, per);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+            if (at(i) < dim) {
+                if constexpr (kRun == 4) *(uint32_t*)(p + at(i)) = w[i];
+                else *(uint2*)(p + at(i)) = make_uint2(w[2 * i], w[2 * i + 1]);
+            }
+    }
+    template <class C> __device__ void load_codes(const C* p, int dim, float* x) const {
+#pragma unroll
+        for (int i = 0; i < kRuns; ++i)
+            if (at(i) < dim) {
+                uint32_t w[kRun / 4];
+                if constexpr (kRun == 4) {
+                    w[0] = *(const uint32_t*)(p + at(i));
+                } else {
+                    const uint2 a = *(const uint2*)(p + at(i));
+                    w[0] = a.x, w[1] = a.y;
+                }
+#pragma unroll
+                for (int k = 0; k < kRun / 4; ++k) Code<C>::unpack4(w[k], x + kRun * i + 4 * k);
+            }
+    }
+};
+template <class X, class C, int kThreads> using PieceOf = Piece<kThreads, sizeof(X) == 4 || sizeof(C) == 4 ? 4 : 8>;
 
 __device__ inline int64_t slot_of(const RowArgs& a, int64_t token) {
     return a.slots64 ? ((const int64_t*)a.slots)[token * a.slot_stride]
@@ -343,51 +436,43 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) 
     }
 }
 
-// The same in pieces of 8 elements: kThreads threads (a power of two) a row, the first
-// head_dim / 8 of them with a piece.
-constexpr int kAtOnce = 2;  // rows
-
+// The same in pieces of 16 elements: kThreads threads (a power of two) a row, its rows of K
+// and of V together.
 template <class X, class C, int kThreads>
 __global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs a) {
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
-    const int which = a.first + blockIdx.y, piece = threadIdx.x % kThreads, d = piece * 8;
-    const bool mine = d < a.head_dim;
-    const uint32_t step = gridDim.x * kGroups, count = (uint32_t)a.row_count;
-    const X* const rows = (const X*)a.rows[which].ptr + d;
-    // every thread of a warp takes every turn: rows' threads exchange their largest elements
-    for (uint32_t base = blockIdx.x * kGroups; base < count; base += kAtOnce * step) {
-        float x[kAtOnce][8];
-        uint32_t token[kAtOnce], head[kAtOnce];
-        int64_t slot[kAtOnce];
+    const PieceOf<X, C, kThreads> piece{(int)(threadIdx.x % kThreads)};
+    const uint32_t count = (uint32_t)a.row_count;
+    // every thread of a warp takes every turn: a row's threads exchange their largest elements
+    for (uint32_t base = blockIdx.x * kGroups; base < count; base += gridDim.x * kGroups) {
+        const uint32_t row = base + threadIdx.x / kThreads;
+        uint32_t head, at;
+        const uint32_t token = a.heads.div(row < count ? row : 0, &head);
+        const int64_t slot = row < count ? slot_of(a, token) : -1;
+        float x[2][kElements] = {};
+        if (row < count)
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            const uint32_t row = base + i * step + threadIdx.x / kThreads;
-            const bool there = row < count;
-            token[i] = a.heads.div(there ? row : 0, &head[i]);
-            slot[i] = there ? slot_of(a, token[i]) : -1;
+            for (int i = 0; i < 2; ++i)
+                piece.load((const X*)a.rows[i].ptr + (int64_t)token * a.rows[i].token + (int64_t)head * a.rows[i].head, a.head_dim, x[i]);
+        const bool there = slot >= 0 && slot < a.total_slots;
+        const uint32_t page = a.page.div(there ? (uint32_t)slot : 0, &at);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
-            if (there && mine) load8(rows + (int64_t)token[i] * a.rows[which].token + (int64_t)head[i] * a.rows[which].head, x[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            const bool there = slot[i] >= 0 && slot[i] < a.total_slots;
-            uint32_t at;
-            const uint32_t page = a.page.div(there ? (uint32_t)slot[i] : 0, &at);
-            C* const c = (C*)a.cache[which].ptr + cache_offset(a.cache[which], page, at, head[i]) + d;
+        for (int i = 0; i < 2; ++i) {
+            C* const c = (C*)a.cache[i].ptr + cache_offset(a.cache[i], page, at, head);
             if constexpr (kScaled) {
                 uint32_t top = 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(fabsf(x[i][k])));
+                for (int k = 0; k < kElements; ++k) top = max(top, __float_as_uint(fabsf(x[i][k])));
 #pragma unroll
                 for (int k = 1; k < kThreads; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+                if (!there) continue;
                 float per;
                 const float s = scale_of<C>(top, &per);
-                if (there && piece == 0) ((float*)a.scale[which].ptr)[cache_offset(a.scale[which], page, at, head[i])] = s;
-                if (there && mine) *(uint2*)c = s > 0.0f ? Code<C>::pack8(x[i], s, per) : make_uint2(0, 0);
+                if (piece.lane == 0) ((float*)a.scale[i].ptr)[cache_offset(a.scale[i], page, at, head)] = s;
+                piece.store_codes(c, a.head_dim, x[i], s, per);
             } else {
-                if (there && mine) store8(c, x[i]);
+                if (there) piece.store(c, a.head_dim, x[i]);
             }
         }
     }
@@ -397,47 +482,43 @@ template <class X, class C, int kThreads>
 __global__ void __launch_bounds__(kRowThreads) cache_read_pieces(const RowArgs a) {
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
-    const int which = a.first + blockIdx.y, d = (int)(threadIdx.x % kThreads) * 8;
-    if (d >= a.head_dim) return;
-    const uint32_t step = gridDim.x * kGroups, count = (uint32_t)a.row_count;
-    for (uint32_t base = blockIdx.x * kGroups + threadIdx.x / kThreads; base < count; base += kAtOnce * step) {
-        uint32_t token[kAtOnce], head[kAtOnce], at[kAtOnce], page[kAtOnce];
-        bool there[kAtOnce];
+    const PieceOf<X, C, kThreads> piece{(int)(threadIdx.x % kThreads)};
+    const uint32_t count = (uint32_t)a.row_count;
+    for (uint32_t row = blockIdx.x * kGroups + threadIdx.x / kThreads; row < count; row += gridDim.x * kGroups) {
+        uint32_t head, at;
+        const uint32_t token = a.heads.div(row, &head);
+        const int64_t slot = slot_of(a, token);
+        const bool there = slot >= 0 && slot < a.total_slots;
+        const uint32_t page = a.page.div(there ? (uint32_t)slot : 0, &at);
+        float x[2][kElements] = {}, s[2] = {1.0f, 1.0f};
+        if (there)
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            const uint32_t row = base + i * step;
-            token[i] = a.heads.div(row < count ? row : 0, &head[i]);
-            const int64_t slot = slot_of(a, token[i]);
-            there[i] = row < count && slot >= 0 && slot < a.total_slots;
-            page[i] = a.page.div(there[i] ? (uint32_t)slot : 0, &at[i]);
-        }
-        float x[kAtOnce][8];
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
-            if (!there[i]) continue;
-            const C* const c = (const C*)a.cache[which].ptr + cache_offset(a.cache[which], page[i], at[i], head[i]) + d;
-            if constexpr (kScaled) {
-                const float s = ((const float*)a.scale[which].ptr)[cache_offset(a.scale[which], page[i], at[i], head[i])];
-                Code<C>::unpack8(*(const uint2*)c, x[i]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[i][k] *= s;
-            } else {
-                load8(c, x[i]);
+            for (int i = 0; i < 2; ++i) {
+                if (!a.rows[i].ptr) continue;
+                const C* const c = (const C*)a.cache[i].ptr + cache_offset(a.cache[i], page, at, head);
+                if constexpr (kScaled) {
+                    s[i] = ((const float*)a.scale[i].ptr)[cache_offset(a.scale[i], page, at, head)];
+                    piece.load_codes(c, a.head_dim, x[i]);
+                } else {
+                    piece.load(c, a.head_dim, x[i]);
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            if (base + i * step < count)
-                store8((X*)a.rows[which].ptr + (int64_t)token[i] * a.rows[which].token + (int64_t)head[i] * a.rows[which].head + d, x[i]);
+        for (int i = 0; i < 2; ++i) {
+            if (!a.rows[i].ptr) continue;
+            if constexpr (kScaled)
+#pragma unroll
+                for (int k = 0; k < kElements; ++k) x[i][k] *= s[i];
+            piece.store((X*)a.rows[i].ptr + (int64_t)token * a.rows[i].token + (int64_t)head * a.rows[i].head, a.head_dim, x[i]);
+        }
     }
 }
 
 template <class X, class C, int kThreads>
 int launch_pieces(bool write, const RowArgs& a, int sms, cudaStream_t st) {
     const int64_t groups = kRowThreads / kThreads, want = (a.row_count + groups - 1) / groups;
-    const dim3 grid((unsigned)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8), a.count);
+    const int64_t resident = (int64_t)sms * 4;  // 64 registers a thread
+    const unsigned grid = (unsigned)(want < resident ? want : resident);
     if (write)
         cache_write_pieces<X, C, kThreads><<<grid, kRowThreads, 0, st>>>(a);
     else
@@ -449,9 +530,9 @@ int launch_pieces(bool write, const RowArgs& a, int sms, cudaStream_t st) {
 template <class X, class C>
 int launch_rows(bool write, const RowArgs& a, int sms, cudaStream_t st) {
     if (a.pieces) {
-        if (a.head_dim <= 64) return launch_pieces<X, C, 8>(write, a, sms, st);
-        if (a.head_dim <= 128) return launch_pieces<X, C, 16>(write, a, sms, st);
-        return launch_pieces<X, C, 32>(write, a, sms, st);
+        if (a.head_dim <= 64) return launch_pieces<X, C, 4>(write, a, sms, st);
+        if (a.head_dim <= 128) return launch_pieces<X, C, 8>(write, a, sms, st);
+        return launch_pieces<X, C, 16>(write, a, sms, st);
     }
     const int64_t want = (a.row_count + kRowThreads / 32 - 1) / (kRowThreads / 32);
     const dim3 grid((unsigned)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8), a.count);
