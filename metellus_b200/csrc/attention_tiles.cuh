@@ -135,18 +135,21 @@ template <bool kBf16> __device__ inline float2 unpack(uint32_t x) {
 // The upper 11 significant bits of a float, to nearest: what a tf32 operand keeps.
 __device__ inline uint32_t upper(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
 
-// Two codes (bytes lo_byte and hi_byte of x) as fp16, exactly.
-template <int CT, int kLo, int kHi> __device__ inline uint32_t decode(uint32_t x) {
+// Four codes as fp16, exactly: bytes 0, 1 and 2, 3 of x (kPairs), or 0, 2 and 1, 3.
+template <int CT, bool kPairs> __device__ inline void decode(uint32_t x, uint32_t& lo, uint32_t& hi) {
     if constexpr (CT == MT_I8) {
         // 0x6400 | u is 1024 + u; with u = code + 128, 1152 more than the code
-        const uint32_t u = __byte_perm(x ^ 0x80808080u, 0x64646464u, kLo | 0x40 | kHi << 8 | 0x4000);
-        const __half2 v = __hsub2(reinterpret_cast<const __half2&>(u), __half2half2(__ushort_as_half(0x6480)));
-        return reinterpret_cast<const uint32_t&>(v);
+        x ^= 0x80808080u;
+        const __half2 off = __half2half2(__ushort_as_half(0x6480));
+        const uint32_t a = __byte_perm(x, 0x64646464u, kPairs ? 0x4140 : 0x4240);
+        const uint32_t b = __byte_perm(x, 0x64646464u, kPairs ? 0x4342 : 0x4341);
+        const __half2 u = __hsub2(reinterpret_cast<const __half2&>(a), off), v = __hsub2(reinterpret_cast<const __half2&>(b), off);
+        lo = reinterpret_cast<const uint32_t&>(u);
+        hi = reinterpret_cast<const uint32_t&>(v);
     } else {
-        const uint32_t two = __byte_perm(x, 0, kLo | kHi << 4);
-        uint32_t v;
-        asm("{ .reg .b16 h, l; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l; }" : "=r"(v) : "r"(two));
-        return v;
+        if constexpr (!kPairs) x = __byte_perm(x, 0, 0x3120);
+        asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }"
+            : "=r"(lo), "=r"(hi) : "r"(x));
     }
 }
 
@@ -172,8 +175,10 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr int PP = CT == MT_F32 ? 2 : kQ32 ? QP : kScaled && std::is_same<Q, __nv_bfloat16>::value ? 1 : 2;
     // queries that fp16 may not hold are divided by a power of two per row
     static constexpr bool kNormed = CT != MT_F32 && !kBf16 && (kQ32 || kScaled);
-    // fp16 probabilities are held times 2^15: the smallest, 2^-24, is 2^-39 of the largest
-    static constexpr float kOffset = CT == MT_F16 || kScaled ? 15.0f : 0.0f;
+    // The exponents' base m is raised only when a score passes it by more than kSlack (a factor of
+    // 2^4), which after a head's first tiles is rare. fp16 probabilities are held times
+    // 2^11, so that they stay below 2^15; the smallest, 2^-24, is 2^-35 of 1.
+    static constexpr float kSlack = 4.0f, kOffset = CT == MT_F16 || kScaled ? 11.0f : 0.0f;
     // A part's queries come into shared memory as they are, while the part before is worked
     // on; then they stay in registers as operands, or, where O leaves too few, in shared memory.
     // Those that are operands as they are (one piece) need no second place, and come late.
@@ -325,10 +330,10 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     }
     in.next_length = in.b + 1 < a.batch ? length_of(t, in.b + 1) : 0;
 
-    // -- a tile to fetch. Lane l finds token l's rows of K and V (of 16 tokens, lane l + 16
-    // that of V).
+    // -- a tile to fetch: lane l looks after token l's rows of K and V
     struct Step {
-        int b, token, page, flags;  // page: -1 for no token
+        int b, page, flags;  // page: -1 for no token
+        uint32_t at;         // the token's place in it
     };
     constexpr int kFirst = 1, kLast = 2, kFromStart = 4, kEnds = 8, kMore = 16;  // of a part; its sequence's ends; parts follow
     int left = tiles;
@@ -336,8 +341,9 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     auto look_up = [&]() {
         Step s;
         s.b = in.b;
-        s.token = in.begin + in.tile * TW + (lane & (TW - 1));
-        s.page = s.token < in.end ? a.tables[(int64_t)in.b * a.table_seq + a.page.div((uint32_t)s.token)] : -1;
+        const int token = in.begin + in.tile * TW + (lane & (TW - 1));
+        const uint32_t j = a.page.div((uint32_t)token, &s.at);
+        s.page = token < in.end ? a.tables[(int64_t)in.b * a.table_seq + j] : -1;
         const bool ends = in.tile + 1 == in.tiles;
         s.flags = (fresh ? kFirst : 0) | (left > in.tiles - in.tile ? kMore : 0) | (ends || left == 1 ? kLast : 0) | (from_start ? kFromStart : 0) | (ends ? kEnds : 0);
         --left;
@@ -351,44 +357,52 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         }
         return s;
     };
+    // of 16 tokens, lanes 16 .. 31 look after V
+    const bool is_v = TW == 16 && lane >= 16;
+    const uint32_t row_page = is_v ? a.v_rows.page : a.k_rows.page, row_token = is_v ? a.v_rows.token : a.k_rows.token;
+    const int64_t head_bytes = (int64_t)kv_head * Z::EB;
+    // the piece of a row that this lane copies, where a row has no more than 32
+    const unsigned char* const k_base = (const unsigned char*)a.cache.k.ptr + head_bytes * a.cache.k.head + (CPR <= 32 ? lane % CPR * 16 : 0);
+    const unsigned char* const v_base = (const unsigned char*)a.cache.v.ptr + head_bytes * a.cache.v.head + (CPR <= 32 ? lane % CPR * 16 : 0);
+    const unsigned char* const k_scales = (const unsigned char*)a.cache.k_scale.ptr + (int64_t)kv_head * a.cache.k_scale.head * 4;
+    const unsigned char* const v_scales = (const unsigned char*)a.cache.v_scale.ptr + (int64_t)kv_head * a.cache.v_scale.head * 4;
     auto fetch = [&](const Step& s, int slot) {
         const uint32_t to = smem_address(ring + slot * Z::STAGE);
         const bool valid = s.page >= 0 && s.page < a.cache.pages;
-        const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-        uint32_t at = 0;
-        if (valid) a.page.div((uint32_t)s.token, &at);
-        auto row_of = [&](const CacheView& c, int bytes) {
-            const unsigned char* row = (const unsigned char*)c.ptr;
-            if (valid) row += ((int64_t)s.page * c.page + (int64_t)at * c.token + (int64_t)kv_head * c.head) * bytes;
-            return row;
-        };
-        const unsigned char *k_row, *v_row;
-        if constexpr (TW == 32) {
-            k_row = row_of(a.cache.k, Z::EB);
-            v_row = row_of(a.cache.v, Z::EB);
-        } else {
-            k_row = v_row = row_of(lane < 16 ? a.cache.k : a.cache.v, Z::EB);
-        }
+        const uint32_t mask = __ballot_sync(0xffffffffu, valid) & (TW == 32 ? 0xffffffffu : 0xffffu);
+        const uint32_t page = valid ? (uint32_t)s.page : 0u, at = valid ? s.at : 0u;
+        const uint32_t row = page * row_page + at * row_token;
+        const uint32_t row_v = TW == 32 ? page * a.v_rows.page + at * a.v_rows.token : row;
         if (lane == 0) sm_meta[slot] = make_int4(s.b, s.flags, (int)mask, 0);
         if constexpr (kScaled) {
-            copy4(to + 2 * TW * Z::ROW + lane * 4, row_of(a.cache.k_scale, 4), valid);
-            copy4(to + 2 * TW * Z::ROW + (32 + lane) * 4, row_of(a.cache.v_scale, 4), valid);
+            const uint32_t zk = page * a.k_scale_rows.page + at * a.k_scale_rows.token;
+            const uint32_t zv = page * a.v_scale_rows.page + at * a.v_scale_rows.token;
+            copy4(to + 2 * TW * Z::ROW + lane * 4, k_scales + (uint64_t)zk * a.k_scale_rows.unit, valid);
+            copy4(to + 2 * TW * Z::ROW + (32 + lane) * 4, v_scales + (uint64_t)zv * a.v_scale_rows.unit, valid);
         }
-        if (mask) {
+        auto copy_rows = [&](auto whole_tile) {
 #pragma unroll
             for (int which = 0; which < 2; ++which)
 #pragma unroll
                 for (int i = 0; i < TW * CPR / 32; ++i) {
                     const int r = (i * 32 + lane) / CPR, piece = (i * 32 + lane) % CPR;
-                    const unsigned char* from = (const unsigned char*)__shfl_sync(
-                        0xffffffffu, (unsigned long long)(which ? v_row : k_row), r + (TW == 16 ? 16 * which : 0));
-                    const bool real = piece < t.row_chunks, there = mask >> r & 1;
+                    const uint32_t number = __shfl_sync(0xffffffffu, which ? row_v : row, r + (TW == 16 ? 16 * which : 0));
+                    const unsigned char* const from = (which ? v_base : k_base) +
+                                                      (uint64_t)number * (which ? a.v_rows.unit : a.k_rows.unit) + (CPR <= 32 ? 0 : piece * 16);
                     const uint32_t dst = to + which * TW * Z::ROW + swizzled<CPR>(r, piece) * 16;
-                    // absent tokens: V must be zeros (their probability is 0, and 0 * NaN is not);
-                    // K's scores are replaced. Padding: K must be zeros, V's columns are not used.
-                    if (which == 0 ? (there || !real) : real) copy16(dst, from + (real ? piece * 16 : 0), real && there);
+                    if constexpr (decltype(whole_tile)::value) {
+                        copy16(dst, from, true);
+                    } else {
+                        // absent tokens: V must be zeros (their probability is 0, and 0 * NaN is not);
+                        // K's scores are replaced. Padding: K must be zeros, V's columns are not used.
+                        const bool real = piece < t.row_chunks, there = mask >> r & 1;
+                        if (which == 0 ? (there || !real) : real)
+                            copy16(dst, real ? from : (const unsigned char*)a.cache.k.ptr, real && there);
+                    }
                 }
-        }
+        };
+        if (mask == (TW == 32 ? 0xffffffffu : 0xffffu) && t.row_chunks == CPR) copy_rows(std::true_type{});
+        else if (mask) copy_rows(std::false_type{});
     };
 
     // -- a part's queries: asked for early, taken when it begins
@@ -516,7 +530,9 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     }
     Step next = ahead[S - 1];
 
-    float o[DP / 16][NT][4], m[NT][2], l[NT][2];
+    // per query head: the largest score when the base was set, the base of the exponents (less the
+    // offset), and the score above which it is set again
+    float o[DP / 16][NT][4], m[NT][2], base[NT][2], limit[NT][2], l[NT][2];
     float v_unit = 0.0f;  // O is in units of this power of two (8-bit caches)
     int slot = 0, in_part = S;  // tiles of this part so far
     for (int tile = 0; tile < tiles; ++tile) {
@@ -551,7 +567,8 @@ attention_tiles(const __grid_constant__ TileArgs t) {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    m[n][i] = -INFINITY;
+                    m[n][i] = limit[n][i] = -INFINITY;
+                    base[n][i] = -Z::kOffset;
                     l[n][i] = 0.0f;
                 }
 #pragma unroll
@@ -613,8 +630,9 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     } else if constexpr (kScaled) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t x[4] = {decode<CT, 0, 1>(r[2 * h]), decode<CT, 0, 1>(r[2 * h + 1]),
-                                                   decode<CT, 2, 3>(r[2 * h]), decode<CT, 2, 3>(r[2 * h + 1])};
+                            uint32_t x[4];
+                            decode<CT, true>(r[2 * h], x[0], x[2]);
+                            decode<CT, true>(r[2 * h + 1], x[1], x[3]);
                             times_queries(2 * c + h, x);
                         }
                     } else {
@@ -622,26 +640,97 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     }
                 }
             }
-            float ks[TB][2], vs[TB][2], shrink = 1.0f;
             if constexpr (kScaled) {
                 const float* z = (const float*)(stage + 2 * TW * Z::ROW);
+#pragma unroll
+                for (int b = 0; b < TB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float ks = z[b * 16 + h * 8 + oct];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            s[b][n][2 * h] *= ks;
+                            s[b][n][2 * h + 1] *= ks;
+                        }
+                    }
+            }
+            if (mask != (TW == 32 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+                for (int b = 0; b < TB; ++b)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!(mask >> (b * 16 + (i >> 1) * 8 + oct) & 1)) s[b][n][i] = -INFINITY;
+            }
+            float vs[TB][2], keep[NT][2];
+            bool grown = false;
+            if constexpr (kScaled) {
+                const float* z = (const float*)(stage + 2 * TW * Z::ROW) + 32;
                 float top = 0.0f;
 #pragma unroll
                 for (int b = 0; b < TB; ++b)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        ks[b][h] = z[b * 16 + h * 8 + oct];
-                        vs[b][h] = z[32 + b * 16 + h * 8 + oct];
+                        vs[b][h] = z[b * 16 + h * 8 + oct];
                         top = fmaxf(top, fabsf(vs[b][h]));
                     }
+                grown = top >= v_unit;
+            }
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                // the power of two above the largest scale so far
-                const float unit = __uint_as_float((min(__float_as_uint(top) >> 23, 252u) + 1) << 23);
-                if (unit > v_unit) {
-                    shrink = v_unit / unit;
-                    v_unit = unit;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < TB; ++b) top = fmaxf(top, fmaxf(s[b][n][i], s[b][n][2 + i]));
+                    grown |= top > limit[n][i];
+                    keep[n][i] = 1.0f;
                 }
+            // scores are compared and kept as the products give them; qscale turns them into exponents
+            const bool rescale = __any_sync(0xffffffffu, grown);
+            if (rescale) {
+                float shrink = 1.0f;
+                if constexpr (kScaled) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < TB; ++b) top = fmaxf(top, fmaxf(fabsf(vs[b][0]), fabsf(vs[b][1])));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    // the power of two above the largest scale so far
+                    const float unit = __uint_as_float((min(__float_as_uint(top) >> 23, 252u) + 1) << 23);
+                    if (unit > v_unit) {
+                        shrink = v_unit / unit;
+                        v_unit = unit;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = m[n][i];
+#pragma unroll
+                        for (int b = 0; b < TB; ++b) top = fmaxf(top, fmaxf(s[b][n][i], s[b][n][2 + i]));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const float now = top == -INFINITY ? 0.0f : top * qscale[n][i];
+                        const float k = m[n][i] == -INFINITY ? 0.0f : exp2_fast((base[n][i] + Z::kOffset) - now);
+                        m[n][i] = top;
+                        base[n][i] = now - Z::kOffset;
+                        limit[n][i] = top == -INFINITY ? top : top + Z::kSlack / qscale[n][i];
+                        l[n][i] *= k;
+                        keep[n][i] = kScaled ? k * shrink : k;
+                    }
+                if constexpr (!Z::kExact) {
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[d][n][i] *= keep[n][i & 1];
+                }
+            }
+            if constexpr (kScaled) {
                 const float per = __uint_as_float((254u << 23) - __float_as_uint(v_unit));  // 1 / v_unit
 #pragma unroll
                 for (int b = 0; b < TB; ++b)
@@ -649,41 +738,19 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     for (int h = 0; h < 2; ++h) vs[b][h] *= per;
             }
             uint32_t pf[TB][NT][2 * PP];
-            bool grown = shrink != 1.0f;
-            float keep[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float top = m[n][i];
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int b = 0; b < TB; ++b)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             float& x = s[b][n][2 * h + i];
-                            x *= kScaled ? qscale[n][i] * ks[b][h] : qscale[n][i];
-                            if (!(mask >> (b * 16 + h * 8 + oct) & 1)) x = -INFINITY;
-                            top = fmaxf(top, x);
-                        }
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const float base = top == -INFINITY ? 0.0f : top;
-                    keep[n][i] = exp2_fast(m[n][i] - base);
-                    grown |= top > m[n][i];
-                    m[n][i] = top;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int b = 0; b < TB; ++b)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float& x = s[b][n][2 * h + i];
-                            x = exp2_fast(x - base + Z::kOffset);
-                            sum += x;
+                            x = exp2_fast(fmaf(x, qscale[n][i], -base[n][i]));
+                            l[n][i] += x;
                             if constexpr (kScaled) x *= vs[b][h];
                         }
-                    l[n][i] = l[n][i] * keep[n][i] + sum;
-                    if constexpr (kScaled) keep[n][i] *= shrink;
-                }
 #pragma unroll
                 for (int b = 0; b < TB; ++b) {
                     if constexpr (CT == MT_F32) {
@@ -709,14 +776,6 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                             }
                     }
                 }
-            }
-            if (!Z::kExact && __any_sync(0xffffffffu, grown)) {
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[d][n][i] *= keep[n][i & 1];
             }
             // O^T: rows are 16 dims, columns heads as above. Where chains are kept short, a tile's
             // product is added to the rescaled O.
@@ -772,10 +831,8 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                             // 8 bits: bytes 0, 2 are two tokens' even dim, bytes 1, 3 their odd one
                             uint32_t x[4];
                             if constexpr (kScaled) {
-                                x[0] = decode<CT, 0, 2>(r[b][2 * h]);
-                                x[1] = decode<CT, 1, 3>(r[b][2 * h]);
-                                x[2] = decode<CT, 0, 2>(r[b][2 * h + 1]);
-                                x[3] = decode<CT, 1, 3>(r[b][2 * h + 1]);
+                                decode<CT, false>(r[b][2 * h], x[0], x[1]);
+                                decode<CT, false>(r[b][2 * h + 1], x[2], x[3]);
                             } else {
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) x[i] = r[b][i];
@@ -811,6 +868,8 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                     const bool none = m[n][i] == -INFINITY && sum == 0.0f;
+                    // what sums are relative to, as an exponent
+                    const float exponent = m[n][i] == -INFINITY ? -INFINITY : base[n][i];
                     const int r = quad * 2 + i, row = n * 8 + r;
                     float f = whole ? 1.0f / sum : 1.0f;
                     if constexpr (kScaled) f *= v_unit;
@@ -822,10 +881,10 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     }
                     if (oct == 0 && row < rows) {
                         if (!whole)
-                            t.part_ml[part * ROWS + row] = make_float2(m[n][i], sum);
+                            t.part_ml[part * ROWS + row] = make_float2(exponent, sum);
                         else if (a.lse)
                             a.lse[(int64_t)meta.x * a.lse_seq + (int64_t)(head0 + row) * a.lse_head] =
-                                (m[n][i] + log2f(sum) - Z::kOffset) * kLn2;
+                                (exponent + log2f(sum)) * kLn2;
                     }
                 }
                 __syncwarp();
@@ -863,7 +922,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 // than sequences, a range: it stands for the sequence that it starts in the middle of, if
 // that ends in it.
 template <class Q, int DP, int ROWS, int TW>
-__global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ TileArgs t, float offset, int by_sequence) {
+__global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ TileArgs t, int by_sequence) {
     constexpr int kLanes = DP / 4, kSide = 8, kJoinThreads = kLanes * kSide;  // threads a part, parts at a time
     __shared__ float4 sm_o[kSide][kLanes];
     __shared__ float2 sm_ml[kSide];
@@ -945,7 +1004,7 @@ __global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ Til
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (lane * 4 + i < a.cache.head_dim) out[i] = rounded<Q>(none ? 0.0f : y[i] * per);
-    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.lse_seq + (int64_t)head * a.lse_head] = (m + log2f(l) - offset) * kLn2;
+    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.lse_seq + (int64_t)head * a.lse_head] = (m + log2f(l)) * kLn2;
 }
 
 // ---- launch ------------------------------------------------------------------------------------
@@ -1007,7 +1066,7 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    RT_CHECK(cudaLaunchKernelEx(&cfg, join_parts<Q, DP, Z::ROWS, Z::TW>, (const TileArgs)t, Z::kOffset, (int)by_sequence));
+    RT_CHECK(cudaLaunchKernelEx(&cfg, join_parts<Q, DP, Z::ROWS, Z::TW>, (const TileArgs)t, (int)by_sequence));
     return 0;
 }
 

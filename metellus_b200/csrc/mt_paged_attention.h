@@ -6,6 +6,12 @@
 
 namespace mt {
 
+// Rows of a cache array by 32-bit numbers: row (p, t) of a head is (p * page + t * token) * unit bytes
+// behind the head's first. unit: the largest power of two that divides the strides.
+struct RowNumbers {
+    uint32_t page = 0, token = 0, unit = 0;
+};
+
 struct AttentionArgs {
     const void* q;
     int64_t q_seq, q_head;  // strides in elements
@@ -18,6 +24,7 @@ struct AttentionArgs {
     const int32_t* lengths;
     int64_t length_seq;
     CacheShape cache;
+    RowNumbers k_rows, v_rows, k_scale_rows, v_scale_rows;  // for the tiles
     FastDiv page;
     int q_type, batch, group, max_tokens, window;
     float scale;

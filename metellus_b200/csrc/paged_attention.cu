@@ -8,6 +8,16 @@ namespace mt {
 
 namespace {
 
+// Whether an array's rows, whose strides are multiples of `least` bytes, can be numbered in 32 bits.
+bool number_rows(const CacheView& view, const CacheShape& c, int bytes, uint32_t least, RowNumbers* out) {
+    const int64_t page = view.page * bytes, token = view.token * bytes;
+    uint32_t unit = least;
+    while (unit < (1u << 20) && page % (2 * unit) == 0 && token % (2 * unit) == 0) unit *= 2;
+    *out = {(uint32_t)(page / unit), (uint32_t)(token / unit), unit};
+    const double last = (double)(c.pages - 1) * (double)(page / unit) + (double)(c.page_size - 1) * (double)(token / unit);
+    return last < 4294967296.0;
+}
+
 int check_attention(const char* who, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
                     int64_t window, AttentionArgs* a, int* batch, int* heads, bool* tiled) {
     CacheShape c;
@@ -43,7 +53,11 @@ int check_attention(const char* who, const mt_array* q, const mt_paged_cache* ca
     *batch = a->batch = (int)q->shape[0];
     *heads = (int)q->shape[1];
     a->window = window == 0 || window > INT32_MAX ? INT32_MAX : (int)window;
-    *tiled = c.head_dim * bytes_of(c.dtype) % 16 == 0 && rows_aligned(cache->k, 16) && rows_aligned(cache->v, 16);
+    const int bytes = bytes_of(c.dtype);
+    *tiled = c.head_dim * bytes % 16 == 0 && rows_aligned(cache->k, 16) && rows_aligned(cache->v, 16) &&
+             number_rows(c.k, c, bytes, 16, &a->k_rows) && number_rows(c.v, c, bytes, 16, &a->v_rows);
+    if (*tiled && c.scaled())
+        *tiled = number_rows(c.k_scale, c, 4, 4, &a->k_scale_rows) && number_rows(c.v_scale, c, 4, 4, &a->v_scale_rows);
     return 0;
 }
 
@@ -113,7 +127,7 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
     OnDevice on;
     RT_CHECK(on.enter(dev));
     if (int rc = call_stream(dev, stream, &st)) return rc;
-    if (!tiled) return attend_by_rows(a, st);
+    if (!tiled || scale < 0.0) return attend_by_rows(a, st);  // tiles compare scores before they are scaled
     uint64_t need = 0;
     if (int rc = attend_tiles(a, false, nullptr, &need, dev, st)) return rc;
     if (need && (!workspace || workspace_bytes < need))

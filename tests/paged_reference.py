@@ -11,8 +11,8 @@ sum p v / sum p, with A = sum p |v| / sum p:
 * probabilities rounded to the product's operand type: u(p) A;
 * sums over n tokens in fp32: n 2^-23 A each for numerator and denominator;
 * probabilities too small for their type: each loses at most half its smallest step, at most
-  2^-40 of the largest one where operands are fp16 (held times 2^15, smallest step 2^-24),
-  2^-126 in the others' range; that is n 2^-40 (or n 2^-126) times the largest value a row of V
+  2^-36 of the largest one where operands are fp16 (held times at least 2^11, smallest step
+  2^-24), 2^-126 in the others' range; that is n 2^-36 (or n 2^-126) times the largest value a row of V
   can hold (scale times largest code, as scales are multiplied in with them);
 * the output's own rounding: u(out) |o|, at least half its type's smallest step.
 
@@ -66,7 +66,7 @@ def attention(q, k_cache, v_cache, tables, lengths, *, k_scale=None, v_scale=Non
     split = q.dtype == torch.float32
     operand = torch.float16 if k_cache.dtype in CODE_MAX else k_cache.dtype
     up = 2.0 ** -21 if split else half_step(operand)
-    lost = 2.0 ** -40 if operand is torch.float16 else 2.0 ** -126
+    lost = 2.0 ** -36 if operand is torch.float16 else 2.0 ** -126
     least = torch.finfo(q.dtype).smallest_normal * half_step(q.dtype)
     for i in range(b):
         n = min(max(int(lengths[i]), 0), tables.shape[1] * ps)
