@@ -32,6 +32,7 @@ template <class Q, class C>
 __global__ void __launch_bounds__(kThreads) attention_rows(const AttentionArgs a) {
     constexpr bool kScaled = sizeof(C) == 1;
     __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows], sm_o[kWarps][kMaxHeadDim];
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int b = blockIdx.x, g = blockIdx.y, r0 = blockIdx.z * kRows;
     const int rows = min(kRows, a.group - r0), dim = a.cache.head_dim;
@@ -118,8 +119,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows(const AttentionArgs a
 
 template <class Q, class C> int launch(const AttentionArgs& a, cudaStream_t st) {
     const dim3 grid(a.batch, a.cache.kv_heads, (a.group + kRows - 1) / kRows);
-    attention_rows<Q, C><<<grid, kThreads, 0, st>>>(a);
-    RT_CHECK(cudaGetLastError());
+    RT_CHECK(launch_early(attention_rows<Q, C>, grid, kThreads, 0, st, a));
     return 0;
 }
 

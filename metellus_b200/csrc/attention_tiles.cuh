@@ -315,6 +315,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     uint32_t row_block;
     const int kv_head = (int)t.row_blocks.div(item, &row_block);
     const int head0 = kv_head * a.group + (int)row_block * ROWS, rows = min(ROWS, a.group - (int)row_block * ROWS);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     Cursor in;
     int tiles;
     if (t.whole) {
@@ -927,6 +928,7 @@ __global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ Til
     __shared__ float4 sm_o[kSide][kLanes];
     __shared__ float2 sm_ml[kSide];
     const AttentionArgs& a = t.a;
+    asm volatile("griddepcontrol.launch_dependents;");
     const int r = blockIdx.y;
     uint32_t item, row_block;
     const int x = (int)t.per_range.div(blockIdx.x, &item);
@@ -1053,20 +1055,12 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
         RT_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::SMEM));
         ready[dev] = true;
     }
-    kernel<<<(unsigned)blocks, Z::NW * 32, Z::SMEM, st>>>(t);
-    RT_CHECK(cudaGetLastError());
+    RT_CHECK(launch_early(kernel, dim3((unsigned)blocks), dim3(Z::NW * 32), Z::SMEM, st, t));
     if (t.whole) return 0;
     const bool by_sequence = a.batch <= ranges;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((by_sequence ? a.batch : ranges) * t.items), a.group < Z::ROWS ? a.group : Z::ROWS);
-    cfg.blockDim = dim3(DP * 2);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    RT_CHECK(cudaLaunchKernelEx(&cfg, join_parts<Q, DP, Z::ROWS, Z::TW>, (const TileArgs)t, (int)by_sequence));
+    RT_CHECK(launch_early(join_parts<Q, DP, Z::ROWS, Z::TW>,
+                          dim3((unsigned)((by_sequence ? a.batch : ranges) * t.items), a.group < Z::ROWS ? a.group : Z::ROWS),
+                          dim3(DP * 2), 0, st, t, (int)by_sequence));
     return 0;
 }
 

@@ -28,6 +28,24 @@ int sm_count(int dev, int* out);
                             __FILE__, __LINE__);                                     \
     } while (0)
 
+// Launches a kernel that begins with `griddepcontrol.wait`: its blocks may be set up while the
+// kernel before it on the stream ends, if that one is of this library too (which allow it early,
+// by `griddepcontrol.launch_dependents`); the wait is for all of that kernel's memory.
+template <class... P, class... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // Makes `dev` current for a call and gives the caller its own device back.
 struct OnDevice {
     int caller = -1;

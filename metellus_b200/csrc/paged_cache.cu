@@ -375,6 +375,7 @@ constexpr int kPerLane = kMaxHeadDim / 32;
 
 template <class X, class C>
 __global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     const int lane = threadIdx.x & 31, which = a.first + blockIdx.y;
     const int64_t stride = (int64_t)gridDim.x * (kRowThreads / 32);
@@ -413,6 +414,7 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a)
 
 template <class X, class C>
 __global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     const int lane = threadIdx.x & 31, which = a.first + blockIdx.y;
     const int64_t stride = (int64_t)gridDim.x * (kRowThreads / 32);
@@ -440,6 +442,7 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) 
 // and of V together.
 template <class X, class C, int kThreads>
 __global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
     const PieceOf<X, C, kThreads> piece{(int)(threadIdx.x % kThreads)};
@@ -480,6 +483,7 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs 
 
 template <class X, class C, int kThreads>
 __global__ void __launch_bounds__(kRowThreads) cache_read_pieces(const RowArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
     const PieceOf<X, C, kThreads> piece{(int)(threadIdx.x % kThreads)};
@@ -520,10 +524,9 @@ int launch_pieces(bool write, const RowArgs& a, int sms, cudaStream_t st) {
     const int64_t resident = (int64_t)sms * 4;  // 64 registers a thread
     const unsigned grid = (unsigned)(want < resident ? want : resident);
     if (write)
-        cache_write_pieces<X, C, kThreads><<<grid, kRowThreads, 0, st>>>(a);
+        RT_CHECK(launch_early(cache_write_pieces<X, C, kThreads>, grid, kRowThreads, 0, st, a));
     else
-        cache_read_pieces<X, C, kThreads><<<grid, kRowThreads, 0, st>>>(a);
-    RT_CHECK(cudaGetLastError());
+        RT_CHECK(launch_early(cache_read_pieces<X, C, kThreads>, grid, kRowThreads, 0, st, a));
     return 0;
 }
 
@@ -537,10 +540,9 @@ int launch_rows(bool write, const RowArgs& a, int sms, cudaStream_t st) {
     const int64_t want = (a.row_count + kRowThreads / 32 - 1) / (kRowThreads / 32);
     const dim3 grid((unsigned)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8), a.count);
     if (write)
-        cache_write_rows<X, C><<<grid, kRowThreads, 0, st>>>(a);
+        RT_CHECK(launch_early(cache_write_rows<X, C>, grid, kRowThreads, 0, st, a));
     else
-        cache_read_rows<X, C><<<grid, kRowThreads, 0, st>>>(a);
-    RT_CHECK(cudaGetLastError());
+        RT_CHECK(launch_early(cache_read_rows<X, C>, grid, kRowThreads, 0, st, a));
     return 0;
 }
 
