@@ -382,9 +382,10 @@ attention_tiles(const __grid_constant__ TileArgs t) {
             copy4(to + 2 * TW * Z::ROW + (32 + lane) * 4, v_scales + (uint64_t)zv * a.v_scale_rows.unit, valid);
         }
         auto copy_rows = [&](auto whole_tile) {
+            constexpr int kUnroll = decltype(whole_tile)::value ? TW * CPR / 32 : 1;  // the rare case's code stays small
 #pragma unroll
             for (int which = 0; which < 2; ++which)
-#pragma unroll
+#pragma unroll kUnroll
                 for (int i = 0; i < TW * CPR / 32; ++i) {
                     const int r = (i * 32 + lane) / CPR, piece = (i * 32 + lane) % CPR;
                     const uint32_t number = __shfl_sync(0xffffffffu, which ? row_v : row, r + (TW == 16 ? 16 * which : 0));

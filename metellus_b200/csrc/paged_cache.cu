@@ -271,12 +271,10 @@ template <class T> __device__ inline float2 floats(uint32_t w) {
     else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// A thread's 16 elements of a row, from and to memory, in runs whose neighbours belong to the
+// A thread's elements of a row, from and to memory, in runs whose neighbours belong to the
 // next thread, so that a warp's accesses are of whole lines: runs of 4 where that fills 16
 // bytes on one side, else of 8.
-constexpr int kElements = 16;
-
-template <int kThreads, int kRun> struct Piece {
+template <int kElements, int kThreads, int kRun> struct Piece {
     static constexpr int kRuns = kElements / kRun;
     int lane;
     __device__ int at(int run) const { return (run * kThreads + lane) * kRun; }
@@ -359,7 +357,8 @@ template <int kThreads, int kRun> struct Piece {
             }
     }
 };
-template <class X, class C, int kThreads> using PieceOf = Piece<kThreads, sizeof(X) == 4 || sizeof(C) == 4 ? 4 : 8>;
+template <class X, class C, int kElements, int kThreads>
+using PieceOf = Piece<kElements, kThreads, sizeof(X) == 4 || sizeof(C) == 4 || kElements == 4 ? 4 : 8>;
 
 __device__ inline int64_t slot_of(const RowArgs& a, int64_t token) {
     return a.slots64 ? ((const int64_t*)a.slots)[token * a.slot_stride]
@@ -438,14 +437,17 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) 
     }
 }
 
-// The same in pieces of 16 elements: kThreads threads (a power of two) a row, its rows of K
-// and of V together.
-template <class X, class C, int kThreads>
+// The same in pieces: kThreads threads (a power of two) a row, kElements of it a thread. With
+// many rows 16 elements, and the rows of K and of V together; with few, where a call takes as
+// long as one thread's work does, 4 or 8, and K and V in different blocks (gridDim.y = 2).
+template <class X, class C, int kElements, int kThreads>
 __global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
-    const PieceOf<X, C, kThreads> piece{(int)(threadIdx.x % kThreads)};
+    constexpr bool kBoth = kElements == 16;
+    const PieceOf<X, C, kElements, kThreads> piece{(int)(threadIdx.x % kThreads)};
+    const int from = kBoth ? 0 : blockIdx.y, to = kBoth ? 2 : from + 1;
     const uint32_t count = (uint32_t)a.row_count;
     // every thread of a warp takes every turn: a row's threads exchange their largest elements
     for (uint32_t base = blockIdx.x * kGroups; base < count; base += gridDim.x * kGroups) {
@@ -453,40 +455,44 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs 
         uint32_t head, at;
         const uint32_t token = a.heads.div(row < count ? row : 0, &head);
         const int64_t slot = row < count ? slot_of(a, token) : -1;
-        float x[2][kElements] = {};
+        float x[kBoth ? 2 : 1][kElements] = {};
         if (row < count)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                piece.load((const X*)a.rows[i].ptr + (int64_t)token * a.rows[i].token + (int64_t)head * a.rows[i].head, a.head_dim, x[i]);
+            for (int i = from; i < to; ++i)
+                piece.load((const X*)a.rows[i].ptr + (int64_t)token * a.rows[i].token + (int64_t)head * a.rows[i].head, a.head_dim,
+                           x[kBoth ? i : 0]);
         const bool there = slot >= 0 && slot < a.total_slots;
         const uint32_t page = a.page.div(there ? (uint32_t)slot : 0, &at);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = from; i < to; ++i) {
+            const float* const xi = x[kBoth ? i : 0];
             C* const c = (C*)a.cache[i].ptr + cache_offset(a.cache[i], page, at, head);
             if constexpr (kScaled) {
                 uint32_t top = 0;
 #pragma unroll
-                for (int k = 0; k < kElements; ++k) top = max(top, __float_as_uint(fabsf(x[i][k])));
+                for (int k = 0; k < kElements; ++k) top = max(top, __float_as_uint(fabsf(xi[k])));
 #pragma unroll
                 for (int k = 1; k < kThreads; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
                 if (!there) continue;
                 float per;
                 const float s = scale_of<C>(top, &per);
                 if (piece.lane == 0) ((float*)a.scale[i].ptr)[cache_offset(a.scale[i], page, at, head)] = s;
-                piece.store_codes(c, a.head_dim, x[i], s, per);
+                piece.store_codes(c, a.head_dim, xi, s, per);
             } else {
-                if (there) piece.store(c, a.head_dim, x[i]);
+                if (there) piece.store(c, a.head_dim, xi);
             }
         }
     }
 }
 
-template <class X, class C, int kThreads>
+template <class X, class C, int kElements, int kThreads>
 __global__ void __launch_bounds__(kRowThreads) cache_read_pieces(const RowArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
-    const PieceOf<X, C, kThreads> piece{(int)(threadIdx.x % kThreads)};
+    constexpr bool kBoth = kElements == 16;
+    const PieceOf<X, C, kElements, kThreads> piece{(int)(threadIdx.x % kThreads)};
+    const int from = kBoth ? 0 : blockIdx.y, to = kBoth ? 2 : from + 1;
     const uint32_t count = (uint32_t)a.row_count;
     for (uint32_t row = blockIdx.x * kGroups + threadIdx.x / kThreads; row < count; row += gridDim.x * kGroups) {
         uint32_t head, at;
@@ -494,48 +500,53 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_pieces(const RowArgs a
         const int64_t slot = slot_of(a, token);
         const bool there = slot >= 0 && slot < a.total_slots;
         const uint32_t page = a.page.div(there ? (uint32_t)slot : 0, &at);
-        float x[2][kElements] = {}, s[2] = {1.0f, 1.0f};
+        float x[kBoth ? 2 : 1][kElements] = {}, s[2] = {1.0f, 1.0f};
         if (there)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = from; i < to; ++i) {
                 if (!a.rows[i].ptr) continue;
+                float* const xi = x[kBoth ? i : 0];
                 const C* const c = (const C*)a.cache[i].ptr + cache_offset(a.cache[i], page, at, head);
                 if constexpr (kScaled) {
                     s[i] = ((const float*)a.scale[i].ptr)[cache_offset(a.scale[i], page, at, head)];
-                    piece.load_codes(c, a.head_dim, x[i]);
+                    piece.load_codes(c, a.head_dim, xi);
                 } else {
-                    piece.load(c, a.head_dim, x[i]);
+                    piece.load(c, a.head_dim, xi);
                 }
             }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = from; i < to; ++i) {
             if (!a.rows[i].ptr) continue;
+            float* const xi = x[kBoth ? i : 0];
             if constexpr (kScaled)
 #pragma unroll
-                for (int k = 0; k < kElements; ++k) x[i][k] *= s[i];
-            piece.store((X*)a.rows[i].ptr + (int64_t)token * a.rows[i].token + (int64_t)head * a.rows[i].head, a.head_dim, x[i]);
+                for (int k = 0; k < kElements; ++k) xi[k] *= s[i];
+            piece.store((X*)a.rows[i].ptr + (int64_t)token * a.rows[i].token + (int64_t)head * a.rows[i].head, a.head_dim, xi);
         }
     }
 }
 
-template <class X, class C, int kThreads>
+template <class X, class C, int kElements, int kThreads>
 int launch_pieces(bool write, const RowArgs& a, int sms, cudaStream_t st) {
     const int64_t groups = kRowThreads / kThreads, want = (a.row_count + groups - 1) / groups;
     const int64_t resident = (int64_t)sms * 4;  // 64 registers a thread
-    const unsigned grid = (unsigned)(want < resident ? want : resident);
+    const dim3 grid((unsigned)(want < resident ? want : resident), kElements == 16 ? 1 : 2);
     if (write)
-        RT_CHECK(launch_early(cache_write_pieces<X, C, kThreads>, grid, kRowThreads, 0, st, a));
+        RT_CHECK(launch_early(cache_write_pieces<X, C, kElements, kThreads>, grid, kRowThreads, 0, st, a));
     else
-        RT_CHECK(launch_early(cache_read_pieces<X, C, kThreads>, grid, kRowThreads, 0, st, a));
+        RT_CHECK(launch_early(cache_read_pieces<X, C, kElements, kThreads>, grid, kRowThreads, 0, st, a));
     return 0;
 }
 
 template <class X, class C>
 int launch_rows(bool write, const RowArgs& a, int sms, cudaStream_t st) {
     if (a.pieces) {
-        if (a.head_dim <= 64) return launch_pieces<X, C, 4>(write, a, sms, st);
-        if (a.head_dim <= 128) return launch_pieces<X, C, 8>(write, a, sms, st);
-        return launch_pieces<X, C, 16>(write, a, sms, st);
+        // few: not even one block an SM at 16 elements a thread. One token of 16 sequences, 8 heads of
+        // 128, bf16 to e4m3: 2.5 us with 4 elements a thread, 5.5 with 16.
+        const bool few = a.row_count * ((a.head_dim + 15) / 16) < (int64_t)sms * kRowThreads;
+        if (a.head_dim <= 64) return few ? launch_pieces<X, C, 4, 16>(write, a, sms, st) : launch_pieces<X, C, 16, 4>(write, a, sms, st);
+        if (a.head_dim <= 128) return few ? launch_pieces<X, C, 4, 32>(write, a, sms, st) : launch_pieces<X, C, 16, 8>(write, a, sms, st);
+        return few ? launch_pieces<X, C, 8, 32>(write, a, sms, st) : launch_pieces<X, C, 16, 16>(write, a, sms, st);
     }
     const int64_t want = (a.row_count + kRowThreads / 32 - 1) / (kRowThreads / 32);
     const dim3 grid((unsigned)(want < (int64_t)sms * 8 ? want : (int64_t)sms * 8), a.count);
