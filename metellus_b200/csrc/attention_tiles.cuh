@@ -55,8 +55,13 @@ struct TileArgs {
 
 __device__ inline uint32_t smem_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-__device__ inline void copy16(uint32_t dst, const void* src, bool really) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(really ? 16 : 0));
+// kBeyond: a row of 8-bit codes is 128 bytes or less, and the next one is another warp's of the
+// same block: L2 fetches 256 bytes (e4m3, 32 sequences of 8192: 107 us, with 128 bytes 111).
+template <bool kBeyond> __device__ inline void copy16(uint32_t dst, const void* src, bool really) {
+    if constexpr (kBeyond)
+        asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(really ? 16 : 0));
+    else
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(really ? 16 : 0));
 }
 __device__ inline void copy4(uint32_t dst, const void* src, bool really) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(really ? 4 : 0));
@@ -178,6 +183,10 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // The exponents' base m is raised only when a score passes it by more than kSlack (a factor of
     // 2^4), which after a head's first tiles is rare. fp16 probabilities are held times
     // 2^11, so that they stay below 2^15; the smallest, 2^-24, is 2^-35 of 1.
+    // A 16-bit cache's next rows are asked for in two bursts a tile, K's before the scores and V's behind
+    // them (64 sequences of 4096 .. 8192, bf16: 249 us, in one burst 257). 8-bit and 32-bit
+    // tiles, whose products take longer, lose by it (int8 44 -> 46, fp32 86 -> 91).
+    static constexpr bool kTwoBursts = EB == 2;
     static constexpr float kSlack = 4.0f, kOffset = CT == MT_F16 || kScaled ? 11.0f : 0.0f;
     // A part's queries come into shared memory as they are, while the part before is worked
     // on; then they stay in registers as operands, or, where O leaves too few, in shared memory.
@@ -367,45 +376,52 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     const unsigned char* const v_base = (const unsigned char*)a.cache.v.ptr + head_bytes * a.cache.v.head + (CPR <= 32 ? lane % CPR * 16 : 0);
     const unsigned char* const k_scales = (const unsigned char*)a.cache.k_scale.ptr + (int64_t)kv_head * a.cache.k_scale.head * 4;
     const unsigned char* const v_scales = (const unsigned char*)a.cache.v_scale.ptr + (int64_t)kv_head * a.cache.v_scale.head * 4;
-    auto fetch = [&](const Step& s, int slot) {
-        const uint32_t to = smem_address(ring + slot * Z::STAGE);
+    // where the rows of the tile being asked for are, and which of them there are
+    uint32_t k_row = 0, v_row = 0, there_mask = 0;
+    constexpr uint32_t kAll = TW == 32 ? 0xffffffffu : 0xffffu;
+    auto find_rows = [&](const Step& s, int slot) {
         const bool valid = s.page >= 0 && s.page < a.cache.pages;
-        const uint32_t mask = __ballot_sync(0xffffffffu, valid) & (TW == 32 ? 0xffffffffu : 0xffffu);
+        there_mask = __ballot_sync(0xffffffffu, valid) & kAll;
         const uint32_t page = valid ? (uint32_t)s.page : 0u, at = valid ? s.at : 0u;
-        const uint32_t row = page * row_page + at * row_token;
-        const uint32_t row_v = TW == 32 ? page * a.v_rows.page + at * a.v_rows.token : row;
-        if (lane == 0) sm_meta[slot] = make_int4(s.b, s.flags, (int)mask, 0);
+        k_row = page * row_page + at * row_token;
+        v_row = TW == 32 ? page * a.v_rows.page + at * a.v_rows.token : k_row;
+        if (lane == 0) sm_meta[slot] = make_int4(s.b, s.flags, (int)there_mask, 0);
         if constexpr (kScaled) {
+            const uint32_t to = smem_address(ring + slot * Z::STAGE) + 2 * TW * Z::ROW;
             const uint32_t zk = page * a.k_scale_rows.page + at * a.k_scale_rows.token;
             const uint32_t zv = page * a.v_scale_rows.page + at * a.v_scale_rows.token;
-            copy4(to + 2 * TW * Z::ROW + lane * 4, k_scales + (uint64_t)zk * a.k_scale_rows.unit, valid);
-            copy4(to + 2 * TW * Z::ROW + (32 + lane) * 4, v_scales + (uint64_t)zv * a.v_scale_rows.unit, valid);
+            copy4(to + lane * 4, k_scales + (uint64_t)zk * a.k_scale_rows.unit, valid);
+            copy4(to + (32 + lane) * 4, v_scales + (uint64_t)zv * a.v_scale_rows.unit, valid);
         }
-        auto copy_rows = [&](auto whole_tile) {
-            constexpr int kUnroll = decltype(whole_tile)::value ? TW * CPR / 32 : 1;  // the rare case's code stays small
-#pragma unroll
-            for (int which = 0; which < 2; ++which)
-#pragma unroll kUnroll
-                for (int i = 0; i < TW * CPR / 32; ++i) {
-                    const int r = (i * 32 + lane) / CPR, piece = (i * 32 + lane) % CPR;
-                    const uint32_t number = __shfl_sync(0xffffffffu, which ? row_v : row, r + (TW == 16 ? 16 * which : 0));
-                    const unsigned char* const from = (which ? v_base : k_base) +
-                                                      (uint64_t)number * (which ? a.v_rows.unit : a.k_rows.unit) + (CPR <= 32 ? 0 : piece * 16);
-                    const uint32_t dst = to + which * TW * Z::ROW + swizzled<CPR>(r, piece) * 16;
-                    if constexpr (decltype(whole_tile)::value) {
-                        copy16(dst, from, true);
-                    } else {
-                        // absent tokens: V must be zeros (their probability is 0, and 0 * NaN is not);
-                        // K's scores are replaced. Padding: K must be zeros, V's columns are not used.
-                        const bool real = piece < t.row_chunks, there = mask >> r & 1;
-                        if (which == 0 ? (there || !real) : real)
-                            copy16(dst, real ? from : (const unsigned char*)a.cache.k.ptr, real && there);
-                    }
-                }
-        };
-        if (mask == (TW == 32 ? 0xffffffffu : 0xffffu) && t.row_chunks == CPR) copy_rows(std::true_type{});
-        else if (mask) copy_rows(std::false_type{});
     };
+    auto copy_rows = [&](int slot, auto of_v, auto whole_tile) {
+        constexpr bool kV = decltype(of_v)::value, kWhole = decltype(whole_tile)::value;
+        constexpr int kUnroll = kWhole ? TW * CPR / 32 : 1;  // the rare case's code stays small
+        const uint32_t to = smem_address(ring + slot * Z::STAGE) + (kV ? TW * Z::ROW : 0);
+#pragma unroll kUnroll
+        for (int i = 0; i < TW * CPR / 32; ++i) {
+            const int r = (i * 32 + lane) / CPR, piece = (i * 32 + lane) % CPR;
+            const uint32_t number = __shfl_sync(0xffffffffu, kV ? v_row : k_row, r + (kV && TW == 16 ? 16 : 0));
+            const unsigned char* const from = (kV ? v_base : k_base) + (uint64_t)number * (kV ? a.v_rows.unit : a.k_rows.unit) +
+                                              (CPR <= 32 ? 0 : piece * 16);
+            const uint32_t dst = to + swizzled<CPR>(r, piece) * 16;
+            if constexpr (kWhole) {
+                copy16<kScaled>(dst, from, true);
+            } else {
+                // absent tokens: V must be zeros (their probability is 0, and 0 * NaN is not); K's
+                // scores are replaced. Padding: K must be zeros, V's columns are not used.
+                const bool real = piece < t.row_chunks, there = there_mask >> r & 1;
+                if (kV ? real : there || !real)
+                    copy16<kScaled>(dst, real ? from : (const unsigned char*)a.cache.k.ptr, real && there);
+            }
+        }
+    };
+    auto fetch = [&](int slot, auto of_v) {
+        if (there_mask == kAll && t.row_chunks == CPR) copy_rows(slot, of_v, std::true_type{});
+        else if (there_mask) copy_rows(slot, of_v, std::false_type{});
+    };
+    constexpr std::false_type kKeys{};
+    constexpr std::true_type kValues{};
 
     // -- a part's queries: asked for early, taken when it begins
     auto ask_queries = [&](int b) {
@@ -414,7 +430,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         if (t.q_chunks)
             for (int i = lane; i < rows * t.q_chunks; i += 32) {
                 const int r = i / t.q_chunks, piece = i - r * t.q_chunks;
-                copy16(to + r * Z::QROW + piece * 16, (const unsigned char*)(q + (int64_t)r * a.q_head) + piece * 16, true);
+                copy16<false>(to + r * Z::QROW + piece * 16, (const unsigned char*)(q + (int64_t)r * a.q_head) + piece * 16, true);
             }
         else
             for (int i = lane; i < rows * a.cache.head_dim; i += 32) {
@@ -527,7 +543,11 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         if (s < tiles) ahead[s] = look_up();
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) {
-        if (s < tiles) fetch(ahead[s], s);
+        if (s < tiles) {
+            find_rows(ahead[s], s);
+            fetch(s, kKeys);
+            fetch(s, kValues);
+        }
         copies_commit();
     }
     Step next = ahead[S - 1];
@@ -539,14 +559,18 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     int slot = 0, in_part = S;  // tiles of this part so far
     for (int tile = 0; tile < tiles; ++tile) {
         __syncwarp();
-        if (tile + S - 1 < tiles) {
-            fetch(next, slot == 0 ? S - 1 : slot - 1);
+        // the tile S - 1 ahead goes into the last one's stage
+        const bool ask = tile + S - 1 < tiles;
+        const int ask_slot = slot == 0 ? S - 1 : slot - 1;
+        if (ask) {
+            find_rows(next, ask_slot);
+            fetch(ask_slot, kKeys);
+            if constexpr (!Z::kTwoBursts) fetch(ask_slot, kValues);
             if (left > 0) next = look_up();
         } else {
             asm volatile("griddepcontrol.launch_dependents;");
         }
-        copies_commit();
-        copies_wait<S - 1>();
+        copies_wait<S - 2>();  // this turn's are not committed yet
         __syncwarp();
         ++in_part;
         const int4 meta = sm_meta[slot];
@@ -581,6 +605,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     for (int i = 0; i < 4; ++i) o[d][n][i] = 0.0f;
             v_unit = 1.17549435e-38f;  // 2^-126
         }
+        if (Z::kTwoBursts && ask && !mask) fetch(ask_slot, kValues);
         if (mask) {
             // S^T: s[.][.][0], [1] are token oct, heads quad * 2 + 0, 1; [2], [3] token oct + 8. The
             // largest pieces' products go into `part` first where they are kept apart.
@@ -656,7 +681,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         }
                     }
             }
-            if (mask != (TW == 32 ? 0xffffffffu : 0xffffu)) {
+            if (mask != kAll) {
 #pragma unroll
                 for (int b = 0; b < TB; ++b)
 #pragma unroll
@@ -739,6 +764,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) vs[b][h] *= per;
             }
+            if (Z::kTwoBursts && ask) fetch(ask_slot, kValues);
             uint32_t pf[TB][NT][2 * PP];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -852,6 +878,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                 }
             }
         }
+        copies_commit();
         if (meta.y & kLast) {
             // -- the part ends: from the accumulators' layout to rows by way of this tile's stage, into which
             // nothing will be fetched before the next tile
