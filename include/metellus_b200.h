@@ -199,7 +199,8 @@ int mt_cache_read(int dev, const mt_paged_cache* cache, const mt_array* slots, c
  * [batch]; lse (may be NULL): MT_F32 [batch, heads], the natural logarithm of the sum of
  * exp(scores), -inf without tokens. Scores, sums and the output's accumulators are fp32.
  * `workspace`: mt_paged_attention_workspace() bytes of device memory, 16-byte aligned,
- * that no other call may use at the same time; its contents do not matter. */
+ * that no other call may use at the same time; its contents do not matter. With both
+ * `stream` and `workspace` NULL it comes from the device's pool for the call. */
 int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, const mt_array* tables,
                        const mt_array* lengths, const mt_array* out, const mt_array* lse, double scale,
                        int64_t window, void* workspace, uint64_t workspace_bytes, void* stream);

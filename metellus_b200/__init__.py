@@ -8,6 +8,7 @@ from metellus_b200.api.paged import cache_read, cache_write, paged_attention
 from metellus_b200.api.run import RunResult, compile_program, run
 from metellus_b200.compute.elementwise import BroadcastSpec
 from metellus_b200.orchestrator.builder import Operations
+from metellus_b200.runtime.cache import PagedCache
 
-__all__ = ["BroadcastSpec", "Executable", "Operations", "RunResult", "cache_read", "cache_write", "compile_program",
+__all__ = ["BroadcastSpec", "Executable", "Operations", "PagedCache", "RunResult", "cache_read", "cache_write", "compile_program",
            "paged_attention", "run"]

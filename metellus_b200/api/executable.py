@@ -27,10 +27,11 @@ import numpy as np
 from metellus_b200.api.run import compile_program
 from metellus_b200.orchestrator.builder import Operations
 from metellus_b200.orchestrator.kernel_group import STATUS_KEY
-from metellus_b200.orchestrator.scheduler import buffer_sizes, dispatch_of, scratch_of
+from metellus_b200.orchestrator.assembly.cache import cache_keys
+from metellus_b200.orchestrator.scheduler import buffer_sizes, check_slots, dispatch_of, scratch_of
 from metellus_b200.runtime import backend
 from metellus_b200.runtime.buffer import Buffer
-from metellus_b200.runtime.program import CheckStatus
+from metellus_b200.runtime.program import BindCache, CheckStatus
 
 
 class Executable:
@@ -42,7 +43,8 @@ class Executable:
         program = ops.build()
         produced = {op.out.name for op in program}
         used = {t.name for op in program for t in op.inputs}
-        self.outputs = tuple(outputs) if outputs is not None else tuple(sorted(produced - used))
+        self.outputs = (tuple(outputs) if outputs is not None
+                        else tuple(sorted(n for n in produced - used if tensors[n].dtype != "cache")))
         bound = {k for g in self.groups for k in g.bindings}
         for name in self.outputs:
             if name not in tensors:
@@ -52,8 +54,15 @@ class Executable:
         self.input_keys = {name: tensors[name].buffer_key for name in ops.uploads}
         sizes = buffer_sizes(ops, self.groups)
         self.env: dict[str, Buffer] = {}
+        self._cache_keys: set[str] = set()
         for name, arr in ops.uploads.items():
+            if tensors[name].dtype == "int32":
+                check_slots(ops, name, arr)
             self.env[tensors[name].buffer_key] = Buffer.from_numpy(arr)
+        # a cache's buffers are its own: bound here, not released with the program
+        for name, cache in ops.caches.items():
+            BindCache(name=name, cache=cache).execute(self.env)
+            self._cache_keys.update(cache_keys(name, cache))
         for k, n in scratch_of(self.groups).items():
             self.env[k] = Buffer.zeros(n)
         for g in self.groups:
@@ -74,6 +83,8 @@ class Executable:
     # -- execution ------------------------------------------------------------------
 
     def _launch(self) -> None:
+        for k in self._cache_keys:
+            _ = self.env[k].handle  # raises where its cache has been released: the graph holds the address
         if self._graph is not None:
             backend.graph_launch(self._graph)
             return
@@ -104,7 +115,14 @@ class Executable:
             if tuple(np.shape(arr)) != tuple(tensors[name].shape):
                 raise ValueError(f"Executable: input {name!r} has shape {np.shape(arr)}, "
                                  f"expected {tensors[name].shape}")
-            self.env[self.input_keys[name]].write(np.asarray(arr, dtype=np.float32), wait=False)
+            if tensors[name].dtype == "int32":
+                arr = np.asarray(arr)
+                if arr.dtype != np.int32:
+                    raise ValueError(f"Executable: input {name!r} must be int32, got {arr.dtype}")
+                check_slots(self.ops, name, arr)
+            else:
+                arr = np.asarray(arr, dtype=np.float32)
+            self.env[self.input_keys[name]].write(arr, wait=False)
         if self._read_pending:  # the previous call's downloads must finish before the outputs change
             backend.stream_wait_event(self._read_done)
         self._launch()
@@ -147,8 +165,9 @@ class Executable:
         if self._graph is not None:
             backend.graph_destroy(self._graph)
             self._graph = None
-        for b in self.env.values():
-            b.release()
+        for key, b in self.env.items():
+            if key not in self._cache_keys:
+                b.release()
         self.env.clear()
 
     def __del__(self) -> None:

@@ -130,6 +130,13 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
     if (!tiled || scale < 0.0) return attend_by_rows(a, st);  // tiles compare scores before they are scaled
     uint64_t need = 0;
     if (int rc = attend_tiles(a, false, nullptr, &need, dev, st)) return rc;
+    if (need && !workspace && !stream) {
+        // this library's stream: workspace from its pool, given back in the stream's order
+        RT_CHECK(cudaMallocAsync(&workspace, need, st));
+        const int rc = attend_tiles(a, true, workspace, &need, dev, st);
+        RT_CHECK(cudaFreeAsync(workspace, st));
+        return rc;
+    }
     if (need && (!workspace || workspace_bytes < need))
         return bad_argument("%s: the workspace has %llu bytes, %llu are needed", who,
                             (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)need);

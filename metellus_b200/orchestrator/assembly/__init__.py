@@ -25,10 +25,12 @@ _ELEMENTWISE = {
 }
 _MULTI = {FusionStrategy.MULTI_PRODUCER_CONVERGENT, FusionStrategy.DIAMOND_SHARED,
           FusionStrategy.DUAL_GEMM_EPILOGUE}
+_CACHE = {FusionStrategy.CACHE_WRITE, FusionStrategy.CACHE_READ, FusionStrategy.PAGED_ATTENTION}
 
 
 def assemble(vertex: Vertex, *, function_name: str | None = None) -> KernelGroup:
     from metellus_b200.orchestrator.assembly.attention import assemble_attention
+    from metellus_b200.orchestrator.assembly.cache import assemble_cache_op
     from metellus_b200.orchestrator.assembly.elementwise import assemble_elementwise
     from metellus_b200.orchestrator.assembly.matmul import assemble_matmul
     from metellus_b200.orchestrator.assembly.multi_anchor import assemble_multi_anchor
@@ -52,6 +54,8 @@ def assemble(vertex: Vertex, *, function_name: str | None = None) -> KernelGroup
         return assemble_row_resident(d, function_name)
     if s is FusionStrategy.FUSED_ATTENTION:
         return assemble_attention(d, function_name)
+    if s in _CACHE:
+        return assemble_cache_op(d, function_name)
     raise ValueError(f"unknown strategy {s!r}")
 
 

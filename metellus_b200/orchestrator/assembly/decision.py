@@ -15,9 +15,12 @@ from dataclasses import dataclass
 from metellus_b200.compute.elementwise import TERNARY_EXPRESSIONS
 from metellus_b200.orchestrator.graph import Vertex
 from metellus_b200.orchestrator.ir import (
+    CacheReadOp,
+    CacheWriteOp,
     ElementwiseOp,
     MatmulOp,
     Op,
+    PagedAttentionOp,
     ReductionOp,
     Scalar,
     ShapeOp,
@@ -82,6 +85,11 @@ def is_linear_chain(ops: tuple[ElementwiseOp, ...]) -> bool:
 def classify(vertex: Vertex) -> DecisionView:
     ops = vertex.ops
     outs = tuple(vertex.outputs)
+    for kind, strategy in ((CacheWriteOp, FusionStrategy.CACHE_WRITE), (CacheReadOp, FusionStrategy.CACHE_READ),
+                           (PagedAttentionOp, FusionStrategy.PAGED_ATTENTION)):
+        if any(isinstance(op, kind) for op in ops):
+            assert len(ops) == 1, "an op on a cache must be standalone"
+            return DecisionView(strategy=strategy, ops=ops, outputs=outs)
     shape_op = next((op for op in ops if isinstance(op, ShapeOp)), None)
     if shape_op is not None:
         assert len(ops) == 1, "ShapeOp must be standalone"

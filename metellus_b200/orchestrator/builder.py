@@ -16,6 +16,11 @@ A failed op leaves the builder unchanged: the output name is registered only aft
 the op has been constructed. ``build()`` returns a copy of the op list, so the
 builder can keep growing afterwards.
 
+Beyond the reference, a program may work on paged key-value caches: ``cache`` declares a
+``PagedCache``, ``indices`` int32 tensors for slots, page tables and lengths, and
+``cache_write`` / ``cache_read`` / ``paged_attention`` are ops like the others. A write
+makes a new name of the cache, and only the newest name can be used.
+
 Batched (rank-3) tensors are accepted everywhere the IR accepts them; ``matmul``
 infers ``a.shape[:-1] + (b.shape[-1],)`` as its output shape.
 """
@@ -29,17 +34,21 @@ import numpy as np
 
 from metellus_b200.compute.elementwise import BroadcastSpec
 from metellus_b200.orchestrator.ir import (
+    CacheReadOp,
+    CacheWriteOp,
     ElementwiseOp,
     Layout,
     MatmulOp,
     Op,
     OperandValue,
+    PagedAttentionOp,
     Program,
     ReductionOp,
     Scalar,
     ShapeOp,
     Tensor,
 )
+from metellus_b200.runtime.cache import PagedCache
 
 
 def addressable_elements(t: Tensor) -> int:
@@ -58,6 +67,9 @@ class Operations:
         self._by_name: dict[str, Tensor] = {}
         self._program: Program = []
         self._payloads: dict[str, np.ndarray] = {}
+        self._caches: dict[str, PagedCache] = {}   # by the name it was declared under
+        self._newest: dict[str, str] = {}          # cache -> its newest name
+        self._cache_read: set[str] = set()         # names of caches that an op has read
 
     # -- lookups --------------------------------------------------------------
 
@@ -112,6 +124,8 @@ class Operations:
         if arr.dtype != np.float32:
             raise ValueError(f"from_numpy({name!r}): the array must be float32, got {arr.dtype}")
         t = self.input(name, tuple(arr.shape))
+        if t.dtype in ("int32", "cache"):
+            raise ValueError(f"from_numpy: {name!r} is {t.dtype}; indices() takes int32 arrays")
         if t.buffer_key != name:
             raise ValueError(f"from_numpy: {name!r} is a view of {t.buffer_key!r}; only a storage owner "
                              "can receive an upload")
@@ -124,6 +138,31 @@ class Operations:
                              f"row_stride={t.row_stride}, col_stride={t.col_stride} the tensor can address "
                              f"{reach} elements")
         self._payloads[name] = arr
+        return t
+
+    def indices(self, arr: np.ndarray, name: str) -> Tensor:
+        """Declare ``name`` as an int32 tensor (slots, page tables, lengths) with ``arr``'s shape and
+        record ``arr`` as its upload. The array must be int32, of 1 or 2 dimensions."""
+        if arr.dtype != np.int32 or arr.ndim not in (1, 2):
+            raise ValueError(f"indices({name!r}): the array must be int32 of 1 or 2 dimensions, got {arr.dtype} "
+                             f"of {arr.ndim}")
+        if name in self._by_name:
+            raise ValueError(f"tensor {name!r} already declared")
+        self._by_name[name] = t = Tensor(name=name, shape=tuple(arr.shape), dtype="int32")
+        self._payloads[name] = arr
+        return t
+
+    def cache(self, cache: PagedCache, name: str) -> Tensor:
+        """Declare ``cache`` under ``name``: storage that the program's ops read and write and
+        that outlives it."""
+        if name in self._by_name:
+            raise ValueError(f"tensor {name!r} already declared")
+        if any(c is cache for c in self._caches.values()):
+            raise ValueError(f"cache({name!r}): the cache is already declared under another name")
+        t = Tensor(name=name, shape=(cache.pages, cache.page_size, cache.kv_heads * cache.head_dim), dtype="cache")
+        self._by_name[name] = t
+        self._caches[name] = cache
+        self._newest[name] = name
         return t
 
     # -- ops -------------------------------------------------------------------
@@ -171,12 +210,69 @@ class Operations:
         shape = tuple(keep) or (1,)
         return self._emit(out, shape, lambda o: ReductionOp(out=o, op=op, input=src, axis=axis))
 
+    # -- paged caches ------------------------------------------------------------
+
+    def _newest_cache(self, name: str) -> tuple[Tensor, PagedCache]:
+        t = self._lookup(name)
+        if t.dtype != "cache":
+            raise ValueError(f"{name!r} is not a cache (declare one with cache())")
+        newest = self._newest[t.buffer_key]
+        if newest != name:
+            raise ValueError(f"cache {name!r} was written since: its newest name is {newest!r}")
+        return t, self._caches[t.buffer_key]
+
+    def cache_write(self, k: str, v: str, cache: str, slots: str, out: str) -> Tensor:
+        """Store the rows of ``k`` and ``v`` (``(tokens, kv_heads, head_dim)``, or ``(tokens,
+        kv_heads * head_dim)`` as a matmul leaves them) in the cache's slots ``slots[i]``
+        (int32; outside the cache, such as -1: skipped). ``out`` is the cache's name from
+        here on. Slots must be distinct. A cache that the program has already read
+        cannot be written again in it."""
+        tc, paged = self._newest_cache(cache)
+        if cache in self._cache_read:
+            raise ValueError(f"cache_write: cache {cache!r} has been read in this program; write it first")
+        tk, tv, ts = self._lookup(k), self._lookup(v), self._lookup(slots)
+        if out in self._by_name:
+            raise ValueError(f"output tensor {out!r} already exists; the IR is SSA, so every op "
+                             "needs a new output name")
+        result = Tensor(name=out, shape=tc.shape, dtype="cache", buffer_key=tc.buffer_key)
+        op = CacheWriteOp(out=result, cache=tc, k=tk, v=tv, slots=ts, paged=paged)
+        self._by_name[out] = result
+        self._program.append(op)
+        self._newest[tc.buffer_key] = out
+        return result
+
+    def cache_read(self, cache: str, slots: str, out: str, part: str = "k") -> Tensor:
+        """The keys (``part="k"``) or values (``"v"``) in ``slots`` (int32), as float32
+        ``(kv_heads, tokens, head_dim)``; slots outside the cache read as zeros."""
+        tc, paged = self._newest_cache(cache)
+        ts = self._lookup(slots)
+        shape = (paged.kv_heads, ts.shape[0] if ts.shape else 1, paged.head_dim)
+        t = self._emit(out, shape, lambda o: CacheReadOp(out=o, cache=tc, slots=ts, part=part, paged=paged))
+        self._cache_read.add(cache)
+        return t
+
+    def paged_attention(self, q: str, cache: str, tables: str, lengths: str, out: str, scale: float | None = None,
+                        window: int = 0) -> Tensor:
+        """Attention of one query row per sequence over the cache: ``q`` is ``(batch, heads, head_dim)``
+        or ``(batch, heads * head_dim)``, ``out`` the same; ``tables`` int32 ``(batch, width)``,
+        ``lengths`` int32 ``(batch,)``. ``scale`` defaults to ``head_dim ** -0.5``;
+        ``window`` > 0 shows the last ``window`` tokens only. See ``metellus_b200.paged_attention``."""
+        tc, paged = self._newest_cache(cache)
+        tq, tt, tl = self._lookup(q), self._lookup(tables), self._lookup(lengths)
+        t = self._emit(out, tq.shape, lambda o: PagedAttentionOp(
+            out=o, q=tq, cache=tc, tables=tt, lengths=tl, paged=paged, window=int(window),
+            scale=float(paged.head_dim ** -0.5 if scale is None else scale)))
+        self._cache_read.add(cache)
+        return t
+
     # -- views -----------------------------------------------------------------
 
     def transpose(self, name: str, out: str) -> Tensor:
         """``out`` = the transpose of ``name``'s (inner) matrix as a view: same storage,
         swapped shape and strides, no op."""
         src = self._lookup(name)
+        if src.dtype == "cache":
+            raise ValueError(f"transpose: {name!r} is a cache; read it with cache_read()")
         self._require_fresh_view_name(out, "transpose")
         self._by_name[out] = view = src.transpose(out)
         return view
@@ -186,6 +282,8 @@ class Operations:
         op); otherwise a ``ShapeOp`` that gathers the source into a new contiguous
         1-D or 2-D tensor."""
         src = self._lookup(name)
+        if src.dtype == "cache":
+            raise ValueError(f"reshape: {name!r} is a cache; read it with cache_read()")
         self._require_fresh_view_name(out, "reshape")
         target = tuple(new_shape)
         if src.can_reshape_as_view(target):
@@ -206,6 +304,10 @@ class Operations:
     @property
     def tensors(self) -> dict[str, Tensor]:
         return dict(self._by_name)
+
+    @property
+    def caches(self) -> dict[str, PagedCache]:
+        return dict(self._caches)
 
     @property
     def uploads(self) -> dict[str, np.ndarray]:

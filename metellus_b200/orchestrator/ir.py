@@ -12,7 +12,13 @@ Every op checks its operand shapes, broadcast modes and dtypes when it is
 constructed, and raises ``ValueError`` naming the problem; the builder relies on
 that instead of checking twice.
 
-Beyond the reference: rank-3 tensors ``(B, M, N)`` are batched matrices. Each op
+Beyond the reference: int32 tensors (``dtype="int32"``: page tables, slots, lengths) and
+paged key-value caches (``dtype="cache"``), which only the cache ops read
+(``CacheWriteOp``, ``CacheReadOp``, ``PagedAttentionOp``). A cache is storage that outlives
+the program; each write makes a new name of it, so that the order of writes and reads
+is in the data flow like any other.
+
+Rank-3 tensors ``(B, M, N)`` are batched matrices. Each op
 then applies to every batch index independently (batched attention without B copies
 of the program); broadcasts and reductions act on the inner matrix. Kernels map the
 batch to ``gridDim.z`` and the multi-GPU runner shards it.
@@ -82,7 +88,7 @@ class Tensor:
 
     @property
     def nbytes(self) -> int:
-        return 4 * self.element_count   # the IR is fp32 throughout
+        return 4 * self.element_count   # float32 and int32
 
     @property
     def batch(self) -> int:
@@ -198,6 +204,12 @@ def _check_secondary(role: str, primary: Tensor, operand: OperandValue, mode: Br
                      f"(expected {want})")
 
 
+def _check_float(what: str, *operands: OperandValue) -> None:
+    for t in operands:
+        if isinstance(t, Tensor) and t.dtype in ("int32", "cache"):
+            raise ValueError(f"{what} works on float32 tensors; {t.name!r} is {t.dtype}")
+
+
 @dataclass(frozen=True)
 class MatmulOp:
     """``out = a @ b``; for rank-3 operands, per batch index."""
@@ -246,6 +258,7 @@ class ElementwiseOp:
         if not isinstance(primary, Tensor):
             raise ValueError(f"elementwise {self.op!r}: operand[0] must be a tensor, got {primary!r}; scalars "
                              "may only be secondary operands")
+        _check_float(f"elementwise {self.op!r}", *self.operands)
         if self.out.shape != primary.shape:
             raise ValueError(f"elementwise out shape {self.out.shape} must match primary operand shape "
                              f"{primary.shape}")
@@ -271,6 +284,7 @@ class ReductionOp:
 
     def __post_init__(self) -> None:
         shape = self.input.shape
+        _check_float(f"reduction {self.op!r}", self.input)
         if len(shape) not in (2, 3):
             raise ValueError(f"reduction input must be 2D (or batched 3D); got shape {shape}")
         if self.axis not in (len(shape) - 1, -1):
@@ -308,5 +322,127 @@ class ShapeOp:
         return (self.input,)
 
 
-Op = MatmulOp | ElementwiseOp | ReductionOp | ShapeOp
+def _check_cache(what: str, cache: Tensor) -> None:
+    if cache.dtype != "cache":
+        raise ValueError(f"{what}: {cache.name!r} is not a cache (declare one with cache())")
+
+
+def _check_int32(what: str, t: Tensor, rank: int) -> None:
+    if t.dtype != "int32" or len(t.shape) != rank:
+        raise ValueError(f"{what}: {t.name!r} must be an int32 tensor of {rank} dimension(s); got {t.dtype} {t.shape}")
+    if rank == 2 and t.shape[1] > 1 and t.col_stride != 1:
+        raise ValueError(f"{what}: the rows of {t.name!r} must be contiguous (it is a transposed view)")
+
+
+def rows_of_heads(what: str, t: Tensor, heads: int | None, head_dim: int) -> tuple[int, int, tuple[int, int, int]]:
+    """(rows, heads, strides) of a float32 tensor of rows of heads: ``(rows, heads, head_dim)``, or
+    ``(rows, heads * head_dim)`` as a projection's product leaves it. ``heads`` None: as many as
+    there are."""
+    _check_float(what, t)
+    if len(t.shape) == 3:
+        rows, n, d = t.shape
+        strides = (t.batch_stride, t.row_stride, t.col_stride)
+    elif len(t.shape) == 2 and t.shape[1] % head_dim == 0:
+        rows, n, d = t.shape[0], t.shape[1] // head_dim, head_dim
+        strides = (t.row_stride, head_dim * t.col_stride, t.col_stride)
+    else:
+        raise ValueError(f"{what}: {t.name!r} {t.shape} is not rows of heads of {head_dim}")
+    if d != head_dim or (heads is not None and n != heads):
+        raise ValueError(f"{what}: {t.name!r} {t.shape} is not rows of {heads if heads is not None else 'the'} "
+                         f"heads of {head_dim}")
+    if d > 1 and strides[2] != 1:
+        raise ValueError(f"{what}: the rows of {t.name!r} must be contiguous (it is a transposed view)")
+    return rows, n, strides
+
+
+@dataclass(frozen=True)
+class CacheWriteOp:
+    """Store rows ``k[i]``, ``v[i]`` in slot ``slots[i]`` of the cache; ``out`` is the cache's new
+    name. ``paged`` is the ``PagedCache`` behind it."""
+
+    out: Tensor
+    cache: Tensor
+    k: Tensor
+    v: Tensor
+    slots: Tensor
+    paged: object
+
+    def __post_init__(self) -> None:
+        what = "cache_write"
+        _check_cache(what, self.cache)
+        _check_int32(what, self.slots, 1)
+        for t in (self.k, self.v):
+            rows, _, _ = rows_of_heads(what, t, self.paged.kv_heads, self.paged.head_dim)
+            if rows != self.slots.shape[0]:
+                raise ValueError(f"{what}: {t.name!r} has {rows} rows, {self.slots.name!r} {self.slots.shape[0]}")
+
+    @property
+    def inputs(self) -> tuple[Tensor, ...]:
+        return (self.cache, self.k, self.v, self.slots)
+
+
+@dataclass(frozen=True)
+class CacheReadOp:
+    """The rows of K or V (``part``) in ``slots``, as float32 ``(kv_heads, tokens, head_dim)``:
+    batched matrices, as matmul takes them."""
+
+    out: Tensor
+    cache: Tensor
+    slots: Tensor
+    part: str
+    paged: object
+
+    def __post_init__(self) -> None:
+        what = "cache_read"
+        _check_cache(what, self.cache)
+        _check_int32(what, self.slots, 1)
+        if self.part not in ("k", "v"):
+            raise ValueError(f"{what}: part must be 'k' or 'v', got {self.part!r}")
+        want = (self.paged.kv_heads, self.slots.shape[0], self.paged.head_dim)
+        if self.out.shape != want:
+            raise ValueError(f"{what}: out shape {self.out.shape} is not {want}")
+
+    @property
+    def inputs(self) -> tuple[Tensor, ...]:
+        return (self.cache, self.slots)
+
+
+@dataclass(frozen=True)
+class PagedAttentionOp:
+    """Attention of one query row per sequence over the cache (``metellus_b200.api.paged``)."""
+
+    out: Tensor
+    q: Tensor
+    cache: Tensor
+    tables: Tensor
+    lengths: Tensor
+    scale: float
+    window: int
+    paged: object
+
+    def __post_init__(self) -> None:
+        what = "paged_attention"
+        _check_cache(what, self.cache)
+        rows, heads, _ = rows_of_heads(what, self.q, None, self.paged.head_dim)
+        if heads % self.paged.kv_heads:
+            raise ValueError(f"{what}: {heads} query heads are not a multiple of {self.paged.kv_heads} key-value heads")
+        _check_int32(what, self.tables, 2)
+        _check_int32(what, self.lengths, 1)
+        if self.tables.shape[0] != rows or self.lengths.shape[0] != rows:
+            raise ValueError(f"{what}: q has {rows} rows, {self.tables.name!r} {self.tables.shape[0]}, "
+                             f"{self.lengths.name!r} {self.lengths.shape[0]}")
+        if not math.isfinite(self.scale):
+            raise ValueError(f"{what}: scale must be finite, got {self.scale}")
+        if self.window < 0:
+            raise ValueError(f"{what}: window must not be negative, got {self.window}")
+        if self.out.shape != self.q.shape:
+            raise ValueError(f"{what}: out shape {self.out.shape} is not q's {self.q.shape}")
+
+    @property
+    def inputs(self) -> tuple[Tensor, ...]:
+        return (self.q, self.cache, self.tables, self.lengths)
+
+
+CacheOp = CacheWriteOp | CacheReadOp | PagedAttentionOp
+Op = MatmulOp | ElementwiseOp | ReductionOp | ShapeOp | CacheOp
 Program = list[Op]

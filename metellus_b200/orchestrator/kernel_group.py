@@ -43,6 +43,10 @@ class FusionStrategy(StrEnum):
     ROW_RESIDENT = "row_resident"
     FUSED_ATTENTION = "fused_attention"
     DUAL_GEMM_EPILOGUE = "dual_gemm_epilogue"
+    # native kernels on paged key-value caches, one op each
+    CACHE_WRITE = "cache_write"
+    CACHE_READ = "cache_read"
+    PAGED_ATTENTION = "paged_attention"
 
 
 @dataclass(frozen=True)

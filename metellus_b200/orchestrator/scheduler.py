@@ -16,11 +16,14 @@ from __future__ import annotations
 
 import numpy as np
 
+from metellus_b200.orchestrator.assembly.cache import cache_keys
 from metellus_b200.orchestrator.builder import Operations
 from metellus_b200.orchestrator.dag import build_dag
+from metellus_b200.orchestrator.ir import CacheWriteOp
 from metellus_b200.orchestrator.kernel_group import STATUS_KEY, KernelGroup
 from metellus_b200.runtime.program import (
     Allocate,
+    BindCache,
     CheckStatus,
     Fill,
     Dispatch,
@@ -29,6 +32,7 @@ from metellus_b200.runtime.program import (
     FromNumpy,
     Runtime,
     RuntimeFragment,
+    Unbind,
 )
 
 
@@ -61,6 +65,16 @@ def buffer_sizes(ops: Operations, groups: tuple[KernelGroup, ...]) -> dict[str, 
     return sizes
 
 
+def check_slots(ops: Operations, name: str, arr: np.ndarray) -> None:
+    """Slots that come from the host must be distinct wherever a write uses them: two rows in one
+    slot would leave a mixture there. (Padding, below 0, may repeat.)"""
+    for op in ops.build():
+        if isinstance(op, CacheWriteOp) and op.slots.buffer_key == name:
+            used = arr[(arr >= 0) & (arr < op.paged.slots)]
+            if np.unique(used).size != used.size:
+                raise ValueError(f"cache_write: slots {name!r} holds a slot twice")
+
+
 def schedule(ops: Operations, groups: tuple[KernelGroup, ...], *, profile: bool = False) -> Runtime:
     program = ops.build()
     dag = build_dag(program)
@@ -71,7 +85,7 @@ def schedule(ops: Operations, groups: tuple[KernelGroup, ...], *, profile: bool 
     required: set[str] = set()
     for n in dag.inputs:
         bk = tensors[n].buffer_key
-        if bk not in produced_keys:
+        if bk not in produced_keys and tensors[n].dtype != "cache":
             required.add(bk)
     provided = set(uploads)
     missing, extra = required - provided, provided - required
@@ -98,12 +112,18 @@ def schedule(ops: Operations, groups: tuple[KernelGroup, ...], *, profile: bool 
 
     steps: list[RuntimeFragment] = []
     for name, arr in uploads.items():
+        if tensors[name].dtype == "int32":
+            check_slots(ops, name, arr)
         steps.append(FromNumpy(name=tensors[name].buffer_key, source=arr))
+    cached: set[str] = set()
+    for name, cache in ops.caches.items():
+        steps.append(BindCache(name=name, cache=cache))
+        cached.update(cache_keys(name, cache))
     scratch = scratch_of(groups)
     for k, n in scratch.items():
         steps.append(Allocate(name=k, nbytes=n))
         steps.append(Fill(name=k, byte_value=0))
-    seen = set(input_keys)
+    seen = set(input_keys) | cached
     for g in groups:
         for k in g.bindings:
             if k not in seen:
@@ -114,7 +134,7 @@ def schedule(ops: Operations, groups: tuple[KernelGroup, ...], *, profile: bool 
     for i, g in enumerate(groups):
         steps.append(dispatch_of(g, f"t_{i}" if profile else None))
         for k in dict.fromkeys(g.bindings):
-            if k in freed or last_use.get(k) != i:
+            if k in freed or last_use.get(k) != i or k in cached:
                 continue
             names = names_per_key.get(k, ())
             for vn in (n for n in names if n != k):
@@ -128,6 +148,8 @@ def schedule(ops: Operations, groups: tuple[KernelGroup, ...], *, profile: bool 
             else:
                 steps.append(Free(name=k))
             freed.add(k)
+    for k in sorted(cached):
+        steps.append(Unbind(name=k))
     for k in scratch:
         if k == STATUS_KEY:
             steps.append(CheckStatus(name=k))

@@ -421,6 +421,29 @@ def reduce_rows(in_handle: int, out_handle: int, rows: int, cols: int, ld: int, 
     return float(ms.value) if timed else None
 
 
+# -- paged key-value caches: on this library's stream, workspaces from its pool -----------
+
+
+def cache_write(cache: MtPagedCache, arrays, *, dev: int | None = None) -> None:
+    """``arrays``: k, v, slots."""
+    k, v, slots = arrays
+    _check(lib().mt_cache_write(_device if dev is None else dev, k, v, cache, slots, None))
+
+
+def cache_read(cache: MtPagedCache, arrays, part: str, *, dev: int | None = None) -> None:
+    """``arrays``: slots, the rows of ``part`` ("k" or "v")."""
+    slots, rows = arrays
+    _check(lib().mt_cache_read(_device if dev is None else dev, cache, slots, rows if part == "k" else None,
+                               rows if part == "v" else None, None))
+
+
+def paged_attention(cache: MtPagedCache, arrays, scale: float, window: int, *, dev: int | None = None) -> None:
+    """``arrays``: q, tables, lengths, out."""
+    q, tables, lengths, out = arrays
+    _check(lib().mt_paged_attention(_device if dev is None else dev, q, cache, tables, lengths, out, None, scale, window,
+                                    None, 0, None))
+
+
 # -- NCCL ------------------------------------------------------------------------------
 
 NCCL_ID_BYTES = 128

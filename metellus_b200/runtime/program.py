@@ -41,6 +41,27 @@ class Allocate:
 
 
 @dataclass(frozen=True)
+class BindCache:
+    """Put a ``PagedCache``'s buffers under their env keys; ``Unbind`` takes one out again
+    without releasing it (the cache outlives the program)."""
+
+    name: str
+    cache: Any
+
+    def execute(self, env: Env) -> None:
+        for part in self.cache.parts:
+            env[f"{self.name}.{part}"] = self.cache.buffer(part)
+
+
+@dataclass(frozen=True)
+class Unbind:
+    name: str
+
+    def execute(self, env: Env) -> None:
+        env.pop(self.name)
+
+
+@dataclass(frozen=True)
 class Free:
     name: str
 
@@ -203,6 +224,23 @@ class Kernel:
         _ = self.handle
 
 
+CACHE_ENTRIES = ("mt_cache_write", "mt_cache_read", "mt_paged_attention")
+
+
+@dataclass(frozen=True)
+class ArraySpec:
+    """A bound buffer as an array of a native entry point (strides in elements)."""
+
+    dtype: str
+    shape: tuple[int, ...]
+    strides: tuple[int, ...]
+
+    def at(self, handle: int):
+        from metellus_b200.runtime.cache import device_array
+
+        return device_array(handle, self.dtype, self.shape, self.strides)
+
+
 class NativeKernel(Kernel):
     """A kernel compiled ahead of time into ``libmetellus_cuda.so`` and launched
     through its own C-ABI entry point (no NVRTC source). ``entry`` names the
@@ -243,6 +281,22 @@ class NativeKernel(Kernel):
             t1.record()
             backend.sync()
             return t0.elapsed_ms(t1)
+        if self.entry in CACHE_ENTRIES:
+            # handles: the entry point's arrays, then the cache's
+            paged, specs, *more = self.params
+            arrays = [s.at(h) for s, h in zip(specs, handles)]
+            cache = paged.descriptor(handles[len(specs):])
+            call = {"mt_cache_write": backend.cache_write, "mt_cache_read": backend.cache_read,
+                    "mt_paged_attention": backend.paged_attention}[self.entry]
+            if not timed:
+                call(cache, arrays, *more)
+                return None
+            t0, t1 = backend.Event(), backend.Event()
+            t0.record()
+            call(cache, arrays, *more)
+            t1.record()
+            backend.sync()
+            return t0.elapsed_ms(t1)
         raise ValueError(f"unknown native kernel {self.entry!r}")
 
 
@@ -267,6 +321,9 @@ class Dispatch:
             )
         handles = tuple(env[name].handle for name in self.bindings)
         if isinstance(self.kernel, NativeKernel):
+            # the paged-cache entry points take addresses, which do not tell their device
+            if self.kernel.entry in CACHE_ENTRIES and any(env[n].device != backend.current_device() for n in self.bindings):
+                raise RuntimeError(f"{self.kernel.entry}: a buffer is not on device {backend.current_device()}")
             t = self.kernel.launch(list(handles), self.time_key is not None)
             if self.time_key is not None:
                 env[self.time_key] = float(t)
