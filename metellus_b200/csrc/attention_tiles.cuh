@@ -171,8 +171,8 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr int ROW = DP * EB;               // bytes of a (padded) cache row
     static constexpr int CPR = ROW / 16;              // its 16-byte pieces
     // tokens a tile: 8-bit rows are short, and a tile's chain of instructions takes as long
-    static constexpr int TW = kScaled ? 32 : 16, TB = TW / 16;
-    static constexpr int STAGE = 2 * TW * ROW + (kScaled ? 2 * TW * 4 : 0);  // rows of K, of V, their scales
+    static constexpr int TW = kScaled && DP <= 128 ? 32 : 16, TB = TW / 16;
+    static constexpr int STAGE = 2 * TW * ROW + (kScaled ? 256 : 0);  // rows of K, of V, scales of 32 tokens each
     static constexpr int KS = CT == MT_F32 ? DP / 8 : DP / 16;    // steps of K Q^T
     // pieces of a query: fp16 11 bits, bf16 8 bits, tf32 11 bits each
     static constexpr int QP = CT == MT_F32 ? 2 : !kQ32 ? 1 : kBf16 ? 3 : 2;
@@ -226,83 +226,65 @@ template <int TW> __device__ inline void enter_sequence(Cursor& c, const TileArg
 }
 __device__ inline int length_of(const TileArgs& t, int b) { return t.a.lengths[(int64_t)b * t.a.length_seq]; }
 
-// The cuts: every range gets tiles / ranges, the first ones one more.
-struct Ranges {
+// The cuts of the line of all sequences' tiles: every range gets tiles / ranges, the first ones
+// one more. Every warp works them out for itself, without barriers: each lane sums a run of
+// sequences, and a scan over the lanes finds the one that a range begins in.
+template <int TW> struct Cuts {
+    const TileArgs& t;
+    int b0, b1, mine;  // this lane's sequences and their tiles
     uint32_t base, more;
-    Ranges() = default;
-    __device__ Ranges(const TileArgs& t, int tiles) { base = t.ranges.div((uint32_t)tiles, &more); }
-    __device__ int first(uint32_t c) const { return (int)(c * base + min(c, more)); }
-    __device__ int owner(uint32_t u) const {
+
+    __device__ int tiles_of(int b, Cursor& c) const {
+        enter_sequence<TW>(c, t, length_of(t, b));
+        return c.tiles;
+    }
+    __device__ explicit Cuts(const TileArgs& args) : t(args), mine(0) {
+        const int per = (t.a.batch + 31) / 32, lane = threadIdx.x & 31;
+        b0 = min(lane * per, t.a.batch);
+        b1 = min(b0 + per, t.a.batch);
+        Cursor c;
+        for (int b = b0; b < b1; ++b) mine += tiles_of(b, c);
+        base = t.ranges.div((uint32_t)__reduce_add_sync(0xffffffffu, mine), &more);
+    }
+    __device__ int first(uint32_t range) const { return (int)(range * base + min(range, more)); }
+    __device__ int owner(uint32_t tile) const {
         const uint32_t big = more * (base + 1);
-        return (int)(u < big ? u / (base + 1) : more + (u - big) / base);  // base is not 0 in the second
+        return (int)(tile < big ? tile / (base + 1) : more + (tile - big) / base);  // base is not 0 in the second
+    }
+    // The tiles of the sequences before b (all lanes of a warp call it).
+    __device__ int before(int b) const {
+        Cursor c;
+        int n = 0;
+        for (int i = b0; i < min(b1, b); ++i) n += tiles_of(i, c);
+        return __reduce_add_sync(0xffffffffu, n);
+    }
+    // The cursor at a range's first tile; returns how many tiles the range has.
+    __device__ int locate(int range, Cursor& c) const {
+        const int lane = threadIdx.x & 31, target = first(range), count = first(range + 1) - target;
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        const uint32_t who = __ballot_sync(0xffffffffu, target < upto);
+        if (!who || count == 0) return 0;  // behind the end
+        const int src = __ffs(who) - 1;
+        int b = b0, p = upto - mine, length = 0;
+        if (lane == src)
+            for (; b < b1; ++b) {
+                length = length_of(t, b);
+                enter_sequence<TW>(c, t, length);
+                if (target < p + c.tiles) break;
+                p += c.tiles;
+            }
+        c.b = __shfl_sync(0xffffffffu, b, src);
+        p = __shfl_sync(0xffffffffu, p, src);
+        enter_sequence<TW>(c, t, __shfl_sync(0xffffffffu, length, src));
+        c.tile = target - p;
+        return count;
     }
 };
-
-// Sums over the block of each thread's `mine`: all (total) and those of threads before it.
-template <int kThreads> __device__ inline int scan(int mine, int& total) {
-    __shared__ int sums[kThreads / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += o;
-    }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    int before = upto - mine;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) before += sums[w];
-        total += sums[w];
-    }
-    return before;
-}
-
-// Finds the first tiles of ranges range_of(0) .. range_of(kCount - 1) (all threads of the block
-// call it): the caller's cursor is at the first tile of range_of(g). Returns how many tiles
-// that range has. Every thread sums some sequences' tiles; a scan over the sums finds the
-// sequence.
-template <int TW, int kThreads, int kCount, class RangeOf>
-__device__ inline int locate(const TileArgs& t, RangeOf range_of, int g, Cursor& c, Ranges& ranges) {
-    __shared__ int found[kCount][3];
-    const int per = (t.a.batch + kThreads - 1) / kThreads;
-    const int b0 = threadIdx.x * per, b1 = min(b0 + per, t.a.batch);
-    int mine = 0, length = 0, total;
-    for (int b = b0; b < b1; ++b) {
-        length = length_of(t, b);
-        enter_sequence<TW>(c, t, length);
-        mine += c.tiles;
-    }
-    const int before = scan<kThreads>(mine, total);
-    ranges = Ranges(t, total);
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-        const int target = ranges.first(range_of(i));
-        int p = before;
-        if (p <= target && target < p + mine) {
-            int b = b0;
-            if (per > 1)
-                for (; b < b1; ++b) {
-                    length = length_of(t, b);
-                    enter_sequence<TW>(c, t, length);
-                    if (target < p + c.tiles) break;
-                    p += c.tiles;
-                }
-            found[i][0] = b;
-            found[i][1] = p;
-            found[i][2] = length;
-        }
-    }
-    __syncthreads();
-    const int u0 = ranges.first(range_of(g)), count = ranges.first(range_of(g) + 1) - u0;
-    if (count == 0) return 0;  // behind the end: nothing was found
-    c.b = found[g][0];
-    enter_sequence<TW>(c, t, found[g][2]);
-    c.tile = u0 - found[g][1];
-    return count;
-}
 
 template <int CT, class Q, int DP, int NT>
 __global__ void __launch_bounds__(Shape<CT, Q, DP, NT>::NW * 32, Shape<CT, Q, DP, NT>::BLOCKS)
@@ -334,9 +316,9 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         enter_sequence<TW>(in, t, length_of(t, in.b));
         tiles = in.tiles;
     } else {
-        Ranges ranges;
-        tiles = locate<TW, NW * 32, NW>(t, [&](int i) { return t.per_range.div((uint32_t)(blockIdx.x * NW + i)); }, warp, in, ranges);
-        if (tiles <= 0 || range >= (int)t.ranges.d) return;
+        if (range >= (int)t.ranges.d) return;
+        tiles = Cuts<TW>(t).locate(range, in);
+        if (tiles == 0) return;
     }
     in.next_length = in.b + 1 < a.batch ? length_of(t, in.b + 1) : 0;
 
@@ -396,7 +378,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     };
     auto copy_rows = [&](int slot, auto of_v, auto whole_tile) {
         constexpr bool kV = decltype(of_v)::value, kWhole = decltype(whole_tile)::value;
-        constexpr int kUnroll = kWhole ? TW * CPR / 32 : 1;  // the rare case's code stays small
+        constexpr int kCopies = TW * CPR / 32, kUnroll = kWhole || kCopies < 4 ? kCopies : 4;  // the rarer case's code stays small
         const uint32_t to = smem_address(ring + slot * Z::STAGE) + (kV ? TW * Z::ROW : 0);
 #pragma unroll kUnroll
         for (int i = 0; i < TW * CPR / 32; ++i) {
@@ -612,6 +594,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
             float s[TB][NT][4];
 #pragma unroll
             for (int b = 0; b < TB; ++b) {
+                // where they are not, `part` takes every second step: two short chains of products
                 float part[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -623,7 +606,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                         for (int p = 0; p < QP; ++p) {
                             const uint2 q = query(k, n, p);
-                            product<CT>(p == 0 && Z::kExact ? part[n] : s[b][n], x, q.x, q.y);
+                            product<CT>((Z::kExact ? p == 0 : k % 2 == 1) ? part[n] : s[b][n], x, q.x, q.y);
                         }
                     if constexpr (Z::kExact) {
                         if (k % 4 == 3 || k == KS - 1) {
@@ -666,6 +649,11 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         times_queries(c, r);
                     }
                 }
+                if constexpr (!Z::kExact)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[b][n][i] += part[n][i];
             }
             if constexpr (kScaled) {
                 const float* z = (const float*)(stage + 2 * TW * Z::ROW);
@@ -945,102 +933,95 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     copies_wait_all();
 }
 
-// Joins the parts of sequences that cuts crossed: block (x, r) row r of an item whose tiles lie
-// in several ranges. Which ones is known from the lengths, so it is found out while
-// attention_tiles still runs. x / items is a sequence, or, where there are fewer ranges
-// than sequences, a range: it stands for the sequence that it starts in the middle of, if
-// that ends in it.
+// Joins the parts of sequences that cuts crossed: block (x, y) the rows y * together .. of an
+// item whose tiles lie in several ranges. Which ones is known from the lengths, so it is
+// found out while attention_tiles still runs. x / items is a sequence, or, where there are
+// fewer ranges than sequences, a range: it stands for the sequence that it starts in the
+// middle of, if that ends in it. A block is kTeams teams of DP / 4 threads (4 dims each):
+// `together` rows (a power of two) at a time, kTeams / together parts of each.
+constexpr int kTeams = 8;
+
 template <class Q, int DP, int ROWS, int TW>
-__global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ TileArgs t, int by_sequence) {
-    constexpr int kLanes = DP / 4, kSide = 8, kJoinThreads = kLanes * kSide;  // threads a part, parts at a time
-    __shared__ float4 sm_o[kSide][kLanes];
-    __shared__ float2 sm_ml[kSide];
+__global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ TileArgs t, int by_sequence, int together) {
+    constexpr int kLanes = DP / 4;
+    __shared__ float4 sm_o[kTeams][kLanes];
+    __shared__ float2 sm_ml[kTeams];
     const AttentionArgs& a = t.a;
     asm volatile("griddepcontrol.launch_dependents;");
-    const int r = blockIdx.y;
     uint32_t item, row_block;
     const int x = (int)t.per_range.div(blockIdx.x, &item);
-    const int head = (int)t.row_blocks.div(item, &row_block) * a.group + (int)row_block * ROWS + r;
-    if ((int)row_block * ROWS + r >= a.group) return;
+    const int head0 = (int)t.row_blocks.div(item, &row_block) * a.group + (int)row_block * ROWS;
+    const int rows = min(ROWS, a.group - (int)row_block * ROWS);
+    const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
+    const int side = team / together, sides = kTeams / together, r = blockIdx.y * together + team % together;
     int b, first, count;
     Cursor c;
+    const Cuts<TW> cuts(t);
     if (by_sequence) {
         b = x;
-        int all = 0, before = 0;
-        for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) {
-            enter_sequence<TW>(c, t, length_of(t, i));
-            all += c.tiles;
-            if (i < b) before += c.tiles;
-        }
-        int total, begin;
-        scan<kJoinThreads>(all, total);
-        __syncthreads();
-        scan<kJoinThreads>(before, begin);
-        enter_sequence<TW>(c, t, length_of(t, b));
-        const Ranges ranges(t, total);
-        first = ranges.owner(begin);
-        count = ranges.owner(begin + c.tiles - 1) - first + 1;
+        const int begin = cuts.before(b);
+        first = cuts.owner(begin);
+        count = cuts.owner(begin + cuts.tiles_of(b, c) - 1) - first + 1;
         if (count == 1) return;
     } else {
-        Ranges ranges;
-        const int tiles = locate<TW, kJoinThreads, 1>(t, [&](int) { return x; }, 0, c, ranges);
+        const int tiles = cuts.locate(x, c);
         if (tiles == 0 || c.tile == 0 || c.tiles - c.tile > tiles) return;
         b = c.b;
-        first = ranges.owner(ranges.first(x) - c.tile);
+        first = cuts.owner(cuts.first(x) - c.tile);
         count = x - first + 1;
     }
-    const int lane = threadIdx.x % kLanes, side = threadIdx.x / kLanes;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // every side takes every kSide-th part, four at a time
+    // every team takes every sides-th part, four at a time
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto take = [&](float2 ml, float4 x) {
+    auto take = [&](float2 ml, float4 y) {
         const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.0f : top;
         const float keep = exp2_fast(m - base), f = exp2_fast(ml.x - base);
         // NaN scores leave m at -inf and l, o NaN: 0 * NaN passes them on
         m = top;
         l = l * keep + ml.y * f;
-        o.x = o.x * keep + x.x * f;
-        o.y = o.y * keep + x.y * f;
-        o.z = o.z * keep + x.z * f;
-        o.w = o.w * keep + x.w * f;
+        o.x = o.x * keep + y.x * f;
+        o.y = o.y * keep + y.y * f;
+        o.z = o.z * keep + y.z * f;
+        o.w = o.w * keep + y.w * f;
     };
-    for (int i = side; i < count; i += 4 * kSide) {
-        float2 ml[4];
-        float4 x[4];
+    if (r < rows)
+        for (int i = side; i < count; i += 4 * sides) {
+            float2 ml[4];
+            float4 y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int part = i + j * kSide;
-            if (part < count) {
-                const int64_t row = (((int64_t)(first + part) * t.items + item) * 2 + (part == 0 ? 1 : 0)) * ROWS + r;
-                ml[j] = t.part_ml[row];
-                x[j] = *(const float4*)(t.part_o + row * DP + lane * 4);
+            for (int j = 0; j < 4; ++j) {
+                const int part = i + j * sides;
+                if (part < count) {
+                    const int64_t row = (((int64_t)(first + part) * t.items + item) * 2 + (part == 0 ? 1 : 0)) * ROWS + r;
+                    ml[j] = t.part_ml[row];
+                    y[j] = *(const float4*)(t.part_o + row * DP + lane * 4);
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + j * sides < count) take(ml[j], y[j]);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j * kSide < count) take(ml[j], x[j]);
+    if (sides > 1) {
+        sm_o[team][lane] = o;
+        if (lane == 0) sm_ml[team] = make_float2(m, l);
+        __syncthreads();
+        for (int w = 1; w < sides && side == 0; ++w) take(sm_ml[team + w * together], sm_o[team + w * together][lane]);
     }
-    sm_o[side][lane] = o;
-    if (lane == 0) sm_ml[side] = make_float2(m, l);
-    __syncthreads();
-    if (side != 0) return;
-#pragma unroll
-    for (int w = 1; w < kSide; ++w) take(sm_ml[w], sm_o[w][lane]);
+    if (side != 0 || r >= rows) return;
     const bool none = m == -INFINITY && l == 0.0f;
     const float per = 1.0f / l;
     const float y[4] = {o.x, o.y, o.z, o.w};
-    Q* out = (Q*)a.out + (int64_t)b * a.out_seq + (int64_t)head * a.out_head + lane * 4;
+    Q* out = (Q*)a.out + (int64_t)b * a.out_seq + (int64_t)(head0 + r) * a.out_head + lane * 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (lane * 4 + i < a.cache.head_dim) out[i] = rounded<Q>(none ? 0.0f : y[i] * per);
-    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.lse_seq + (int64_t)head * a.lse_head] = (m + log2f(l)) * kLn2;
+    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.lse_seq + (int64_t)(head0 + r) * a.lse_head] = (m + log2f(l)) * kLn2;
 }
 
 // ---- launch ------------------------------------------------------------------------------------
 
 constexpr int kMaxDevices = 16;
-constexpr int kWholeTiles = 6;
 
 template <int CT, class Q, int DP, int NT>
 int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
@@ -1062,11 +1043,14 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     const int64_t most = tokens > 0 ? (tokens + Z::TW - 1) / Z::TW : 1;
     if (a.batch * most > INT32_MAX || (int64_t)a.batch * t.items > INT32_MAX - 64)
         return bad_argument("paged_attention: the tables' width allows over 2^31 - 1 tiles of %d tokens", Z::TW);
-    // A range a sequence where none has more than a few tiles: that costs less than a join.
+    // A range a sequence where none has more than a few tiles: that costs less than a join. bf16, 8
+    // heads of 128, us: 1 sequence of 3 tiles 6.3, cut 6.9, of 6 tiles 9.0, cut 7.6; 64
+    // sequences, which alone occupy half the warps, of 6 tiles 10.2, cut 12.9.
     // Otherwise as many ranges as the warps that fit the GPU at once can take the heads of, or
     // fewer where there cannot be as many tiles.
-    t.whole = most <= kWholeTiles;
-    int64_t ranges = (int64_t)sms * Z::BLOCKS * Z::NW / t.items;
+    const int64_t resident = (int64_t)sms * Z::BLOCKS * Z::NW;
+    t.whole = most <= 4 || (most <= 8 && (int64_t)a.batch * t.items * 3 >= resident);
+    int64_t ranges = resident / t.items;
     if (ranges < 1) ranges = 1;
     if (ranges > a.batch * most) ranges = a.batch * most;
     if (t.whole) ranges = a.batch;
@@ -1086,9 +1070,13 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     RT_CHECK(launch_early(kernel, dim3((unsigned)blocks), dim3(Z::NW * 32), Z::SMEM, st, t));
     if (t.whole) return 0;
     const bool by_sequence = a.batch <= ranges;
-    RT_CHECK(launch_early(join_parts<Q, DP, Z::ROWS, Z::TW>,
-                          dim3((unsigned)((by_sequence ? a.batch : ranges) * t.items), a.group < Z::ROWS ? a.group : Z::ROWS),
-                          dim3(DP * 2), 0, st, t, (int)by_sequence));
+    // long chains of few items: a block a row; short ones of many: rows together, so that the
+    // blocks fit the GPU about once
+    const int64_t joined = (by_sequence ? a.batch : ranges) * t.items, rows = a.group < Z::ROWS ? a.group : Z::ROWS;
+    int together = 1;
+    while (together < kTeams && joined * ((rows + together - 1) / together) > (int64_t)sms * 4) together *= 2;
+    RT_CHECK(launch_early(join_parts<Q, DP, Z::ROWS, Z::TW>, dim3((unsigned)joined, (unsigned)((rows + together - 1) / together)),
+                          dim3(DP * 2), 0, st, t, (int)by_sequence, together));
     return 0;
 }
 
