@@ -193,15 +193,21 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // Those that are operands as they are (one piece) need no second place, and come late.
     static constexpr bool kQReg = KS * 2 * NT * QP + DP / 4 * NT <= 168, kQRaw = !kQReg && QP == 1 && !kNormed;
     static constexpr int ROWS = NT * 8;
-    static constexpr int QROW = DP * (kQ32 ? 4 : 2) + 16;  // 8 rows' words of a column in different banks
+    static constexpr int QROW = DP * (kQ32 ? 4 : 2), QPIECES = QROW / 16;
     static constexpr int Q_BYTES = ROWS * QROW + (kQReg || kQRaw ? 0 : KS * NT * QP * 256);
-    static constexpr int warp_bytes(int stages) { return stages * STAGE + (Q_BYTES + 127) / 128 * 128 + 128; }
-    static constexpr int kMost = 226 * 1024;          // of shared memory a block
-    static constexpr int NW = ROW < 1024 && 4 * warp_bytes(2) <= kMost ? 4 : 2;  // warps a block
-    static constexpr int S = ROW * TW <= 2048 ? 4 : NW * warp_bytes(3) <= kMost ? 3 : 2;  // stages
+    static constexpr int warp_bytes(int stages) { return stages * STAGE + Q_BYTES + 128; }
+    // stages and resident blocks: 3 blocks an SM (12 warps, 168 registers, enough for O of 64
+    // each) with 3 stages at least, else 2 blocks, else one. With one warp a scheduler instead of two, bf16 under float32
+    // queries took 79 us for 41 us of bytes.
+    static constexpr int kMost = 227 * 1024;          // of shared memory a block
+    static constexpr bool fits(int warps, int stages, int blocks) {
+        return warps * warp_bytes(stages) <= kMost && blocks * (warps * warp_bytes(stages) + 1024) <= 228 * 1024;
+    }
+    static constexpr int NW = ROW < 1024 && fits(4, 2, 1) ? 4 : 2;  // warps a block
+    static constexpr int kMany = fits(NW, 3, 3) && DP * NT <= 128 ? 3 : fits(NW, 2, 2) ? 2 : 1;
+    static constexpr int S = fits(NW, 4, kMany) ? 4 : fits(NW, 3, kMany) ? 3 : 2;
     static constexpr int WARP = warp_bytes(S), SMEM = NW * WARP;
-    static constexpr int kFit = 228 * 1024 / (SMEM + 1024 + 256);  // with what the system and the scan take
-    static constexpr int BLOCKS = kFit > 4 ? 4 : kFit < 1 ? 1 : kFit;  // resident blocks an SM
+    static constexpr int BLOCKS = kMany;
     static_assert(SMEM <= kMost, "a block's shared memory");
 };
 
@@ -405,25 +411,42 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     constexpr std::false_type kKeys{};
     constexpr std::true_type kValues{};
 
-    // -- a part's queries: asked for early, taken when it begins
+    // -- a part's queries: asked for early, taken when it begins. Their rows' 16-byte pieces are
+    // exchanged as the cache's are.
+    auto q_place = [](int r, int d) {
+        const int byte = d * (int)sizeof(Q);
+        return r * Z::QROW + ((byte >> 4 ^ (r & 7)) << 4 | (byte & 15));
+    };
     auto ask_queries = [&](int b) {
         const Q* const q = (const Q*)a.q + (int64_t)b * a.q_seq + (int64_t)head0 * a.q_head;
         const uint32_t to = smem_address(sm_raw);
         if (t.q_chunks)
             for (int i = lane; i < rows * t.q_chunks; i += 32) {
                 const int r = i / t.q_chunks, piece = i - r * t.q_chunks;
-                copy16<false>(to + r * Z::QROW + piece * 16, (const unsigned char*)(q + (int64_t)r * a.q_head) + piece * 16, true);
+                copy16<false>(to + r * Z::QROW + (piece ^ (r & 7)) * 16, (const unsigned char*)(q + (int64_t)r * a.q_head) + piece * 16, true);
             }
         else
             for (int i = lane; i < rows * a.cache.head_dim; i += 32) {
                 const int r = i / a.cache.head_dim, d = i - r * a.cache.head_dim;
-                ((Q*)(sm_raw + r * Z::QROW))[d] = q[(int64_t)r * a.q_head + d];
+                *(Q*)(sm_raw + q_place(r, d)) = q[(int64_t)r * a.q_head + d];
             }
     };
     // in the order that the products take them: four lanes a row
     uint2 qf[Z::kQReg ? KS : 1][NT][QP];
     float qscale[NT][2];
-    auto lay_out = [&](int n, const Q* row, int dim) {
+    auto lay_out = [&](int n, int dim) {
+        const int r = n * 8 + oct;
+        if constexpr (QP == 1 && !Z::kNormed) {
+            // operands as they are
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const int d = k * 16 + quad * 2;
+                qf[k][n][0] = make_uint2(d < dim ? *(const uint32_t*)(sm_raw + q_place(r, d)) : 0u,
+                                         d + 8 < dim ? *(const uint32_t*)(sm_raw + q_place(r, d + 8)) : 0u);
+            }
+            qscale[n][0] = qscale[n][1] = a.scale * kLog2e;
+            return;
+        }
         constexpr int XS = CT == MT_F32 ? 2 : 4;
         float x[KS][XS];
 #pragma unroll
@@ -433,12 +456,13 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                 const int d = CT == MT_F32 ? k * 8 + quad + i * 4
                               : kScaled ? k * 16 + quad * 4 + i : k * 16 + quad * 2 + i * 4;
                 if constexpr (CT == MT_F32) {
-                    x[k][i] = d < dim ? (float)row[d] : 0.0f;
+                    x[k][i] = d < dim ? (float)*(const Q*)(sm_raw + q_place(r, d)) : 0.0f;
                 } else {  // head_dim is even here
                     float2 v = make_float2(0.0f, 0.0f);
                     if (d < dim) {
-                        if constexpr (sizeof(Q) == 4) v = *(const float2*)(row + d);
-                        else v = unpack<std::is_same<Q, __nv_bfloat16>::value>(*(const uint32_t*)(row + d));
+                        const unsigned char* const at = sm_raw + q_place(r, d);
+                        if constexpr (sizeof(Q) == 4) v = *(const float2*)at;
+                        else v = unpack<std::is_same<Q, __nv_bfloat16>::value>(*(const uint32_t*)at);
                     }
                     x[k][i] = v.x;
                     x[k][i + 1] = v.y;
@@ -495,14 +519,13 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     auto take_queries = [&]() {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            Q* const row = (Q*)(sm_raw + (n * 8 + oct) * Z::QROW);
             const int dim = n * 8 + oct < rows ? a.cache.head_dim : 0;  // behind it: zeros
             if constexpr (Z::kQRaw) {
                 // products read the rows themselves: zeros where nothing was copied
-                for (int d = dim + quad; d < DP; d += 4) row[d] = Q(0.0f);
+                for (int d = dim + quad; d < DP; d += 4) *(Q*)(sm_raw + q_place(n * 8 + oct, d)) = Q(0.0f);
                 qscale[n][0] = qscale[n][1] = a.scale * kLog2e;
             } else {
-                lay_out(n, row, dim);
+                lay_out(n, dim);
             }
         }
     };
@@ -510,14 +533,16 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         if constexpr (Z::kQReg) {
             return qf[k][n][p];
         } else if constexpr (Z::kQRaw) {
-            const uint32_t* const w = (const uint32_t*)(sm_raw + (n * 8 + oct) * Z::QROW) + k * 8 + quad;
-            return make_uint2(w[0], w[4]);
+            // dims 16 k + quad * 2 and 8 more: pieces 2 k and 2 k + 1
+            const unsigned char* const row = sm_raw + (n * 8 + oct) * Z::QROW + quad * 4;
+            return make_uint2(*(const uint32_t*)(row + ((2 * k ^ oct) << 4)), *(const uint32_t*)(row + (((2 * k + 1) ^ oct) << 4)));
         } else {
             return sm_q[((k * NT + n) * QP + p) * 32 + lane];
         }
     };
 
     ask_queries(in.b);
+    copies_commit();
     // the first tiles' pages are looked up together
     Step ahead[S];
 #pragma unroll
@@ -552,21 +577,16 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         } else {
             asm volatile("griddepcontrol.launch_dependents;");
         }
-        copies_wait<S - 2>();  // this turn's are not committed yet
-        __syncwarp();
-        ++in_part;
         const int4 meta = sm_meta[slot];
-        const uint32_t mask = (uint32_t)meta.z;
-        unsigned char* const stage = ring + slot * Z::STAGE;
-        const uint32_t k_at = smem_address(stage), v_at = k_at + TW * Z::ROW;
+        ++in_part;
         if (meta.y & kFirst) {
-            if (tile > 0) {
-                // asked for when the last part began; that copy is among those waited for once S tiles
-                // have passed
-                if (Z::kQRaw) ask_queries(meta.x);
-                if (Z::kQRaw || in_part <= S) copies_wait_all();
-                __syncwarp();
-            }
+            // the part's queries, while its tiles are on their way: the first part's are the oldest copy;
+            // another's were asked for when the last part began, and have been waited for if that is
+            // S tiles ago
+            if (Z::kQRaw && tile > 0) ask_queries(meta.x);
+            if (tile == 0) copies_wait<S - 1>();
+            else if (Z::kQRaw || in_part <= S) copies_wait_all();
+            __syncwarp();
             take_queries();
             __syncwarp();
             if (!Z::kQRaw && (meta.y & kMore)) ask_queries(meta.x + 1);
@@ -587,6 +607,11 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     for (int i = 0; i < 4; ++i) o[d][n][i] = 0.0f;
             v_unit = 1.17549435e-38f;  // 2^-126
         }
+        copies_wait<S - 2>();  // this turn's are not committed yet
+        __syncwarp();
+        const uint32_t mask = (uint32_t)meta.z;
+        unsigned char* const stage = ring + slot * Z::STAGE;
+        const uint32_t k_at = smem_address(stage), v_at = k_at + TW * Z::ROW;
         if (Z::kTwoBursts && ask && !mask) fetch(ask_slot, kValues);
         if (mask) {
             // S^T: s[.][.][0], [1] are token oct, heads quad * 2 + 0, 1; [2], [3] token oct + 8. The
@@ -888,13 +913,13 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     // what sums are relative to, as an exponent
                     const float exponent = m[n][i] == -INFINITY ? -INFINITY : base[n][i];
                     const int r = quad * 2 + i, row = n * 8 + r;
-                    float f = whole ? 1.0f / sum : 1.0f;
+                    float f = !whole ? 1.0f : none ? 0.0f : 1.0f / sum;
                     if constexpr (kScaled) f *= v_unit;
 #pragma unroll
                     for (int d = 0; d < DP / 16; ++d) {
                         const int d0 = 16 * d + (kScaled ? 2 * oct : oct), d1 = d0 + (kScaled ? 1 : 8);
-                        mine[r * DP + (d0 ^ quad * 8)] = none ? 0.0f : o[d][n][i] * f;
-                        mine[r * DP + (d1 ^ quad * 8)] = none ? 0.0f : o[d][n][2 + i] * f;
+                        mine[r * DP + (d0 ^ quad * 8)] = o[d][n][i] * f;
+                        mine[r * DP + (d1 ^ quad * 8)] = o[d][n][2 + i] * f;
                     }
                     if (oct == 0 && row < rows) {
                         if (!whole)
