@@ -173,6 +173,9 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // tokens a tile: 8-bit rows are short, and a tile's chain of instructions takes as long
     static constexpr int TW = kScaled && DP <= 128 ? 32 : 16, TB = TW / 16;
     static constexpr int STAGE = 2 * TW * ROW + (kScaled ? 256 : 0);  // rows of K, of V, scales of 32 tokens each
+    // Whether step c of a row's pairs of pieces may be behind its end: rows are longer than half of
+    // DP, but for DP = 64
+    __host__ __device__ static constexpr bool may_end(int c) { return DP == 64 ? c >= 1 : 4 * c >= CPR; }
     static constexpr int KS = CT == MT_F32 ? DP / 8 : DP / 16;    // steps of K Q^T
     // pieces of a query: fp16 11 bits, bf16 8 bits, tf32 11 bits each
     static constexpr int QP = CT == MT_F32 ? 2 : !kQ32 ? 1 : kBf16 ? 3 : 2;
@@ -191,7 +194,7 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // A part's queries come into shared memory as they are, while the part before is worked
     // on; then they stay in registers as operands, or, where O leaves too few, in shared memory.
     // Those that are operands as they are (one piece) need no second place, and come late.
-    static constexpr bool kQReg = KS * 2 * NT * QP + DP / 4 * NT <= 168, kQRaw = !kQReg && QP == 1 && !kNormed;
+    static constexpr bool kQReg = KS * 2 * NT * QP + DP / 4 * NT <= (EB == 4 ? 192 : 168), kQRaw = !kQReg && QP == 1 && !kNormed;
     static constexpr int ROWS = NT * 8;
     static constexpr int QROW = DP * (kQ32 ? 4 : 2), QPIECES = QROW / 16;
     static constexpr int Q_BYTES = ROWS * QROW + (kQReg || kQRaw ? 0 : KS * NT * QP * 256);
@@ -203,7 +206,9 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr bool fits(int warps, int stages, int blocks) {
         return warps * warp_bytes(stages) <= kMost && blocks * (warps * warp_bytes(stages) + 1024) <= 228 * 1024;
     }
-    static constexpr int NW = ROW < 1024 && fits(4, 2, 1) ? 4 : 2;  // warps a block
+    // warps a block: 4, or where two blocks of them do not fit, 6 of 32-bit rows with 2 stages (their
+    // products take long), else as many as fit
+    static constexpr int NW = EB == 4 && !fits(4, 2, 2) && fits(6, 2, 1) ? 6 : fits(4, 2, 1) ? 4 : fits(3, 2, 1) ? 3 : 2;
     static constexpr int kMany = fits(NW, 3, 3) && DP * NT <= 128 ? 3 : fits(NW, 2, 2) ? 2 : 1;
     static constexpr int S = fits(NW, 4, kMany) ? 4 : fits(NW, 3, kMany) ? 3 : 2;
     static constexpr int WARP = warp_bytes(S), SMEM = NW * WARP;
@@ -292,7 +297,10 @@ template <int TW> struct Cuts {
     }
 };
 
-template <int CT, class Q, int DP, int NT>
+// kPadded: rows are shorter than DP. Only that form looks for their end: with the tests in it, the
+// other would be 5 to 30 % slower (bf16, 16 sequences of 4096 tokens, 8 heads of 256: 88 us, 115);
+// it takes 42 us at 80 dims, 98 of fp32, where products of whole DPs took 47, 157.
+template <int CT, class Q, int DP, int NT, bool kPadded>
 __global__ void __launch_bounds__(Shape<CT, Q, DP, NT>::NW * 32, Shape<CT, Q, DP, NT>::BLOCKS)
 attention_tiles(const __grid_constant__ TileArgs t) {
     using Z = Shape<CT, Q, DP, NT>;
@@ -360,6 +368,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     const uint32_t row_page = is_v ? a.v_rows.page : a.k_rows.page, row_token = is_v ? a.v_rows.token : a.k_rows.token;
     const int64_t head_bytes = (int64_t)kv_head * Z::EB;
     // the piece of a row that this lane copies, where a row has no more than 32
+    const int row_chunks = kPadded ? t.row_chunks : CPR;
     const unsigned char* const k_base = (const unsigned char*)a.cache.k.ptr + head_bytes * a.cache.k.head + (CPR <= 32 ? lane % CPR * 16 : 0);
     const unsigned char* const v_base = (const unsigned char*)a.cache.v.ptr + head_bytes * a.cache.v.head + (CPR <= 32 ? lane % CPR * 16 : 0);
     const unsigned char* const k_scales = (const unsigned char*)a.cache.k_scale.ptr + (int64_t)kv_head * a.cache.k_scale.head * 4;
@@ -394,19 +403,26 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                                               (CPR <= 32 ? 0 : piece * 16);
             const uint32_t dst = to + swizzled<CPR>(r, piece) * 16;
             if constexpr (kWhole) {
-                copy16<kScaled>(dst, from, true);
+                if (piece < row_chunks) copy16<kScaled>(dst, from, true);
             } else {
                 // absent tokens: V must be zeros (their probability is 0, and 0 * NaN is not); K's
-                // scores are replaced. Padding: K must be zeros, V's columns are not used.
-                const bool real = piece < t.row_chunks, there = there_mask >> r & 1;
-                if (kV ? real : there || !real)
-                    copy16<kScaled>(dst, real ? from : (const unsigned char*)a.cache.k.ptr, real && there);
+                // scores are replaced
+                const bool there = there_mask >> r & 1;
+                if (piece < row_chunks && (kV || there)) copy16<kScaled>(dst, from, there);
             }
         }
     };
     auto fetch = [&](int slot, auto of_v) {
-        if (there_mask == kAll && t.row_chunks == CPR) copy_rows(slot, of_v, std::true_type{});
+        if (there_mask == kAll) copy_rows(slot, of_v, std::true_type{});
         else if (there_mask) copy_rows(slot, of_v, std::false_type{});
+    };
+    // Behind a row's last piece K is zeros, as the queries are there; V's columns are not used. Copies
+    // leave it alone, a part's end (which uses a stage otherwise) puts it back.
+    auto clear_padding = [&](int slot) {
+        for (int i = lane; i < TW * (CPR - row_chunks); i += 32) {
+            const int r = i % TW, piece = row_chunks + i / TW;
+            *(uint4*)(ring + slot * Z::STAGE + swizzled<CPR>(r, piece) * 16) = make_uint4(0, 0, 0, 0);
+        }
     };
     constexpr std::false_type kKeys{};
     constexpr std::true_type kValues{};
@@ -543,6 +559,8 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 
     ask_queries(in.b);
     copies_commit();
+    if constexpr (kPadded)
+        for (int s = 0; s < S; ++s) clear_padding(s);
     // the first tiles' pages are looked up together
     Step ahead[S];
 #pragma unroll
@@ -634,7 +652,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                             product<CT>((Z::kExact ? p == 0 : k % 2 == 1) ? part[n] : s[b][n], x, q.x, q.y);
                         }
                     if constexpr (Z::kExact) {
-                        if (k % 4 == 3 || k == KS - 1) {
+                        if (k % 4 == 3 || (!kPadded && k == KS - 1)) {
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -647,6 +665,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                 };
 #pragma unroll
                 for (int c = 0; c < CPR / 2; ++c) {
+                    if (kPadded && Z::may_end(c) && 2 * c >= row_chunks) break;
                     uint32_t r[4];
                     load_matrices(r, k_at + swizzled<CPR>(b * 16 + (lane & 15), 2 * c + (lane >> 4)) * 16);
                     if constexpr (CT == MT_F32) {
@@ -674,7 +693,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         times_queries(c, r);
                     }
                 }
-                if constexpr (!Z::kExact)
+                if constexpr (!Z::kExact || kPadded)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -828,6 +847,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                 const float* v = (const float*)(stage + TW * Z::ROW);
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d) {
+                    if (kPadded && Z::may_end(2 * d) && 4 * d >= row_chunks) break;
                     float tile_o[NT][4] = {};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -858,6 +878,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                 // 16 dims of 16-bit rows are two pieces, of 8-bit ones one
 #pragma unroll
                 for (int c = 0; c < CPR / 2; ++c) {
+                    if (kPadded && Z::may_end(c) && 2 * c >= row_chunks) break;
                     uint32_t r[TB][4];
 #pragma unroll
                     for (int b = 0; b < TB; ++b)
@@ -952,6 +973,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                 }
                 __syncwarp();
             }
+            if constexpr (kPadded) clear_padding(slot);
         }
         if (++slot == S) slot = 0;
     }
@@ -1086,11 +1108,12 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     t.ranges = FastDiv((uint32_t)ranges);
     t.part_ml = (float2*)workspace;
     t.part_o = (float*)((char*)workspace + ml_bytes);
-    auto kernel = attention_tiles<CT, Q, DP, NT>;
-    static bool ready[kMaxDevices] = {};
-    if (!ready[dev]) {
+    auto kernel = t.row_chunks < Z::CPR ? attention_tiles<CT, Q, DP, NT, true> : attention_tiles<CT, Q, DP, NT, false>;
+    static bool ready[2][kMaxDevices] = {};
+    bool& is_ready = ready[t.row_chunks < Z::CPR][dev];
+    if (!is_ready) {
         RT_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::SMEM));
-        ready[dev] = true;
+        is_ready = true;
     }
     RT_CHECK(launch_early(kernel, dim3((unsigned)blocks), dim3(Z::NW * 32), Z::SMEM, st, t));
     if (t.whole) return 0;
