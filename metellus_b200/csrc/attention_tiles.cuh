@@ -1128,12 +1128,32 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     return 0;
 }
 
+// Over 8 query heads a key-value head: 16 of them a warp, or 8, so that neighbouring warps read the
+// same rows, which one of them finds in L2. 16 halve what the SMs read, and a warp then has fewer
+// registers left and twice as much to hand over; they win where a warp has many tiles (as far as
+// the tables' width tells). bf16, 2 heads of 128, 32 query heads, us: 16 sequences of 2048 tokens
+// (4 tiles a warp) 20.7, by eights 16.5; of 8192 (14) 38.0, 36.4; of 16384 (28) 56.6, 62.5; 64 of
+// 32768 (221) 322, 436. fp16, 1 head of 256: 7 of 16384 (12) 44.2, 39.8; 32 of 16384 (55) 118, 138.
+// 32-bit rows of over 64 dims leave 16 heads too few registers: 426, by eights 392 at 110 tiles a warp.
+template <int CT, class Q, int DP>
+int by_group(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
+    if constexpr (CT != MT_F32 || DP <= 64) {
+        using Z = Shape<CT, Q, DP, 2>;
+        int sms;
+        if (int rc = sm_count(dev, &sms)) return rc;
+        const int64_t tiles = (a.max_tokens < a.window ? a.max_tokens : a.window) / Z::TW;
+        const int64_t lines = (int64_t)a.cache.kv_heads * ((a.group + Z::ROWS - 1) / Z::ROWS);
+        if (a.group > 8 && a.batch * lines * tiles >= 20LL * sms * Z::BLOCKS * Z::NW)
+            return launch<CT, Q, DP, 2>(a, run, workspace, bytes, dev, st);
+    }
+    return launch<CT, Q, DP, 1>(a, run, workspace, bytes, dev, st);
+}
+
 template <int CT, class Q> int by_shape(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
     const int dim = a.cache.head_dim;
-    const bool wide = a.group > 8;
-    if (dim <= 64) return wide ? launch<CT, Q, 64, 2>(a, run, workspace, bytes, dev, st) : launch<CT, Q, 64, 1>(a, run, workspace, bytes, dev, st);
-    if (dim <= 128) return wide ? launch<CT, Q, 128, 2>(a, run, workspace, bytes, dev, st) : launch<CT, Q, 128, 1>(a, run, workspace, bytes, dev, st);
-    return wide ? launch<CT, Q, 256, 2>(a, run, workspace, bytes, dev, st) : launch<CT, Q, 256, 1>(a, run, workspace, bytes, dev, st);
+    if (dim <= 64) return by_group<CT, Q, 64>(a, run, workspace, bytes, dev, st);
+    if (dim <= 128) return by_group<CT, Q, 128>(a, run, workspace, bytes, dev, st);
+    return by_group<CT, Q, 256>(a, run, workspace, bytes, dev, st);
 }
 
 }  // namespace tiles

@@ -202,6 +202,13 @@ def test_attention_batches(q_type, dtype, batch, longest, extra_width):
     compare(*make(lengths, 6, 3, 64, 16, q_type, dtype, extra_width=extra_width))
 
 
+@pytest.mark.parametrize("q_type,dtype", PAIRS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(11, 1, 64), (32, 2, 96), (40, 2, 128), (33, 1, 32), (16, 1, 256), (20, 1, 192)])
+def test_attention_wide_groups(q_type, dtype, heads, kv_heads, dim):
+    """Tables wide enough for many tiles a warp: 16 query heads are taken at a time."""
+    compare(*make([0, 5, 300, 2500, 1], heads, kv_heads, dim, 128, q_type, dtype, extra_width=4000))
+
+
 @pytest.mark.parametrize("q_type,dtype", [(F32, F32), (BF16, BF16), (F32, I8), (F16, E4M3)])
 @pytest.mark.parametrize("dim", [1, 7, 36, 100, 200, 250])
 def test_attention_odd_head_dims(q_type, dtype, dim):
