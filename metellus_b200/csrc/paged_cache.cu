@@ -158,48 +158,69 @@ template <> __device__ inline float from_float<float>(float x) { return x; }
 template <> __device__ inline __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// A row's codes. x / s in fp32 can be rounded onto, or over, the border between two codes, so
-// the nearest code is found in two ways:
-//
-// * quick(): from t = x * per, which is x / s up to a few ulps, unless t is next to a border (a part
-//   in 2^13 or less of all values): then `close` is set.
-// * number(): from the remainder x - n s of the candidate n, which one fma gives exactly. More than
-//   half of s, or half of it and n odd: the other neighbour is nearer, or even.
-//
-// `per` is 1 / s, or 0 where s is so small that this may not be a number; then x / s is taken as
-// it is. s is not 0.
-constexpr float kBig = 12582912.0f;  // 1.5 * 2^23: its ulp is 1, so adding it rounds to whole numbers
+// What a row is divided by: its scale s, as pairs of numbers for the instructions that take two
+// elements. Rows of scales up to 1e-30 are raised by 2^96 first, both exactly, for 1 / s to be a
+// number.
+struct Divisor {
+    uint64_t minus_s, per, quarter;
+    template <int N> __device__ Divisor(float s, float (&x)[N]) {
+        if (s <= 1e-30f) {
+            s *= 0x1p96f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] *= 0x1p96f;
+        }
+        const float y = 1.0f / s;
+        minus_s = both(-s, -s), per = both(y, y), quarter = both(0.25f * y, 0.25f * y);
+    }
+    static __device__ uint64_t both(float a, float b) {
+        uint64_t y;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+        return y;
+    }
 
-__device__ inline float nearest_multiple(float x, float s, float t) {
-    const float shifted = t + kBig, n = shifted - kBig, r = fmaf(-n, s, x), twice = 2.0f * fabsf(r);
-    const bool odd = __float_as_uint(shifted) & 1;
-    return twice > s || (twice == s && odd) ? n + copysignf(1.0f, r) : n;
-}
+    // x / s, rounded so that it rounds to the code that x / s itself is nearest to (of two as near the
+    // even one). x / s in fp32 can be rounded onto, or over, the border between two codes. t = x / s up
+    // to 2 ulps; g = 9 t - (9 t - t), Veltkamp's way to drop t's last bits, is the multiple of 8 ulps
+    // next to it, so x / s is within 6 ulps of g. Borders have 8 leading bits at most: none but g itself
+    // is as near to x / s, and all that counts is on which side of g it lies: the sign of r = x - g s, which one fma gives exactly (where g is a border, s > 1e-30 keeps
+    // it from underflow). g + r / 4s, rounded up, and down, and both moves added: g where r is 0, else a
+    // number between g and x / s, or the next to g on that side. The last sum rounds down so that
+    // -0 stays what it is.
+    // 9 instructions for two elements and no branch. 2^25 elements fp16 -> e4m3, whose quotients often
+    // are borders: 26 us (15.6 at the copy rate); 57 with a check that sent rows next to a border a slower
+    // way, 28 with the sign of r taken in integers.
+    __device__ float2 quotients(float x0, float x1) const {
+        constexpr uint64_t kNine = 0x4110000041100000ull, kMinus1 = 0xBF800000BF800000ull;
+        const uint64_t x = both(x0, x1);
+        float2 y;
+        asm("{.reg .b64 t, c, g, r, u, d, e, q;\n\t"
+            "mul.rn.f32x2 t, %2, %3;\n\t"
+            "mul.rn.f32x2 c, t, %6;\n\t"
+            "fma.rn.f32x2 e, t, %7, c;\n\t"
+            "fma.rn.f32x2 g, e, %7, c;\n\t"
+            "fma.rn.f32x2 r, g, %4, %2;\n\t"
+            "fma.rp.f32x2 u, r, %5, g;\n\t"
+            "fma.rm.f32x2 d, r, %5, g;\n\t"
+            "fma.rn.f32x2 e, g, %7, u;\n\t"
+            "add.rm.f32x2 q, d, e;\n\t"
+            "mov.b64 {%0, %1}, q;}"
+            : "=f"(y.x), "=f"(y.y) : "l"(x), "l"(per), "l"(minus_s), "l"(quarter), "l"(kNine), "l"(kMinus1));
+        return y;
+    }
+};
+
+constexpr float kBig = 12582912.0f;  // 1.5 * 2^23: its ulp is 1, so adding it rounds to whole numbers
 
 template <class C> struct Code;
 template <> struct Code<int8_t> {
     static constexpr float kLargest = 127.0f;
-    static __device__ int number(float x, float s, float per) {
-        const float n = nearest_multiple(x, s, per != 0.0f ? x * per : x / s);
-        return (int)fminf(fmaxf(n, -127.0f), 127.0f);
-    }
-    static __device__ int8_t of(float x, float s, float per) { return (int8_t)number(x, s, per); }
+    static __device__ int8_t of(float x, const Divisor& by) { return (int8_t)__float_as_uint(by.quotients(x, x).x + kBig); }
     static __device__ uint32_t bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
         return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
     }
-    static __device__ uint32_t quick4(const float* x, float per, bool& close) {
-        uint32_t y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float shifted = fmaf(x[i], per, kBig), n = shifted - kBig;
-            // |t| < 128: t and this distance are good to 2^-15
-            close |= fabsf(fmaf(x[i], per, -n)) > 0.5f - 0x1p-14f;
-            y[i] = __float_as_uint(shifted);  // its low byte is n's
-        }
-        return bytes(y[0], y[1], y[2], y[3]);
-    }
-    static __device__ uint32_t pack4(const float* x, float s, float per) {
-        return bytes(number(x[0], s, per), number(x[1], s, per), number(x[2], s, per), number(x[3], s, per));
+    static __device__ uint32_t pack4(const float* x, const Divisor& by) {
+        const float2 a = by.quotients(x[0], x[1]), b = by.quotients(x[2], x[3]);  // their low bytes, with kBig added
+        return bytes(__float_as_uint(a.x + kBig), __float_as_uint(a.y + kBig), __float_as_uint(b.x + kBig), __float_as_uint(b.y + kBig));
     }
     static __device__ void unpack4(uint32_t y, float* x) {
 #pragma unroll
@@ -209,33 +230,10 @@ template <> struct Code<int8_t> {
 };
 template <> struct Code<__nv_fp8_e4m3> {
     static constexpr float kLargest = 448.0f;
-    static __device__ float number(float x, float s, float per) {
-        const float t = per != 0.0f ? x * per : x / s;
-        // the spacing of e4m3 around t: 2^(exponent - 3), at least 2^-9
-        const int e = max((int)(__float_as_uint(t) >> 23 & 0xff), 121) - 3;
-        const float u = __uint_as_float((uint32_t)e << 23), inverse = __uint_as_float((uint32_t)(254 - e) << 23);
-        return nearest_multiple(x, s * u, t * inverse) * u;
-    }
-    static __device__ __nv_fp8_e4m3 of(float x, float s, float per) { return __nv_fp8_e4m3(number(x, s, per)); }
-    static __device__ uint32_t codes(const float* t) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[0], t[1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[2], t[3]), __NV_SATFINITE, __NV_E4M3);
-        return lo | hi << 16;
-    }
-    static __device__ uint32_t quick4(const float* x, float per, bool& close) {
-        float t[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            t[i] = x[i] * per;
-            // a border of normal codes has its 20 bits behind the third fraction bit at 0x80000; t
-            // is good to 4 ulps. Below 2^-6 the spacing is another, and 0 needs no look.
-            close |= ((__float_as_uint(t[i]) + (4u - 0x80000u)) & 0xfffffu) <= 8u || (fabsf(t[i]) < 0x1p-6f && t[i] != 0.0f);
-        }
-        return codes(t);
-    }
-    static __device__ uint32_t pack4(const float* x, float s, float per) {
-        const float t[4] = {number(x[0], s, per), number(x[1], s, per), number(x[2], s, per), number(x[3], s, per)};
-        return codes(t);
+    static __device__ __nv_fp8_e4m3 of(float x, const Divisor& by) { return __nv_fp8_e4m3(by.quotients(x, x).x); }
+    static __device__ uint32_t pack4(const float* x, const Divisor& by) {
+        return __nv_cvt_float2_to_fp8x2(by.quotients(x[0], x[1]), __NV_SATFINITE, __NV_E4M3) |
+               (uint32_t)__nv_cvt_float2_to_fp8x2(by.quotients(x[2], x[3]), __NV_SATFINITE, __NV_E4M3) << 16;
     }
     static __device__ void unpack4(uint32_t y, float* x) {
 #pragma unroll
@@ -248,12 +246,14 @@ template <> struct Code<__nv_fp8_e4m3> {
     }
 };
 
-// A row's scale from the bits of its largest magnitude (as bits, magnitudes order like
-// numbers, with infinities and NaN on top), and its reciprocal.
-template <class C> __device__ inline float scale_of(uint32_t top, float* per) {
-    const float s = top < 0x7f800000u ? __uint_as_float(top) / Code<C>::kLargest : __uint_as_float(0x7fc00000u);
-    *per = s > 1e-30f ? 1.0f / s : 0.0f;
-    return s;
+// A row's largest magnitude; NaN if it has one. Then its scale, NaN too if that is not finite.
+__device__ inline float largest(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+template <class C> __device__ inline float scale_of(float top) {
+    return top < INFINITY ? top / Code<C>::kLargest : __uint_as_float(0x7fc00000u);
 }
 
 // Two 16-bit elements as a word.
@@ -323,16 +323,12 @@ template <int kElements, int kThreads, int kRun> struct Piece {
                 else *(uint4*)(p + at(i)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
     }
-    template <class C> __device__ void store_codes(C* p, int dim, const float* x, float s, float per) const {
+    template <class C> __device__ void store_codes(C* p, int dim, float (&x)[kElements], float s) const {
         uint32_t w[kElements / 4] = {};
         if (s > 0.0f) {
-            bool close = per == 0.0f;
+            const Divisor by(s, x);
 #pragma unroll
-            for (int k = 0; k < kElements / 4; ++k) w[k] = Code<C>::quick4(x + 4 * k, per, close);
-            if (close) {
-#pragma unroll
-                for (int k = 0; k < kElements / 4; ++k) w[k] = Code<C>::pack4(x + 4 * k, s, per);
-            }
+            for (int k = 0; k < kElements / 4; ++k) w[k] = Code<C>::pack4(x + 4 * k, by);
         }
 #pragma unroll
         for (int i = 0; i < kRuns; ++i)
@@ -391,18 +387,19 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a)
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) v[i] = lane + 32 * i < a.head_dim ? to_float(x[lane + 32 * i]) : 0.0f;
         if constexpr (kScaled) {
-            uint32_t top = 0;
+            float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) top = max(top, __float_as_uint(fabsf(v[i])));
-            top = __reduce_max_sync(0xffffffffu, top);
-            float per;
-            const float s = scale_of<C>(top, &per);
+            for (int i = 0; i < kPerLane; ++i) top = largest(top, fabsf(v[i]));
+#pragma unroll
+            for (int i = 1; i < 32; i <<= 1) top = largest(top, __shfl_xor_sync(0xffffffffu, top, i));
+            const float s = scale_of<C>(top);
             if (lane == 0)
                 ((float*)a.scale[which].ptr)[cache_offset(a.scale[which], page, at, head)] = s;
             const bool none = !(s > 0.0f);
+            const Divisor by(s, v);
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i)
-                if (lane + 32 * i < a.head_dim) c[lane + 32 * i] = none ? C(0.0f) : Code<C>::of(v[i], s, per);
+                if (lane + 32 * i < a.head_dim) c[lane + 32 * i] = none ? C(0.0f) : Code<C>::of(v[i], by);
         } else {
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i)
@@ -438,14 +435,14 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_rows(const RowArgs a) 
 }
 
 // The same in pieces: kThreads threads (a power of two) a row, kElements of it a thread. With
-// many rows 16 elements, and the rows of K and of V together; with few, where a call takes as
+// many rows 16 or 24 elements, and the rows of K and of V together; with few, where a call takes as
 // long as one thread's work does, 4 or 8, and K and V in different blocks (gridDim.y = 2).
 template <class X, class C, int kElements, int kThreads>
 __global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
-    constexpr bool kBoth = kElements == 16;
+    constexpr bool kBoth = kElements >= 16;
     const PieceOf<X, C, kElements, kThreads> piece{(int)(threadIdx.x % kThreads)};
     const int from = kBoth ? 0 : blockIdx.y, to = kBoth ? 2 : from + 1;
     const uint32_t count = (uint32_t)a.row_count;
@@ -465,19 +462,18 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_pieces(const RowArgs 
         const uint32_t page = a.page.div(there ? (uint32_t)slot : 0, &at);
 #pragma unroll
         for (int i = from; i < to; ++i) {
-            const float* const xi = x[kBoth ? i : 0];
+            auto& xi = x[kBoth ? i : 0];
             C* const c = (C*)a.cache[i].ptr + cache_offset(a.cache[i], page, at, head);
             if constexpr (kScaled) {
-                uint32_t top = 0;
+                float top = 0.0f;
 #pragma unroll
-                for (int k = 0; k < kElements; ++k) top = max(top, __float_as_uint(fabsf(xi[k])));
+                for (int k = 0; k < kElements; ++k) top = largest(top, fabsf(xi[k]));
 #pragma unroll
-                for (int k = 1; k < kThreads; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+                for (int k = 1; k < kThreads; k <<= 1) top = largest(top, __shfl_xor_sync(0xffffffffu, top, k));
                 if (!there) continue;
-                float per;
-                const float s = scale_of<C>(top, &per);
+                const float s = scale_of<C>(top);
                 if (piece.lane == 0) ((float*)a.scale[i].ptr)[cache_offset(a.scale[i], page, at, head)] = s;
-                piece.store_codes(c, a.head_dim, xi, s, per);
+                piece.store_codes(c, a.head_dim, xi, s);
             } else {
                 if (there) piece.store(c, a.head_dim, xi);
             }
@@ -490,7 +486,7 @@ __global__ void __launch_bounds__(kRowThreads) cache_read_pieces(const RowArgs a
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr bool kScaled = sizeof(C) == 1;
     constexpr int kGroups = kRowThreads / kThreads;
-    constexpr bool kBoth = kElements == 16;
+    constexpr bool kBoth = kElements >= 16;
     const PieceOf<X, C, kElements, kThreads> piece{(int)(threadIdx.x % kThreads)};
     const int from = kBoth ? 0 : blockIdx.y, to = kBoth ? 2 : from + 1;
     const uint32_t count = (uint32_t)a.row_count;
@@ -530,7 +526,7 @@ template <class X, class C, int kElements, int kThreads>
 int launch_pieces(bool write, const RowArgs& a, int sms, cudaStream_t st) {
     const int64_t groups = kRowThreads / kThreads, want = (a.row_count + groups - 1) / groups;
     const int64_t resident = (int64_t)sms * 4;  // 64 registers a thread
-    const dim3 grid((unsigned)(want < resident ? want : resident), kElements == 16 ? 1 : 2);
+    const dim3 grid((unsigned)(want < resident ? want : resident), kElements >= 16 ? 1 : 2);
     if (write)
         RT_CHECK(launch_early(cache_write_pieces<X, C, kElements, kThreads>, grid, kRowThreads, 0, st, a));
     else
@@ -544,7 +540,11 @@ int launch_rows(bool write, const RowArgs& a, int sms, cudaStream_t st) {
         // few: not even one block an SM at 16 elements a thread. One token of 16 sequences, 8 heads of
         // 128, bf16 to e4m3: 2.5 us with 4 elements a thread, 5.5 with 16.
         const bool few = a.row_count * ((a.head_dim + 15) / 16) < (int64_t)sms * kRowThreads;
+        // Many: 16 elements, or 24 where 5 or 6 threads would not be a power of two. 2^25 elements fp16 ->
+        // e4m3 in rows of 32: 26 us, 53 with 4 threads a row; of 80: 34 us, 44 with 8 threads of 16.
+        if (a.head_dim <= 32 && !few) return launch_pieces<X, C, 16, 2>(write, a, sms, st);
         if (a.head_dim <= 64) return few ? launch_pieces<X, C, 4, 16>(write, a, sms, st) : launch_pieces<X, C, 16, 4>(write, a, sms, st);
+        if (a.head_dim > 64 && a.head_dim <= 96 && !few) return launch_pieces<X, C, 24, 4>(write, a, sms, st);
         if (a.head_dim <= 128) return few ? launch_pieces<X, C, 4, 32>(write, a, sms, st) : launch_pieces<X, C, 16, 8>(write, a, sms, st);
         return few ? launch_pieces<X, C, 8, 32>(write, a, sms, st) : launch_pieces<X, C, 16, 16>(write, a, sms, st);
     }
