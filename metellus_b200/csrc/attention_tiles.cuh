@@ -1090,13 +1090,18 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     const int64_t most = tokens > 0 ? (tokens + Z::TW - 1) / Z::TW : 1;
     if (a.batch * most > INT32_MAX || (int64_t)a.batch * t.items > INT32_MAX - 64)
         return bad_argument("paged_attention: the tables' width allows over 2^31 - 1 tiles of %d tokens", Z::TW);
-    // A range a sequence where none has more than a few tiles: that costs less than a join. bf16, 8
-    // heads of 128, us: 1 sequence of 3 tiles 6.3, cut 6.9, of 6 tiles 9.0, cut 7.6; 64
-    // sequences, which alone occupy half the warps, of 6 tiles 10.2, cut 12.9.
-    // Otherwise as many ranges as the warps that fit the GPU at once can take the heads of, or
-    // fewer where there cannot be as many tiles.
-    const int64_t resident = (int64_t)sms * Z::BLOCKS * Z::NW;
-    t.whole = most <= 4 || (most <= 8 && (int64_t)a.batch * t.items * 3 >= resident);
+    // A range a sequence where none has more than a few tiles: that costs less than a join. The more
+    // so, the more of the warps that fit the GPU at once the sequences occupy: then a join has many
+    // parts, and cutting gives each warp less to gain. Long tiles make up for a join sooner. us, whole
+    // and cut: bf16, 8 heads of 128, 1 sequence of 4 tiles 8.3, 7.3; 40 sequences (a quarter of the
+    // warps) of 6 tiles 10.4, 11.4, of 12 tiles 15.5, 12.5; fp32, 8 heads of 256, 8 sequences of 2 tiles
+    // 18.6, 15.5, of 4 tiles 29.8, 15.5.
+    // Otherwise as many ranges as those warps can take the heads of, or fewer where there cannot be as
+    // many tiles.
+    const int64_t resident = (int64_t)sms * Z::BLOCKS * Z::NW, used = (int64_t)a.batch * t.items;
+    constexpr int kTile = Z::TW * DP * (Z::EB == 4 ? 2 : 1), kFew = kTile <= 1024 ? 4 : kTile <= 2048 ? 3 : 2;
+    constexpr int kMore = Z::EB == 4 || Z::TW == 32 ? 6 : 24;
+    t.whole = most <= kFew + (used <= resident ? kMore * used / resident : 0);
     int64_t ranges = resident / t.items;
     if (ranges < 1) ranges = 1;
     if (ranges > a.batch * most) ranges = a.batch * most;
