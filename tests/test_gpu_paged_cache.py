@@ -202,6 +202,19 @@ def test_attention_batches(q_type, dtype, batch, longest, extra_width):
     compare(*make(lengths, 6, 3, 64, 16, q_type, dtype, extra_width=extra_width))
 
 
+@pytest.mark.parametrize("q_type,dtype", [(F32, F32), (BF16, BF16), (F16, F16), (F32, I8), (BF16, E4M3)])
+@pytest.mark.parametrize("heads,dim", [(8, 128), (6, 64), (16, 256), (6, 36)])
+def test_attention_padded_batch(q_type, dtype, heads, dim):
+    """Sequences without tokens alone and in runs, first and last, between long and short ones:
+    their rows are zeros, written over what was there."""
+    lengths = [0, 0, 700, 0, 3, 0, 0, 0, 40, 1, 0, 1500] + [0] * 70 + [17, 0, 90] + [0] * 40
+    q, c, tables, n = make(lengths, heads, 2, dim, 16, q_type, dtype)
+    out = torch.full_like(q, math.nan)
+    paged_attention(q, c[0], c[1], tables, n, out=out, **kw(c))
+    assert not out[n == 0].any()
+    assert torch.equal(out, compare(q, c, tables, n)[0])
+
+
 @pytest.mark.parametrize("q_type,dtype", PAIRS)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(11, 1, 64), (32, 2, 96), (40, 2, 128), (33, 1, 32), (16, 1, 256), (20, 1, 192)])
 def test_attention_wide_groups(q_type, dtype, heads, kv_heads, dim):
