@@ -160,14 +160,15 @@ template <> __device__ inline __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
 
 // What a row is divided by: its scale s, as pairs of numbers for the instructions that take two
 // elements. Rows of scales up to 1e-30 are raised by 2^96 first, both exactly, for 1 / s to be a
-// number.
+// number, and cut to `top`, the largest code: scales of a few of fp32's smallest steps are rounded
+// so far that quotients would pass it.
 struct Divisor {
     uint64_t minus_s, per, quarter;
-    template <int N> __device__ Divisor(float s, float (&x)[N]) {
+    template <int N> __device__ Divisor(float s, float (&x)[N], float top) {
         if (s <= 1e-30f) {
             s *= 0x1p96f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] *= 0x1p96f;
+            for (int i = 0; i < N; ++i) x[i] = fminf(fmaxf(x[i] * 0x1p96f, -top * s), top * s);
         }
         const float y = 1.0f / s;
         minus_s = both(-s, -s), per = both(y, y), quarter = both(0.25f * y, 0.25f * y);
@@ -326,7 +327,7 @@ template <int kElements, int kThreads, int kRun> struct Piece {
     template <class C> __device__ void store_codes(C* p, int dim, float (&x)[kElements], float s) const {
         uint32_t w[kElements / 4] = {};
         if (s > 0.0f) {
-            const Divisor by(s, x);
+            const Divisor by(s, x, Code<C>::kLargest);
 #pragma unroll
             for (int k = 0; k < kElements / 4; ++k) w[k] = Code<C>::pack4(x + 4 * k, by);
         }
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(kRowThreads) cache_write_rows(const RowArgs a)
             if (lane == 0)
                 ((float*)a.scale[which].ptr)[cache_offset(a.scale[which], page, at, head)] = s;
             const bool none = !(s > 0.0f);
-            const Divisor by(s, v);
+            const Divisor by(s, v, Code<C>::kLargest);
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i)
                 if (lane + 32 * i < a.head_dim) c[lane + 32 * i] = none ? C(0.0f) : Code<C>::of(v[i], by);

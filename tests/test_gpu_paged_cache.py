@@ -125,6 +125,21 @@ def test_codes_at_borders(dtype, x_type):
     assert bool(torch.isnan(k[1001:1004]).all()) and bool(torch.isfinite(k[:1000]).all()) and not k[1000].any()
 
 
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+@pytest.mark.parametrize("dim", [64, 36])
+def test_codes_of_smallest_rows(dtype, dim):
+    """Scales around and below fp32's smallest normal number, down to a few of its steps,
+    where largest / scale passes the largest code by up to half."""
+    x = torch.randn((400, 1, dim), device=DEV) * torch.exp2(-torch.linspace(90, 149, 400, device=DEV))[:, None, None]
+    x[::7, 0, 0] = -0.0
+    c = new_cache(25, 16, 1, dim, dtype)
+    cache_write(x, -x, c[0], c[1], torch.arange(400, device=DEV), **kw(c))
+    for y, cache, scale in ((x, c[0], c[2]), (-x, c[1], c[3])):
+        code, z = ref.codes(y, dtype)
+        assert torch.equal(scale.flatten(0, 1), z)
+        assert torch.equal(cache.float().flatten(0, 1), code.float().clamp(-ref.CODE_MAX[dtype], ref.CODE_MAX[dtype]))
+
+
 def test_read_into_strided_rows():
     """Heads first, as the batched attention of programs takes K."""
     c = new_cache(9, 16, 4, 64, I8)
