@@ -1018,24 +1018,27 @@ __global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ Til
     const int rows = min(ROWS, a.group - (int)row_block * ROWS);
     const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
     const int side = team / together, sides = kTeams / together, r = blockIdx.y * together + team % together;
-    int b, first, count;
+    int b, first = 0, count = 0;  // count: parts to join, none or several
     Cursor c;
     const Cuts<TW> cuts(t);
     if (by_sequence) {
         b = x;
         const int begin = cuts.before(b), tiles = cuts.tiles_of(b, c);
-        if (tiles == 0) return;
-        first = cuts.owner(begin);
-        count = cuts.owner(begin + tiles - 1) - first + 1;
-        if (count == 1) return;
+        if (tiles > 0) {
+            first = cuts.owner(begin);
+            count = cuts.owner(begin + tiles - 1) - first + 1;
+        }
     } else {
         const int tiles = cuts.locate(x, c);
-        if (tiles == 0 || c.tile == 0 || c.tiles - c.tile > tiles) return;
         b = c.b;
-        first = cuts.owner(cuts.first(x) - c.tile);
-        count = x - first + 1;
+        if (tiles > 0 && c.tile > 0 && c.tiles - c.tile <= tiles) {
+            first = cuts.owner(cuts.first(x) - c.tile);
+            count = x - first + 1;
+        }
     }
+    // every block waits, those without work too: what comes after this kernel waits for it alone
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (count <= 1) return;
     // every team takes every sides-th part, four at a time
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

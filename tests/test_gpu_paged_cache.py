@@ -394,6 +394,24 @@ def test_captured_steps_share_nothing():
             ref.check(out, want, tol)
 
 
+@pytest.mark.parametrize("longest,extra_width", [(16, 4000), (3000, 0)])
+def test_calls_follow_one_another(longest, extra_width):
+    """What comes after an attention (here a write into the pages that it reads) waits for all of
+    it: with no sequence to join, though the tables are wide, and with long ones."""
+    lengths = torch.randint(1, longest + 1, (64,)).tolist()
+    q, c, tables, n = make(lengths, 32, 8, 128, 16, BF16, BF16, extra_width=extra_width)
+    want = paged_attention(q, c[0], c[1], tables, n)
+    slots = torch.arange(c[0].shape[0] * 16, device=DEV)
+    kept = cache_read(c[0], c[1], slots)
+    other = [torch.full_like(x, 9.0) for x in kept]
+    for _ in range(20):
+        out = paged_attention(q, c[0], c[1], tables, n)
+        cache_write(*other, c[0], c[1], slots)
+        cache_write(*kept, c[0], c[1], slots)
+        again = paged_attention(q, c[0], c[1], tables, n)
+        assert torch.equal(out, want) and torch.equal(again, want)
+
+
 def test_runs_on_the_current_stream():
     """Work queued before a call on the current stream is seen by it, on a side stream and on
     the default one; results are the same in repeated calls."""
