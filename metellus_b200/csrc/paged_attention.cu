@@ -115,7 +115,7 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
         a.lse_seq = lse->strides[0];
         a.lse_head = lse->strides[1];
     }
-    if (!std::isfinite(scale)) return bad_argument("%s: scale must be finite", who);
+    if (!std::isfinite((float)scale)) return bad_argument("%s: scale must be finite", who);
     if (batch == 0) return 0;
     a.lengths = (const int32_t*)lengths->ptr;
     a.length_seq = lengths->strides[0];

@@ -431,7 +431,7 @@ class PagedAttentionOp:
         if self.tables.shape[0] != rows or self.lengths.shape[0] != rows:
             raise ValueError(f"{what}: q has {rows} rows, {self.tables.name!r} {self.tables.shape[0]}, "
                              f"{self.lengths.name!r} {self.lengths.shape[0]}")
-        if not math.isfinite(self.scale):
+        if not abs(self.scale) <= 3.4028234663852886e38:  # float32's largest
             raise ValueError(f"{what}: scale must be finite, got {self.scale}")
         if self.window < 0:
             raise ValueError(f"{what}: window must not be negative, got {self.window}")

@@ -69,6 +69,7 @@ def attend(match, **other):
     ("lse must be", {"lse": array("float32", (3, 2))}),
     ("lse cannot be bfloat16", {"lse": array("bfloat16", (3, 4))}),
     ("scale must be finite", {"scale": float("nan")}),
+    ("scale must be finite", {"scale": -1e39}),
     ("window must not be negative", {"window": -1}),
     ("the cache is missing", {"cache": None}),
     ("one type", {"cache": cache(v=array("float16", (4, 16, 2, 64)))}),
