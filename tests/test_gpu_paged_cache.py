@@ -298,6 +298,12 @@ def test_attention_ignores_what_is_not_visible(q_type, dtype):
     compare(q, c, tables, lengths, window=0 if dtype is F32 else 90)
 
 
+@pytest.mark.parametrize("q_type,dtype", [(F32, F32), (BF16, BF16), (F16, I8)])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 0.02, 0.5])
+def test_attention_scale(q_type, dtype, scale):
+    compare(*make([0, 1, 77, 400], 8, 2, 64, 16, q_type, dtype), scale=scale)
+
+
 @pytest.mark.parametrize("q_type,dtype", [(F32, F32), (BF16, BF16), (F32, I8)])
 def test_attention_large_scores(q_type, dtype):
     """A row that attends to one token alone, and scores far apart in magnitude."""
@@ -308,6 +314,29 @@ def test_attention_large_scores(q_type, dtype):
     ref.check(out, want, tol)
     q *= 0
     compare(q, c, tables, lengths)
+
+
+@pytest.mark.parametrize("q_type,dtype,dim", [(BF16, BF16, 128), (F32, I8, 128), (F32, F32, 64), (BF16, BF16, 36), (F16, E4M3, 80)])
+def test_caches_of_over_32_bits(q_type, dtype, dim):
+    """Pages behind 2^31 elements (and 2^32 bytes) of a cache: the same, bit for bit, as in a small one."""
+    q, c, tables, n = make([5, 700, 90], 8, 2, dim, 16, q_type, dtype, spare=0)
+    used = c[0].shape[0]
+    pages = (2 ** 31 + 2 ** 30 * (4 // dtype.itemsize)) // (16 * 2 * dim) + used
+    big = [None if x is None else torch.empty((pages, *x.shape[1:]), device=DEV, dtype=x.dtype) for x in c]
+    slots = torch.arange(used * 16, device=DEV) + (pages - used) * 16
+    for x, y in zip(big, c):
+        if x is not None:
+            raw(x)[pages - used:] = raw(y)
+    far = torch.where(tables >= 0, tables + (pages - used), tables)
+    assert torch.equal(paged_attention(q, big[0], big[1], far, n, **kw(big)), paged_attention(q, c[0], c[1], tables, n, **kw(c)))
+    rows = cache_read(big[0], big[1], slots, **kw(big))
+    here = cache_read(c[0], c[1], slots - slots[0], **kw(c))
+    assert torch.equal(rows[0], here[0]) and torch.equal(rows[1], here[1])
+    x = torch.randn((used * 16, 2, dim), device=DEV)
+    cache_write(x, -x, big[0], big[1], slots, **kw(big))
+    cache_write(x, -x, c[0], c[1], slots - slots[0], **kw(c))
+    for y, z in zip(big, c):
+        assert z is None or torch.equal(raw(y)[pages - used:], raw(z))
 
 
 def test_nothing_to_do():
