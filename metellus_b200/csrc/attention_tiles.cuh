@@ -166,7 +166,8 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr bool kScaled = EB == 1, kBf16 = CT == MT_BF16;
     // The matrix pipe truncates what it adds to an accumulator, so a long chain of products
     // drifts. For 32-bit outputs chains are short (4 steps of a score, one tile of O) and
-    // are added up in fp32, rounded to nearest.
+    // are added up in fp32, rounded to nearest; smaller pieces have a chain of their own. fp32, heads of
+    // 128, 18 sequences up to 2280: off by 3.9e-7 (in fp32 throughout 7.6e-7; in one chain 1.7e-6).
     static constexpr bool kExact = kQ32;
     static constexpr int ROW = DP * EB;               // bytes of a (padded) cache row
     static constexpr int CPR = ROW / 16;              // its 16-byte pieces
@@ -183,13 +184,13 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr int PP = CT == MT_F32 ? 2 : kQ32 ? QP : kScaled && std::is_same<Q, __nv_bfloat16>::value ? 1 : 2;
     // queries that fp16 may not hold are divided by a power of two per row
     static constexpr bool kNormed = CT != MT_F32 && !kBf16 && (kQ32 || kScaled);
-    // The exponents' base m is raised only when a score passes it by more than kSlack (a factor of
-    // 2^4), which after a head's first tiles is rare. fp16 probabilities are held times
-    // 2^11, so that they stay below 2^15; the smallest, 2^-24, is 2^-35 of 1.
     // A 16-bit cache's next rows are asked for in two bursts a tile, K's before the scores and V's behind
     // them (64 sequences of 4096 .. 8192, bf16: 249 us, in one burst 257). 8-bit and 32-bit
     // tiles, whose products take longer, lose by it (int8 44 -> 46, fp32 86 -> 91).
     static constexpr bool kTwoBursts = EB == 2;
+    // The exponents' base m is raised only when a score passes it by more than kSlack (a factor of
+    // 2^4), which after a head's first tiles is rare. fp16 probabilities are held times
+    // 2^11, so that they stay below 2^15; the smallest, 2^-24, is 2^-35 of 1.
     static constexpr float kSlack = 4.0f, kOffset = CT == MT_F16 || kScaled ? 11.0f : 0.0f;
     // A part's queries come into shared memory as they are, while the part before is worked
     // on; then they stay in registers as operands, or, where O leaves too few, in shared memory.
@@ -199,15 +200,16 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr int QROW = DP * (kQ32 ? 4 : 2), QPIECES = QROW / 16;
     static constexpr int Q_BYTES = ROWS * QROW + (kQReg || kQRaw ? 0 : KS * NT * QP * 256);
     static constexpr int warp_bytes(int stages) { return stages * STAGE + Q_BYTES + 128; }
-    // stages and resident blocks: 3 blocks an SM (12 warps, 168 registers, enough for O of 64
-    // each) with 3 stages at least, else 2 blocks, else one. With one warp a scheduler instead of two, bf16 under float32
-    // queries took 79 us for 41 us of bytes.
+    // stages and resident blocks: 3 blocks an SM (12 warps, 168 registers, enough for O of 64 each)
+    // with 3 stages at least, else 2 blocks, else one. With one warp a scheduler instead of two, bf16
+    // under float32 queries took 79 us for 41 us of bytes.
     static constexpr int kMost = 227 * 1024;          // of shared memory a block
     static constexpr bool fits(int warps, int stages, int blocks) {
         return warps * warp_bytes(stages) <= kMost && blocks * (warps * warp_bytes(stages) + 1024) <= 228 * 1024;
     }
     // warps a block: 4, or where two blocks of them do not fit, 6 of 32-bit rows with 2 stages (their
-    // products take long), else as many as fit
+    // products take long: 8 heads of 128, 16 sequences of 4096 tokens 107 us, 120 with 4 warps), else
+    // as many as fit
     static constexpr int NW = EB == 4 && !fits(4, 2, 2) && fits(6, 2, 1) ? 6 : fits(4, 2, 1) ? 4 : fits(3, 2, 1) ? 3 : 2;
     static constexpr int kMany = fits(NW, 3, 3) && DP * NT <= 128 ? 3 : fits(NW, 2, 2) ? 2 : 1;
     static constexpr int S = fits(NW, 4, kMany) ? 4 : fits(NW, 3, kMany) ? 3 : 2;
@@ -650,23 +652,24 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         if (Z::kTwoBursts && ask && !mask) fetch(ask_slot, kValues);
         if (mask) {
             // S^T: s[.][.][0], [1] are token oct, heads quad * 2 + 0, 1; [2], [3] token oct + 8. The
-            // largest pieces' products go into `part` first where they are kept apart.
+            // largest pieces' products go into `part` first where they are kept apart, and those of smaller
+            // ones into `small`: added to s each, they would be truncated to its steps.
             float s[TB][NT][4];
 #pragma unroll
             for (int b = 0; b < TB; ++b) {
                 // where they are not, `part` takes every second step: two short chains of products
-                float part[NT][4];
+                float part[NT][4], small[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[b][n][i] = part[n][i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) s[b][n][i] = part[n][i] = small[n][i] = 0.0f;
                 auto times_queries = [&](int k, const uint32_t (&x)[4]) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int p = 0; p < QP; ++p) {
                             const uint2 q = query(k, n, p);
-                            product<CT>((Z::kExact ? p == 0 : k % 2 == 1) ? part[n] : s[b][n], x, q.x, q.y);
+                            product<CT>(Z::kExact ? p == 0 ? part[n] : small[n] : k % 2 == 1 ? part[n] : s[b][n], x, q.x, q.y);
                         }
                     if constexpr (Z::kExact) {
                         if (k % 4 == 3 || (!kPadded && k == KS - 1)) {
@@ -696,7 +699,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             const uint2 q = query(c, n, 0);
-                            product<CT>(s[b][n], lo, q.x, q.y);
+                            product<CT>(small[n], lo, q.x, q.y);
                         }
                     } else if constexpr (kScaled) {
 #pragma unroll
@@ -710,11 +713,13 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         times_queries(c, r);
                     }
                 }
-                if constexpr (!Z::kExact || kPadded)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[b][n][i] += part[n][i];
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (!Z::kExact || kPadded) s[b][n][i] += part[n][i];
+                        if constexpr (Z::kExact && (QP > 1 || CT == MT_F32)) s[b][n][i] += small[n][i];
+                    }
             }
             if constexpr (kScaled) {
                 const float* z = (const float*)(stage + 2 * TW * Z::ROW);
