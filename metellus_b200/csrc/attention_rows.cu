@@ -3,9 +3,16 @@
 // Softmax in one pass: with the running maximum m of the scores, l = sum exp(s - m) and
 // o = sum exp(s - m) v; a new maximum m' scales l and o by exp(m - m'). Every warp of a
 // block keeps its own (m, l, o) over every eighth token; they are joined at the end.
+//
+// It serves what tiles cannot: rows that are not whole 16-byte pieces, caches whose rows have no 32-bit
+// numbers, scales that are not positive. Instructions bound it (a dot product's 5 exchanges for each
+// query head and token): bf16, 32 query heads on 8 of 100, 64 sequences of 1024 tokens 516 us (32 at the
+// copy rate; heads of 104, in tiles, 48). Few sequences are split over clusters of up to 8 blocks:
+// 1 of 16384 tokens 261 us, 2.6 ms in one block each, a token at a time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <cooperative_groups.h>
 
 #include "mt_paged_attention.h"
 
@@ -28,13 +35,20 @@ __device__ inline float rescale(float m_old, float m_new) {
     return m_old == -INFINITY ? 0.0f : exp2f(m_old - m_new);
 }
 
+// Blocks blockIdx.x % splits of a cluster share a sequence's tokens: kChunk at a time a warp, whose rows
+// are asked for together.
+constexpr int kChunk = 4;
+
 template <class Q, class C>
-__global__ void __launch_bounds__(kThreads) attention_rows(const AttentionArgs a) {
+__global__ void __launch_bounds__(kThreads) attention_rows(const AttentionArgs a, int splits) {
     constexpr bool kScaled = sizeof(C) == 1;
     __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows], sm_o[kWarps][kMaxHeadDim];
+    __shared__ float block_m[kRows], block_l[kRows], block_o[kRows][kMaxHeadDim];
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.x, g = blockIdx.y, r0 = blockIdx.z * kRows;
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, split = (int)(blockIdx.x % splits);
+    const int64_t b = blockIdx.x / splits;
+    const int g = blockIdx.y, r0 = blockIdx.z * kRows;
     const int rows = min(kRows, a.group - r0), dim = a.cache.head_dim;
     const int n = min(max(a.lengths[b * a.length_seq], 0), a.max_tokens);
     const int first = n > a.window ? n - a.window : 0;
@@ -51,41 +65,58 @@ __global__ void __launch_bounds__(kThreads) attention_rows(const AttentionArgs a
             o[r][i] = 0.0f;
         }
     }
-    for (int t = first + warp; t < n; t += kWarps) {
-        uint32_t at;
-        const uint32_t j = a.page.div((uint32_t)t, &at);
-        const int page = a.tables[b * a.table_seq + j];
-        if (page < 0 || page >= a.cache.pages) continue;
-        const C* krow = (const C*)a.cache.k.ptr + page * a.cache.k.page + at * a.cache.k.token + g * a.cache.k.head;
-        const C* vrow = (const C*)a.cache.v.ptr + page * a.cache.v.page + at * a.cache.v.token + g * a.cache.v.head;
-        float ks = 1.0f, vs = 1.0f;
-        if constexpr (kScaled) {
-            const CacheView &zk = a.cache.k_scale, &zv = a.cache.v_scale;
-            ks = ((const float*)zk.ptr)[page * zk.page + at * zk.token + g * zk.head];
-            vs = ((const float*)zv.ptr)[page * zv.page + at * zv.token + g * zv.head];
+    // n and a chunk's end are below 2^31 - 1024
+    for (int64_t t0 = first + (int64_t)(split * kWarps + warp) * kChunk; t0 < n; t0 += (int64_t)splits * kWarps * kChunk) {
+        // lanes 0 .. kChunk - 1 look up a token's place each
+        uint32_t at = 0;
+        int page = -1;
+        if (lane < kChunk && t0 + lane < n) {
+            const uint32_t j = a.page.div((uint32_t)(t0 + lane), &at);
+            page = a.tables[b * a.table_seq + j];
+            if (page >= a.cache.pages) page = -1;
         }
-        float k[kPerLane], v[kPerLane];
+        C k[kChunk][kPerLane], v[kChunk][kPerLane];
+        float ks[kChunk], vs[kChunk];
+        bool there[kChunk];
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-            const int d = lane + 32 * i;
-            k[i] = d < dim ? (float)krow[d] : 0.0f;
-            v[i] = d < dim ? (float)vrow[d] * vs : 0.0f;
+        for (int c = 0; c < kChunk; ++c) {
+            const int64_t p = __shfl_sync(0xffffffffu, page, c), u = __shfl_sync(0xffffffffu, at, c);
+            there[c] = p >= 0;
+            ks[c] = vs[c] = 1.0f;
+            if (!there[c]) continue;
+            const C* krow = (const C*)a.cache.k.ptr + p * a.cache.k.page + u * a.cache.k.token + g * a.cache.k.head;
+            const C* vrow = (const C*)a.cache.v.ptr + p * a.cache.v.page + u * a.cache.v.token + g * a.cache.v.head;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+                const int d = lane + 32 * i;
+                k[c][i] = d < dim ? krow[d] : C(0.0f);
+                v[c][i] = d < dim ? vrow[d] : C(0.0f);
+            }
+            if constexpr (kScaled) {
+                const CacheView &zk = a.cache.k_scale, &zv = a.cache.v_scale;
+                ks[c] = ((const float*)zk.ptr)[p * zk.page + u * zk.token + g * zk.head];
+                vs[c] = ((const float*)zv.ptr)[p * zv.page + u * zv.token + g * zv.head];
+            }
         }
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            if (r >= rows) break;
-            float s = 0.0f;
+        for (int c = 0; c < kChunk; ++c) {
+            if (!there[c]) continue;
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) s = fmaf(q[r][i], k[i], s);
+            for (int r = 0; r < kRows; ++r) {
+                if (r >= rows) break;
+                float s = 0.0f;
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            s *= ks * a.scale * kLog2e;
-            const float top = fmaxf(m[r], s);
-            const float keep = rescale(m[r], top), p = s == -INFINITY ? 0.0f : exp2f(s - top);
-            m[r] = top;
-            l[r] = l[r] * keep + p;
+                for (int i = 0; i < kPerLane; ++i) s = fmaf(q[r][i], (float)k[c][i], s);
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) o[r][i] = o[r][i] * keep + p * v[i];
+                for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+                s *= ks[c] * a.scale * kLog2e;
+                const float top = fmaxf(m[r], s);
+                const float keep = rescale(m[r], top), p = s == -INFINITY ? 0.0f : exp2f(s - top);
+                m[r] = top;
+                l[r] = l[r] * keep + p;
+#pragma unroll
+                for (int i = 0; i < kPerLane; ++i) o[r][i] = o[r][i] * keep + p * ((float)v[c][i] * vs[c]);
+            }
         }
     }
 #pragma unroll
@@ -105,40 +136,65 @@ __global__ void __launch_bounds__(kThreads) attention_rows(const AttentionArgs a
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) sm_o[warp][lane + 32 * i] = o[r][i] * keep;
         __syncthreads();
-        const int head = g * a.group + r0 + r;
         for (int d = threadIdx.x; d < dim; d += kThreads) {
             float x = 0.0f;
             for (int w = 0; w < kWarps; ++w) x += sm_o[w][d];
-            ((Q*)a.out)[b * a.out_seq + head * a.out_head + d] = rounded<Q>(sum == 0.0f && top == -INFINITY ? 0.0f : x / sum);
+            block_o[r][d] = x;
         }
-        if (a.lse && threadIdx.x == 0)
-            a.lse[b * a.lse_seq + head * a.lse_head] = (top + log2f(sum)) * kLn2;
+        if (threadIdx.x == 0) {
+            block_m[r] = top;
+            block_l[r] = sum;
+        }
         __syncthreads();
     }
+    // the cluster's blocks join theirs, some rows each
+    cluster.sync();
+    for (int r = split; r < rows; r += splits) {
+        float top = -INFINITY, sum = 0.0f, x[kMaxHeadDim / kThreads] = {};
+        for (int s = 0; s < splits; ++s) top = fmaxf(top, *cluster.map_shared_rank(&block_m[r], s));
+        for (int s = 0; s < splits; ++s) {
+            const float keep = rescale(*cluster.map_shared_rank(&block_m[r], s), top);
+            sum += *cluster.map_shared_rank(&block_l[r], s) * keep;
+            for (int d = threadIdx.x, i = 0; d < dim; d += kThreads, ++i) x[i] += *cluster.map_shared_rank(&block_o[r][d], s) * keep;
+        }
+        const int64_t head = g * a.group + r0 + r;
+        for (int d = threadIdx.x, i = 0; d < dim; d += kThreads, ++i)
+            ((Q*)a.out)[b * a.out_seq + head * a.out_head + d] = rounded<Q>(sum == 0.0f && top == -INFINITY ? 0.0f : x[i] / sum);
+        if (a.lse && threadIdx.x == 0) a.lse[b * a.lse_seq + head * a.lse_head] = (top + log2f(sum)) * kLn2;
+    }
+    cluster.sync();  // until all have read
 }
 
-template <class Q, class C> int launch(const AttentionArgs& a, cudaStream_t st) {
-    const dim3 grid(a.batch, a.cache.kv_heads, (a.group + kRows - 1) / kRows);
-    RT_CHECK(launch_early(attention_rows<Q, C>, grid, kThreads, 0, st, a));
+template <class Q, class C> int launch(const AttentionArgs& a, int sms, cudaStream_t st) {
+    const int row_blocks = (a.group + kRows - 1) / kRows;
+    // a sequence's tokens in up to 8 blocks, as long as there are SMs for them and chunks for their warps
+    const int64_t tokens = a.max_tokens < a.window ? a.max_tokens : a.window;
+    unsigned splits = 1;
+    while (splits < 8 && (int64_t)a.batch * a.cache.kv_heads * row_blocks * splits < sms && tokens > (int64_t)splits * kWarps * kChunk)
+        splits *= 2;
+    const dim3 grid((unsigned)a.batch * splits, a.cache.kv_heads, row_blocks);
+    RT_CHECK(launch_clusters(splits, attention_rows<Q, C>, grid, kThreads, 0, st, a, (int)splits));
     return 0;
 }
 
-template <class Q> int launch8(const AttentionArgs& a, cudaStream_t st) {
-    return a.cache.dtype == MT_I8 ? launch<Q, int8_t>(a, st) : launch<Q, __nv_fp8_e4m3>(a, st);
+template <class Q> int launch8(const AttentionArgs& a, int sms, cudaStream_t st) {
+    return a.cache.dtype == MT_I8 ? launch<Q, int8_t>(a, sms, st) : launch<Q, __nv_fp8_e4m3>(a, sms, st);
 }
 
 }  // namespace
 
-int attend_by_rows(const AttentionArgs& a, cudaStream_t st) {
+int attend_by_rows(const AttentionArgs& a, int dev, cudaStream_t st) {
+    int sms;
+    if (int rc = sm_count(dev, &sms)) return rc;
     const int q = a.q_type, c = a.cache.dtype;
     if (a.cache.scaled()) {
-        if (q == MT_F32) return launch8<float>(a, st);
-        if (q == MT_F16) return launch8<__half>(a, st);
-        return launch8<__nv_bfloat16>(a, st);
+        if (q == MT_F32) return launch8<float>(a, sms, st);
+        if (q == MT_F16) return launch8<__half>(a, sms, st);
+        return launch8<__nv_bfloat16>(a, sms, st);
     }
-    if (c == MT_F32) return launch<float, float>(a, st);
-    if (c == MT_F16) return q == MT_F32 ? launch<float, __half>(a, st) : launch<__half, __half>(a, st);
-    return q == MT_F32 ? launch<float, __nv_bfloat16>(a, st) : launch<__nv_bfloat16, __nv_bfloat16>(a, st);
+    if (c == MT_F32) return launch<float, float>(a, sms, st);
+    if (c == MT_F16) return q == MT_F32 ? launch<float, __half>(a, sms, st) : launch<__half, __half>(a, sms, st);
+    return q == MT_F32 ? launch<float, __nv_bfloat16>(a, sms, st) : launch<__nv_bfloat16, __nv_bfloat16>(a, sms, st);
 }
 
 }  // namespace mt

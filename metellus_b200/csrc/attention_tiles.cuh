@@ -19,6 +19,14 @@
 //   its heads in the workspace, and a second kernel joins them; it is launched early and
 //   waits for the first on the device.
 //
+// Measured (bf16, 32 query heads on 8 of 128, pages of 16 in random order): 64 sequences of 4096 to
+// 8192 tokens 243 us = 6.7 TB/s, the copy rate; 16 of 37 to 4001 27 us = 4.5 TB/s; 1 of 120001 84 us =
+// 5.9 TB/s; 1 of 100 7.6 us. The matrix pipe is busy 14 % of the time and a third of the issue slots are
+// used, so its 16-row form loses nothing here, and the 128-row form of tcgen05 would cut a line of
+// tiles eight times as coarsely and tie the warps of a block to one another's loads. What is left at
+// short lines are the ends: lengths, then page numbers, then rows have to arrive before the first
+// product (4 us), SMs finish up to 3 us apart, and the join takes 2 to 3 us.
+//
 // 8-bit codes become fp16 in registers, exactly; K's scales multiply the scores, V's the
 // probabilities. 32-bit queries (and 32-bit caches) are split into pieces whose products
 // together keep at least 22 bits.

@@ -31,19 +31,28 @@ int sm_count(int dev, int* out);
 // Launches a kernel that begins with `griddepcontrol.wait`: its blocks may be set up while the
 // kernel before it on the stream ends, if that one is of this library too (which allow it early,
 // by `griddepcontrol.launch_dependents`); the wait is for all of that kernel's memory.
+// launch_clusters: in clusters of `cluster` blocks along x.
 template <class... P, class... A>
-cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+cudaError_t launch_clusters(unsigned cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                            A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+template <class... P, class... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+    return launch_clusters(1, kernel, grid, block, smem, st, args...);
 }
 
 // Makes `dev` current for a call and gives the caller its own device back.

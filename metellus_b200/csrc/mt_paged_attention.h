@@ -31,7 +31,7 @@ struct AttentionArgs {
 };
 
 // Any head_dim and alignment: one warp a key row (attention_rows.cu).
-int attend_by_rows(const AttentionArgs& a, cudaStream_t st);
+int attend_by_rows(const AttentionArgs& a, int dev, cudaStream_t st);
 
 // Rows of the cache that 16-byte copies can fetch: tiles on the matrix pipe
 // (attention_tiles.cuh), split over the sequences' lengths. `bytes`: the workspace needed,

@@ -127,7 +127,7 @@ int mt_paged_attention(int dev, const mt_array* q, const mt_paged_cache* cache, 
     OnDevice on;
     RT_CHECK(on.enter(dev));
     if (int rc = call_stream(dev, stream, &st)) return rc;
-    if (!tiled || !(a.scale > 0.0f)) return attend_by_rows(a, st);  // tiles mask and compare scores before they are scaled
+    if (!tiled || !(a.scale > 0.0f)) return attend_by_rows(a, dev, st);  // tiles mask and compare scores before they are scaled
     uint64_t need = 0;
     if (int rc = attend_tiles(a, false, nullptr, &need, dev, st)) return rc;
     if (need && !workspace && !stream) {
