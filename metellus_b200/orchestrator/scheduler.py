@@ -54,6 +54,11 @@ def scratch_of(groups: tuple[KernelGroup, ...]) -> dict[str, int]:
 def buffer_sizes(ops: Operations, groups: tuple[KernelGroup, ...]) -> dict[str, int]:
     """Bytes of every buffer key the plan touches."""
     tensors = ops.tensors
+    keys = {t.buffer_key for t in tensors.values()}
+    for name, cache in ops.caches.items():
+        for key in cache_keys(name, cache):
+            if key in keys:
+                raise ValueError(f"tensor {key!r} has the name of an array of cache {name!r}")
     sizes: dict[str, int] = {}
     for op in ops.build():
         sizes[op.out.buffer_key] = op.out.nbytes

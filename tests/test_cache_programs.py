@@ -153,3 +153,13 @@ def test_cache_arguments(kwargs):
     a.update(kwargs)
     with pytest.raises(ValueError):
         PagedCache(**a)
+
+
+def test_names_of_a_caches_arrays_are_taken():
+    ops = Operations()
+    ops.cache(PagedCache(4, 16, 2, 64), "kv")
+    ops.from_numpy(f32(3, 128), "kv.k")
+    ops.indices(i32(3), "slots")
+    ops.cache_write(k="kv.k", v="kv.k", cache="kv", slots="slots", out="kv1")
+    with pytest.raises(ValueError, match="'kv.k' has the name of an array of cache 'kv'"):
+        schedule(ops, compile_program(ops))
