@@ -218,7 +218,7 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // warps a block: 4, or where two blocks of them do not fit, 6 of 32-bit rows with 2 stages (their
     // products take long: 8 heads of 128, 16 sequences of 4096 tokens 107 us, 120 with 4 warps), else
     // as many as fit
-    static constexpr int NW = EB == 4 && !fits(4, 2, 2) && fits(6, 2, 1) ? 6 : fits(4, 2, 1) ? 4 : fits(3, 2, 1) ? 3 : 2;
+    static constexpr int NW = !fits(4, 2, 2) && fits(6, 2, 1) ? 6 : fits(4, 2, 1) ? 4 : fits(3, 2, 1) ? 3 : 2;
     static constexpr int kMany = fits(NW, 3, 3) && DP * NT <= 128 ? 3 : fits(NW, 2, 2) ? 2 : 1;
     static constexpr int S = fits(NW, 4, kMany) ? 4 : fits(NW, 3, kMany) ? 3 : 2;
     static constexpr int WARP = warp_bytes(S), SMEM = NW * WARP;
@@ -1014,23 +1014,26 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 // item whose tiles lie in several ranges. Which ones is known from the lengths, so it is
 // found out while attention_tiles still runs. x / items is a sequence, or, where there are
 // fewer ranges than sequences, a range: it stands for the sequence that it starts in the
-// middle of, if that ends in it. A block is kTeams teams of DP / 4 threads (4 dims each):
-// `together` rows (a power of two) at a time, kTeams / together parts of each.
-constexpr int kTeams = 8;
+// middle of, if that ends in it. A block is teams of `lanes` threads, 4 dims each: all of DP, or,
+// for long chains of few rows, a slice of it (blockIdx.z), which leaves more teams. They take
+// `together` rows at a time, and of each row every teams / together-th part (all powers of two).
+// 1 sequence of 30000 tokens, 1 head of 256, 592 parts: 20 us, 28 with 8 teams of whole rows.
+constexpr int kLeastLanes = 8;
 
 template <class Q, int DP, int ROWS, int TW>
-__global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ TileArgs t, int by_sequence, int together) {
-    constexpr int kLanes = DP / 4;
-    __shared__ float4 sm_o[kTeams][kLanes];
-    __shared__ float2 sm_ml[kTeams];
+__global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ TileArgs t, int by_sequence, int together, int lanes) {
+    constexpr int kThreads = DP * 2;
+    __shared__ float4 sm_o[kThreads];
+    __shared__ float2 sm_ml[kThreads / kLeastLanes];
     const AttentionArgs& a = t.a;
     asm volatile("griddepcontrol.launch_dependents;");
     uint32_t item, row_block;
     const int x = (int)t.per_range.div(blockIdx.x, &item);
     const int head0 = (int)t.row_blocks.div(item, &row_block) * a.group + (int)row_block * ROWS;
     const int rows = min(ROWS, a.group - (int)row_block * ROWS);
-    const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
-    const int side = team / together, sides = kTeams / together, r = blockIdx.y * together + team % together;
+    const int lane = threadIdx.x % lanes, team = threadIdx.x / lanes, teams = kThreads / lanes;
+    const int side = team / together, sides = teams / together, r = blockIdx.y * together + team % together;
+    const int d0 = (blockIdx.z * lanes + lane) * 4;
     int b, first = 0, count = 0;  // count: parts to join, none or several
     Cursor c;
     const Cuts<TW> cuts(t);
@@ -1076,28 +1079,31 @@ __global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ Til
                 if (part < count) {
                     const int64_t row = (((int64_t)(first + part) * t.items + item) * 2 + (part == 0 ? 1 : 0)) * ROWS + r;
                     ml[j] = t.part_ml[row];
-                    y[j] = *(const float4*)(t.part_o + row * DP + lane * 4);
+                    y[j] = *(const float4*)(t.part_o + row * DP + d0);
                 }
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (i + j * sides < count) take(ml[j], y[j]);
         }
-    if (sides > 1) {
-        sm_o[team][lane] = o;
-        if (lane == 0) sm_ml[team] = make_float2(m, l);
+    for (int half = sides / 2; half > 0; half /= 2) {
+        // the upper half of a row's teams hands over to the lower one
+        if (side >= half) {
+            sm_o[threadIdx.x] = o;
+            if (lane == 0) sm_ml[team] = make_float2(m, l);
+        }
         __syncthreads();
-        for (int w = 1; w < sides && side == 0; ++w) take(sm_ml[team + w * together], sm_o[team + w * together][lane]);
+        if (side < half) take(sm_ml[team + half * together], sm_o[threadIdx.x + half * together * lanes]);
     }
     if (side != 0 || r >= rows) return;
     const bool none = m == -INFINITY && l == 0.0f;
     const float per = 1.0f / l;
     const float y[4] = {o.x, o.y, o.z, o.w};
-    Q* out = (Q*)a.out + (int64_t)b * a.out_seq + (int64_t)(head0 + r) * a.out_head + lane * 4;
+    Q* out = (Q*)a.out + (int64_t)b * a.out_seq + (int64_t)(head0 + r) * a.out_head + d0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (lane * 4 + i < a.cache.head_dim) out[i] = rounded<Q>(none ? 0.0f : y[i] * per);
-    if (lane == 0 && a.lse) a.lse[(int64_t)b * a.lse_seq + (int64_t)(head0 + r) * a.lse_head] = (m + log2f(l)) * kLn2;
+        if (d0 + i < a.cache.head_dim) out[i] = rounded<Q>(none ? 0.0f : y[i] * per);
+    if (d0 == 0 && a.lse) a.lse[(int64_t)b * a.lse_seq + (int64_t)(head0 + r) * a.lse_head] = (m + log2f(l)) * kLn2;
 }
 
 // ---- launch ------------------------------------------------------------------------------------
@@ -1160,10 +1166,14 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     // long chains of few items: a block a row; short ones of many: rows together, so that the
     // blocks fit the GPU about once
     const int64_t joined = (by_sequence ? a.batch : ranges) * t.items, rows = a.group < Z::ROWS ? a.group : Z::ROWS;
-    int together = 1;
-    while (together < kTeams && joined * ((rows + together - 1) / together) > (int64_t)sms * 4) together *= 2;
-    RT_CHECK(launch_early(join_parts<Q, DP, Z::ROWS, Z::TW>, dim3((unsigned)joined, (unsigned)((rows + together - 1) / together)),
-                          dim3(DP * 2), 0, st, t, (int)by_sequence, together));
+    int together = 1, lanes = DP / 4;
+    while (together < 8 && joined * ((rows + together - 1) / together) > (int64_t)sms * 4) together *= 2;
+    // rows in slices while each team has more than one turn of 4 parts (as many as the ranges make on average)
+    const int64_t parts = by_sequence ? ranges / a.batch : 2;
+    while (together == 1 && lanes > kLeastLanes && parts > DP * 2 / lanes * 4 && joined * rows * (DP / 4 / lanes) < (int64_t)sms * 2) lanes /= 2;
+    RT_CHECK(launch_early(join_parts<Q, DP, Z::ROWS, Z::TW>,
+                          dim3((unsigned)joined, (unsigned)((rows + together - 1) / together), (unsigned)(DP / 4 / lanes)), dim3(DP * 2), 0, st, t,
+                          (int)by_sequence, together, lanes));
     return 0;
 }
 
