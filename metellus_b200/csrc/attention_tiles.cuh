@@ -314,7 +314,7 @@ template <int CT, class Q, int DP, int NT, bool kPadded>
 __global__ void __launch_bounds__(Shape<CT, Q, DP, NT>::NW * 32, Shape<CT, Q, DP, NT>::BLOCKS)
 attention_tiles(const __grid_constant__ TileArgs t) {
     using Z = Shape<CT, Q, DP, NT>;
-    constexpr int NW = Z::NW, TW = Z::TW, TB = Z::TB, S = Z::S, CPR = Z::CPR, ROWS = Z::ROWS, QP = Z::QP, PP = Z::PP, KS = Z::KS;
+    constexpr int TW = Z::TW, TB = Z::TB, S = Z::S, CPR = Z::CPR, ROWS = Z::ROWS, QP = Z::QP, PP = Z::PP, KS = Z::KS;
     constexpr bool kScaled = Z::kScaled, kBf16 = Z::kBf16;
     extern __shared__ __align__(128) unsigned char smem[];
     const AttentionArgs& a = t.a;
@@ -324,7 +324,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     uint2* const sm_q = (uint2*)(sm_raw + ROWS * Z::QROW);                // and as operands, where not in registers
     int4* const sm_meta = (int4*)(ring + Z::WARP - 128);
 
-    const int me = blockIdx.x * NW + warp;
+    const int me = blockIdx.x * (blockDim.x >> 5) + warp;
     uint32_t item;
     const int range = (int)t.per_range.div((uint32_t)me, &item);
     uint32_t row_block;
@@ -1134,19 +1134,20 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     // so, the more of the warps that fit the GPU at once the sequences occupy: then a join has many
     // parts, and cutting gives each warp less to gain. Long tiles make up for a join sooner. us, whole
     // and cut: bf16, 8 heads of 128, 1 sequence of 4 tiles 8.3, 7.3; 40 sequences (a quarter of the
-    // warps) of 6 tiles 10.4, 11.4, of 12 tiles 15.5, 12.5; fp32, 8 heads of 256, 8 sequences of 2 tiles
-    // 18.6, 15.5, of 4 tiles 29.8, 15.5.
+    // warps) of 6 tiles 10.4, 11.4, of 12 tiles 15.5, 12.5; 110 (three quarters) of 16 tiles 23.1,
+    // 29.7; fp32, 8 heads of 256, 8 sequences of 2 tiles 18.6, 15.5, of 4 tiles 29.8, 15.5.
     // Otherwise as many ranges as those warps can take the heads of, or fewer where there cannot be as
     // many tiles.
     const int64_t resident = (int64_t)sms * Z::BLOCKS * Z::NW, used = (int64_t)a.batch * t.items;
-    constexpr int kTile = Z::TW * DP * (Z::EB == 4 ? 2 : 1), kFew = kTile <= 1024 ? 4 : kTile <= 2048 ? 3 : 2;
-    constexpr int kMore = Z::EB == 4 || Z::TW == 32 ? 6 : 24;
-    t.whole = most <= kFew + (used <= resident ? kMore * used / resident : 0);
+    constexpr int kTile = Z::TW * DP * (Z::EB == 4 ? 2 : 1), kFew = kTile <= 1024 ? 4 : kTile <= 2048 ? 3 : kTile <= 4096 ? 2 : 1;
+    constexpr int kMore = Z::EB == 4 || Z::TW == 32 ? 5 : 18;
+    const double share = used <= resident ? (double)used / (double)resident : 0.0;
+    t.whole = (double)most <= kFew + kMore * share * (1.0 + share);
     int64_t ranges = resident / t.items;
     if (ranges < 1) ranges = 1;
     if (ranges > a.batch * most) ranges = a.batch * most;
     if (t.whole) ranges = a.batch;
-    const int64_t warps = ranges * t.items, blocks = (warps + Z::NW - 1) / Z::NW;
+    const int64_t warps = ranges * t.items;
     const uint64_t ml_bytes = (uint64_t)warps * 2 * Z::ROWS * 8;
     *bytes = t.whole ? 0 : ml_bytes + (uint64_t)warps * 2 * Z::ROWS * DP * 4;
     if (!run) return 0;
@@ -1160,7 +1161,10 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
         RT_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::SMEM));
         is_ready = true;
     }
-    RT_CHECK(launch_early(kernel, dim3((unsigned)blocks), dim3(Z::NW * 32), Z::SMEM, st, t));
+    // warps of whole sequences are spread over the SMs, where one block fits them at a time
+    const int64_t spread = (warps + sms - 1) / sms;
+    const int per_block = t.whole && Z::BLOCKS == 1 && spread < Z::NW ? (int)spread : Z::NW;
+    RT_CHECK(launch_early(kernel, dim3((unsigned)((warps + per_block - 1) / per_block)), dim3(per_block * 32), per_block * Z::WARP, st, t));
     if (t.whole) return 0;
     const bool by_sequence = a.batch <= ranges;
     // long chains of few items: a block a row; short ones of many: rows together, so that the
