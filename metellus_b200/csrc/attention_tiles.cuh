@@ -20,8 +20,8 @@
 //   waits for the first on the device.
 //
 // Measured (bf16, 32 query heads on 8 of 128, pages of 16 in random order): 64 sequences of 4096 to
-// 8192 tokens 243 us = 6.7 TB/s, the copy rate; 16 of 37 to 4001 27 us = 4.5 TB/s; 1 of 120001 84 us =
-// 5.9 TB/s; 1 of 100 7.6 us. The matrix pipe is busy 14 % of the time and a third of the issue slots are
+// 8192 tokens 243 us = 6.7 TB/s, the copy rate; 16 of 37 to 4001 27 us = 4.5 TB/s; 1 of 120001 82 us =
+// 6.0 TB/s; 1 of 100 7.6 us. The matrix pipe is busy 14 % of the time and a third of the issue slots are
 // used, so its 16-row form loses nothing here, and the 128-row form of tcgen05 would cut a line of
 // tiles eight times as coarsely and tie the warps of a block to one another's loads. What is left at
 // short lines are the ends: lengths, then page numbers, then rows have to arrive before the first
@@ -1017,7 +1017,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 // middle of, if that ends in it. A block is teams of `lanes` threads, 4 dims each: all of DP, or,
 // for long chains of few rows, a slice of it (blockIdx.z), which leaves more teams. They take
 // `together` rows at a time, and of each row every teams / together-th part (all powers of two).
-// 1 sequence of 30000 tokens, 1 head of 256, 592 parts: 20 us, 28 with 8 teams of whole rows.
+// 1 sequence of 30000 tokens, 1 head of 256, 888 parts: 18 us, 47 with 8 teams of whole rows.
 constexpr int kLeastLanes = 8;
 
 template <class Q, int DP, int ROWS, int TW>
@@ -1135,12 +1135,12 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     // parts, and cutting gives each warp less to gain. Long tiles make up for a join sooner. us, whole
     // and cut: bf16, 8 heads of 128, 1 sequence of 4 tiles 8.3, 7.3; 40 sequences (a quarter of the
     // warps) of 6 tiles 10.4, 11.4, of 12 tiles 15.5, 12.5; 110 (three quarters) of 16 tiles 23.1,
-    // 29.7; fp32, 8 heads of 256, 8 sequences of 2 tiles 18.6, 15.5, of 4 tiles 29.8, 15.5.
+    // 29.7 (of 1 to 16 tiles 21.4, 22.6); fp32, 8 heads of 256, 8 sequences of 2 tiles 18.6, 15.5, of 4 tiles 29.8, 15.5.
     // Otherwise as many ranges as those warps can take the heads of, or fewer where there cannot be as
     // many tiles.
     const int64_t resident = (int64_t)sms * Z::BLOCKS * Z::NW, used = (int64_t)a.batch * t.items;
     constexpr int kTile = Z::TW * DP * (Z::EB == 4 ? 2 : 1), kFew = kTile <= 1024 ? 4 : kTile <= 2048 ? 3 : kTile <= 4096 ? 2 : 1;
-    constexpr int kMore = Z::EB == 4 || Z::TW == 32 ? 5 : 18;
+    constexpr int kMore = Z::EB == 4 || Z::TW == 32 ? 5 : 15;
     const double share = used <= resident ? (double)used / (double)resident : 0.0;
     t.whole = (double)most <= kFew + kMore * share * (1.0 + share);
     int64_t ranges = resident / t.items;
