@@ -183,8 +183,8 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr int TW = kScaled && DP <= 128 ? 32 : 16, TB = TW / 16;
     static constexpr int STAGE = 2 * TW * ROW + (kScaled ? 256 : 0);  // rows of K, of V, scales of 32 tokens each
     // Whether step c of a row's pairs of pieces may be behind its end: rows are longer than half of
-    // DP, but for DP = 64
-    __host__ __device__ static constexpr bool may_end(int c) { return DP == 64 ? c >= 1 : 4 * c >= CPR; }
+    // DP, but for DP = 32
+    __host__ __device__ static constexpr bool may_end(int c) { return DP == 32 ? c >= 1 : 4 * c >= CPR; }
     static constexpr int KS = CT == MT_F32 ? DP / 8 : DP / 16;    // steps of K Q^T
     // pieces of a query: fp16 11 bits, bf16 8 bits, tf32 11 bits each
     static constexpr int QP = CT == MT_F32 ? 2 : !kQ32 ? 1 : kBf16 ? 3 : 2;
@@ -205,11 +205,11 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // Those that are operands as they are (one piece) need no second place, and come late.
     static constexpr bool kQReg = KS * 2 * NT * QP + DP / 4 * NT <= (EB == 4 ? 192 : 168), kQRaw = !kQReg && QP == 1 && !kNormed;
     static constexpr int ROWS = NT * 8;
-    static constexpr int QROW = DP * (kQ32 ? 4 : 2), QPIECES = QROW / 16;
+    static constexpr int QROW = DP * (kQ32 ? 4 : 2), QPIECES = QROW / 16, QSPREAD = QPIECES < 8 ? QPIECES - 1 : 7;
     static constexpr int Q_BYTES = ROWS * QROW + (kQReg || kQRaw ? 0 : KS * NT * QP * 256);
     static constexpr int warp_bytes(int stages) { return stages * STAGE + Q_BYTES + 128; }
-    // stages and resident blocks: 3 blocks an SM (12 warps, 168 registers, enough for O of 64 each)
-    // with 3 stages at least, else 2 blocks, else one. With one warp a scheduler instead of two, bf16
+    // stages and resident blocks: 3 blocks an SM (12 warps, 168 registers, enough for O of 64 each;
+    // 4 for heads of 32) with 3 stages at least, else 2 blocks, else one. With one warp a scheduler instead of two, bf16
     // under float32 queries took 79 us for 41 us of bytes.
     static constexpr int kMost = 227 * 1024;          // of shared memory a block
     static constexpr bool fits(int warps, int stages, int blocks) {
@@ -219,7 +219,7 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // products take long: 8 heads of 128, 16 sequences of 4096 tokens 107 us, 120 with 4 warps), else
     // as many as fit
     static constexpr int NW = !fits(4, 2, 2) && fits(6, 2, 1) ? 6 : fits(4, 2, 1) ? 4 : fits(3, 2, 1) ? 3 : 2;
-    static constexpr int kMany = fits(NW, 3, 3) && DP * NT <= 128 ? 3 : fits(NW, 2, 2) ? 2 : 1;
+    static constexpr int kMany = fits(NW, 3, 4) && DP * NT <= 32 ? 4 : fits(NW, 3, 3) && DP * NT <= 128 ? 3 : fits(NW, 2, 2) ? 2 : 1;
     static constexpr int S = fits(NW, 4, kMany) ? 4 : fits(NW, 3, kMany) ? 3 : 2;
     static constexpr int WARP = warp_bytes(S), SMEM = NW * WARP;
     static constexpr int BLOCKS = kMany;
@@ -446,7 +446,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     // exchanged as the cache's are.
     auto q_place = [](int r, int d) {
         const int byte = d * (int)sizeof(Q);
-        return r * Z::QROW + ((byte >> 4 ^ (r & 7)) << 4 | (byte & 15));
+        return r * Z::QROW + ((byte >> 4 ^ (r & Z::QSPREAD)) << 4 | (byte & 15));
     };
     auto ask_queries = [&](int b) {
         const Q* const q = (const Q*)a.q + (int64_t)b * a.q_seq + (int64_t)head0 * a.q_head;
@@ -454,7 +454,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         if (t.q_chunks)
             for (int i = lane; i < rows * t.q_chunks; i += 32) {
                 const int r = i / t.q_chunks, piece = i - r * t.q_chunks;
-                copy16<false>(to + r * Z::QROW + (piece ^ (r & 7)) * 16, (const unsigned char*)(q + (int64_t)r * a.q_head) + piece * 16, true);
+                copy16<false>(to + r * Z::QROW + (piece ^ (r & Z::QSPREAD)) * 16, (const unsigned char*)(q + (int64_t)r * a.q_head) + piece * 16, true);
             }
         else
             for (int i = lane; i < rows * a.cache.head_dim; i += 32) {
@@ -1204,6 +1204,8 @@ int by_group(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes,
 
 template <int CT, class Q> int by_shape(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
     const int dim = a.cache.head_dim;
+    // (bf16 heads of 32, 8 of them, 16 sequences of 4096 tokens: 20 us, 33 as half of 64)
+    if (dim <= 32) return by_group<CT, Q, 32>(a, run, workspace, bytes, dev, st);
     if (dim <= 64) return by_group<CT, Q, 64>(a, run, workspace, bytes, dev, st);
     if (dim <= 128) return by_group<CT, Q, 128>(a, run, workspace, bytes, dev, st);
     return by_group<CT, Q, 256>(a, run, workspace, bytes, dev, st);

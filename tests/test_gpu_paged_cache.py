@@ -243,6 +243,12 @@ def test_attention_odd_head_dims(q_type, dtype, dim):
     compare(*make([0, 50, 300], 6, 2, dim, 16, q_type, dtype))
 
 
+@pytest.mark.parametrize("q_type,dtype", PAIRS)
+@pytest.mark.parametrize("dim", [4, 8, 16, 24, 32, 48])
+def test_attention_small_head_dims(q_type, dtype, dim):
+    compare(*make([0, 1, 50, 300, 2000], 12, 3, dim, 16, q_type, dtype))
+
+
 @pytest.mark.parametrize("q_type,dtype", [(F32, F32), (BF16, BF16), (F32, F16), (BF16, I8), (F32, E4M3)])
 @pytest.mark.parametrize("window", [1, 16, 100, 5000])
 def test_attention_window(q_type, dtype, window):
