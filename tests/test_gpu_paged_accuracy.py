@@ -1,0 +1,82 @@
+"""How near the paged attention's outputs are to the formula in 64 bits, where the bounds of
+``paged_reference`` are too wide to show it: every output must be what some number within the
+kernel's own error of the exact one rounds to.
+
+That error, with D terms a score, n tokens and A = sum p |v|:
+
+* scores: (D + 12) 2^-23 sum |q k|, and D 2^-24 max |q| max |k| where elements of a query are held
+  as multiples of 2^-24 of its largest; a score off by ds moves an output by 2 ds A;
+* exponentials, products and sums: 2 (n + 16) 2^-23 A;
+* probabilities in two pieces, of half a step each: 2^-22 A (fp16), 2^-16 A (bf16), and, of fp16, half
+  the smallest step: 2^-35 of the largest weight that a token has, times the largest V, n times."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from metellus_b200 import paged_attention
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16, I8, E4M3 = torch.float32, torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _device(cuda_device):
+    torch.manual_seed(7)
+
+
+def attend(q, k, v, n, k_scale=None, v_scale=None):
+    """The kernel's outputs for caches given as rows [batch, tokens, kv_heads, dim], in pages of 8."""
+    b, tokens = k.shape[:2]
+    k, v, k_scale, v_scale = (None if x is None else x.unflatten(1, (-1, 8)).flatten(0, 1) for x in (k, v, k_scale, v_scale))
+    tables = torch.arange(b * tokens // 8, device=DEV, dtype=torch.int32).view(b, -1)
+    return paged_attention(q, k, v, tables, n, k_scale=k_scale, v_scale=v_scale)
+
+
+def exact(q, k, v, n, k_scale=None, v_scale=None):
+    """(outputs, error before they are rounded), float64."""
+    b, heads, dim = q.shape
+    piece = 2.0 ** -16 if k.dtype is BF16 else 2.0 ** -22
+    one = torch.ones(k.shape[:3], device=DEV, dtype=torch.float64)
+    ks, vs = (one if z is None else z.double() for z in (k_scale, v_scale))
+    codes, k, v = v.double(), k.double() * ks[..., None], v.double() * vs[..., None]
+    q = q.double().unflatten(1, (k.shape[2], -1))
+    there = (torch.arange(k.shape[1], device=DEV) < n[:, None])[:, None, None, :]
+    s = torch.einsum("bhgd,bthd->bhgt", q, k) * dim ** -0.5
+    p = torch.softmax(s.masked_fill(~there, -torch.inf), -1)
+    size = torch.einsum("bhgd,bthd->bhgt", q.abs(), k.abs()).masked_fill(~there, 0).amax(-1, keepdim=True)
+    least = q.abs().amax(-1, keepdim=True) * k.abs().amax((1, 3))[:, :, None, None]
+    ds = ((dim + 12) * 2.0 ** -23 * size + dim * 2.0 ** -24 * least) * dim ** -0.5
+    o = torch.einsum("bhgt,bthd->bhgd", p, v)
+    A = torch.einsum("bhgt,bthd->bhgd", p, v.abs())
+    weight = (p * vs.transpose(1, 2)[:, :, None, :]).amax(-1, keepdim=True)
+    d = A * (piece + 2 * ds + 2 * (n.double()[:, None, None, None] + 16) * 2.0 ** -23)
+    d = d + n[:, None, None, None] * 2.0 ** -35 * weight * codes.abs().amax()
+    return o.flatten(1, 2), d.flatten(1, 2)
+
+
+def check(got, o, d):
+    lo, hi = (o - d).to(got.dtype), (o + d).to(got.dtype)
+    bad = ~((lo <= got) & (got <= hi))
+    assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} outside, such as {got[bad][0]:.9g} of "
+                           f"{lo[bad][0]:.9g} .. {hi[bad][0]:.9g}")
+
+
+def codes(shape, dtype):
+    return (torch.randn(shape, device=DEV) * 30).round().clamp(-100, 100).to(dtype)
+
+
+@pytest.mark.parametrize("q_type,dtype", [(BF16, I8), (BF16, E4M3), (F16, I8), (F16, E4M3), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (16, 1, 80)])
+def test_probabilities_keep_their_bits(q_type, dtype, heads, kv_heads, dim):
+    """A few tokens of about equal weight: one rounded piece a probability would show in the outputs."""
+    shape = (96, 8, kv_heads, dim)
+    scaled = dtype in (I8, E4M3)
+    k, v = (codes(shape, dtype) if scaled else torch.randn(shape, device=DEV).to(dtype) for _ in range(2))
+    z = [0.002 + 0.03 * torch.rand(shape[:3], device=DEV) if scaled else None for _ in range(2)]
+    q = (torch.randn((shape[0], heads, dim), device=DEV) * 0.3).to(q_type)
+    n = torch.randint(2, 9, (shape[0],), device=DEV, dtype=torch.int32)
+    check(attend(q, k, v, n, *z), *exact(q, k, v, n, *z))
