@@ -177,6 +177,11 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // are added up in fp32, rounded to nearest; smaller pieces have a chain of their own. fp32, heads of
     // 128, 18 sequences up to 2280: off by 3.9e-7 (in fp32 throughout 7.6e-7; in one chain 1.7e-6).
     static constexpr bool kExact = kQ32;
+    // For 16-bit outputs O's chains are kChain tiles long, and added up in the workspace. 1770 tiles of values
+    // around 1 come out 1.5e-5 too small (7e-6 with 64), in one chain 2.4e-4, fp16's
+    // half step. 64 sequences of 4096 to 8192 tokens, bf16: 246.4 us, in one chain 243.7, 64 tiles 248; a sum
+    // a tile, in registers, would cost up to 14 % (16-bit) and 31 % (8-bit, 16 heads a warp).
+    static constexpr int kChain = 128;
     static constexpr int ROW = DP * EB;               // bytes of a (padded) cache row
     static constexpr int CPR = ROW / 16;              // its 16-byte pieces
     // tokens a tile: 8-bit rows are short, and a tile's chain of instructions takes as long
@@ -610,6 +615,43 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     float o[DP / 16][NT][4], m[NT][2], base[NT][2], limit[NT][2], l[NT][2];
     float v_unit = 0.0f;  // O is in units of this power of two (8-bit caches)
     int slot = 0, in_part = S;  // tiles of this part so far
+    // O of a part's earlier tiles lies where the part's own is left at its end, each lane's accumulators, and
+    // what they are relative to beside it. (Sequences taken whole, without a workspace, are shorter than kChain.)
+    auto place_of = [&](int flags) { return (int64_t)me * 2 + (flags & kFromStart ? 1 : 0); };
+    auto add_earlier = [&](int flags) {
+        const float* const from = t.part_o + place_of(flags) * (ROWS * DP) + lane;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 then = t.part_ml[place_of(flags) * ROWS + n * 8 + quad * 2 + i];
+                float by = exp2_fast(then.x - base[n][i]);
+                if constexpr (kScaled) by *= then.y / v_unit;
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                    for (int j = i; j < 4; j += 2) o[d][n][j] += from[((d * NT + n) * 4 + j) * 32] * by;
+            }
+    };
+    auto leave = [&](int flags) {
+        if (in_part > Z::kChain) add_earlier(flags);
+        __syncwarp();
+        float* const to = t.part_o + place_of(flags) * (ROWS * DP) + lane;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (oct == 0) t.part_ml[place_of(flags) * ROWS + n * 8 + quad * 2 + i] = make_float2(m[n][i] == -INFINITY ? -INFINITY : base[n][i], v_unit);
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                    for (int j = i; j < 4; j += 2) {
+                        to[((d * NT + n) * 4 + j) * 32] = o[d][n][j];
+                        o[d][n][j] = 0.0f;
+                    }
+            }
+        __syncwarp();
+    };
     for (int tile = 0; tile < tiles; ++tile) {
         __syncwarp();
         // the tile S - 1 ahead goes into the last one's stage
@@ -944,7 +986,9 @@ attention_tiles(const __grid_constant__ TileArgs t) {
             }
         }
         copies_commit();
+        if (!Z::kExact && in_part % Z::kChain == 0 && !(meta.y & kLast)) leave(meta.y);
         if (meta.y & kLast) {
+            if (!Z::kExact && in_part > Z::kChain) add_earlier(meta.y);
             // -- the part ends: from the accumulators' layout to rows by way of this tile's stage, into which
             // nothing will be fetched before the next tile
             __syncwarp();
@@ -1144,6 +1188,7 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     constexpr int kMore = Z::EB == 4 || Z::TW == 32 ? 5 : 15;
     const double share = used <= resident ? (double)used / (double)resident : 0.0;
     t.whole = (double)most <= kFew + kMore * share * (1.0 + share);
+    static_assert(kFew + 2 * kMore < Z::kChain, "whole sequences have no workspace");
     int64_t ranges = resident / t.items;
     if (ranges < 1) ranges = 1;
     if (ranges > a.batch * most) ranges = a.batch * most;

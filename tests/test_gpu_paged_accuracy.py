@@ -80,3 +80,25 @@ def test_probabilities_keep_their_bits(q_type, dtype, heads, kv_heads, dim):
     q = (torch.randn((shape[0], heads, dim), device=DEV) * 0.3).to(q_type)
     n = torch.randint(2, 9, (shape[0],), device=DEV, dtype=torch.int32)
     check(attend(q, k, v, n, *z), *exact(q, k, v, n, *z))
+
+
+@pytest.mark.parametrize("q_type,dtype", [(F16, F16), (BF16, BF16), (F16, E4M3), (F32, F16), (F32, F32)])
+def test_long_sums_do_not_drift(q_type, dtype):
+    """Values of one sign, thousands of tiles a warp, in a cache of 512 tokens that is seen 256 times over. Outputs
+    are, on the average, what the exact ones round to: a shift of them by 2^-15, a sixteenth of fp16's half step,
+    moves that many more to the next value. (Not the mean of their errors: the 1024 values differ little from
+    one sequence to another, so bf16's roundings alone have a mean of 2^-8 / sqrt(3 * 1024).)"""
+    batch, heads, kv_heads, dim, tokens, times = 32, 32, 8, 128, 512, 256
+    k = torch.randn((1, tokens, kv_heads, dim), device=DEV).to(dtype)
+    v = (1 + 0.2 * torch.randn((1, tokens, kv_heads, dim), device=DEV)).to(dtype)
+    q = (torch.randn((batch, heads, dim), device=DEV) * 0.25).to(q_type)
+    z = [torch.ones((1, tokens, kv_heads), device=DEV) if dtype is E4M3 else None] * 2
+    pages = [None if x is None else x.unflatten(1, (-1, 8)).flatten(0, 1) for x in (k, v, *z)]
+    tables = torch.arange(tokens // 8, device=DEV, dtype=torch.int32).repeat(batch, times)
+    n = torch.full((batch,), tokens * times, device=DEV, dtype=torch.int32)
+    got = paged_attention(q, *pages[:2], tables, n, k_scale=pages[2], v_scale=pages[3]).double()
+    seen = torch.full((batch,), tokens, device=DEV, dtype=torch.int32)
+    o, _ = exact(q, *(x.expand(batch, -1, -1, -1) for x in (k, v)), seen, *(None if x is None else x.expand(batch, -1, -1) for x in z))
+    assert abs(float(((got - o.to(q_type).double()) / o).mean())) <= 2.0 ** -15
+    half_step = torch.finfo(q_type).eps / 2
+    assert float(((got - o) / o).abs().max()) <= half_step + 2.0 ** -13
