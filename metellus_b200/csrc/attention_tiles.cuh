@@ -204,8 +204,13 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr bool kTwoBursts = EB == 2;
     // The exponents' base m is raised only when a score passes it by more than kSlack (a factor of
     // 2^4), which after a head's first tiles is rare. fp16 probabilities are held times
-    // 2^11, so that they stay below 2^15; the smallest, 2^-24, is 2^-35 of 1.
-    static constexpr float kSlack = 4.0f, kOffset = CT == MT_F16 || kScaled ? 11.0f : 0.0f;
+    // 2^11, so that they stay below 2^15; the smallest, 2^-24, is 2^-35 of 1. Those of an 8-bit cache are
+    // multiplied by V's scales before they are fp16, and held in units of 2^-11 of the largest scale, or, where
+    // that is kSpread times a head's largest product or more, of 2^-5 of the product. (In units of the scale
+    // alone a token that has no weight cost the others their bits: float32 queries, one token's scale 10^8
+    // times the others': off by 5.5e-4, now 2.3e-7.)
+    static constexpr float kSlack = 4.0f, kOffset = CT == MT_F16 ? 11.0f : 0.0f;
+    static constexpr float kLeastUnit = 1.17549435e-38f, kSpread = 64.0f;  // 2^-126, 2^6
     // A part's queries come into shared memory as they are, while the part before is worked
     // on; then they stay in registers as operands, or, where O leaves too few, in shared memory.
     // Those that are operands as they are (one piece) need no second place, and come late.
@@ -613,7 +618,10 @@ attention_tiles(const __grid_constant__ TileArgs t) {
     // per query head: the largest score when the base was set, the base of the exponents (less the
     // offset), and the score above which it is set again
     float o[DP / 16][NT][4], m[NT][2], base[NT][2], limit[NT][2], l[NT][2];
-    float v_unit = 0.0f;  // O is in units of this power of two (8-bit caches)
+    auto inverse = [](float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); };  // of a power of two
+    // 8-bit caches: O, and the products of probabilities and scales, are in units of this power of two; scales
+    // up to `roof` cannot take a product out of fp16's range
+    float unit[NT][2], roof = 0.0f;
     int slot = 0, in_part = S;  // tiles of this part so far
     // O of a part's earlier tiles lies where the part's own is left at its end, each lane's accumulators, and
     // what they are relative to beside it. (Sequences taken whole, without a workspace, are shorter than kChain.)
@@ -626,7 +634,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
             for (int i = 0; i < 2; ++i) {
                 const float2 then = t.part_ml[place_of(flags) * ROWS + n * 8 + quad * 2 + i];
                 float by = exp2_fast(then.x - base[n][i]);
-                if constexpr (kScaled) by *= then.y / v_unit;
+                if constexpr (kScaled) by *= then.y / unit[n][i];
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
@@ -641,7 +649,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (oct == 0) t.part_ml[place_of(flags) * ROWS + n * 8 + quad * 2 + i] = make_float2(m[n][i] == -INFINITY ? -INFINITY : base[n][i], v_unit);
+                if (oct == 0) t.part_ml[place_of(flags) * ROWS + n * 8 + quad * 2 + i] = make_float2(m[n][i] == -INFINITY ? -INFINITY : base[n][i], unit[n][i]);
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
@@ -686,14 +694,15 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     m[n][i] = limit[n][i] = -INFINITY;
                     base[n][i] = -Z::kOffset;
                     l[n][i] = 0.0f;
+                    unit[n][i] = Z::kLeastUnit;
                 }
+            roof = 0.0f;
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[d][n][i] = 0.0f;
-            v_unit = 1.17549435e-38f;  // 2^-126
         }
         copies_wait<S - 2>();  // this turn's are not committed yet
         __syncwarp();
@@ -795,19 +804,18 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         for (int i = 0; i < 4; ++i)
                             if (!(mask >> (b * 16 + (i >> 1) * 8 + oct) & 1)) s[b][n][i] = -INFINITY;
             }
-            float vs[TB][2], keep[NT][2];
+            float vs[TB][2], keep[NT][2], most_v = 0.0f;
             bool grown = false;
             if constexpr (kScaled) {
                 const float* z = (const float*)(stage + 2 * TW * Z::ROW) + 32;
-                float top = 0.0f;
 #pragma unroll
                 for (int b = 0; b < TB; ++b)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         vs[b][h] = z[b * 16 + h * 8 + oct];
-                        top = fmaxf(top, fabsf(vs[b][h]));
+                        most_v = fmaxf(most_v, fabsf(vs[b][h]));
                     }
-                grown = top >= v_unit;
+                grown = most_v > roof;
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -822,20 +830,9 @@ attention_tiles(const __grid_constant__ TileArgs t) {
             // scores are compared and kept as the products give them; qscale turns them into exponents
             const bool rescale = __any_sync(0xffffffffu, grown);
             if (rescale) {
-                float shrink = 1.0f;
-                if constexpr (kScaled) {
-                    float top = 0.0f;
+                if constexpr (kScaled)
 #pragma unroll
-                    for (int b = 0; b < TB; ++b) top = fmaxf(top, fmaxf(fabsf(vs[b][0]), fabsf(vs[b][1])));
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    // the power of two above the largest scale so far
-                    const float unit = __uint_as_float((min(__float_as_uint(top) >> 23, 252u) + 1) << 23);
-                    if (unit > v_unit) {
-                        shrink = v_unit / unit;
-                        v_unit = unit;
-                    }
-                }
+                    for (int d = 4; d < 32; d <<= 1) most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, d));
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -849,30 +846,15 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                         const float k = m[n][i] == -INFINITY ? 0.0f : exp2_fast((base[n][i] + Z::kOffset) - now);
                         m[n][i] = top;
                         base[n][i] = now - Z::kOffset;
-                        limit[n][i] = top == -INFINITY ? top : top + Z::kSlack / qscale[n][i];
+                        // (with the division that rounds to nearest 1 sequence of 100 tokens, int8, takes 9.4 us, so 8.4)
+                        limit[n][i] = top == -INFINITY ? top : top + __fdividef(Z::kSlack, qscale[n][i]);
                         l[n][i] *= k;
-                        keep[n][i] = kScaled ? k * shrink : k;
+                        keep[n][i] = k;
                     }
-                if constexpr (!Z::kExact) {
-#pragma unroll
-                    for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[d][n][i] *= keep[n][i & 1];
-                }
-            }
-            if constexpr (kScaled) {
-                const float per = __uint_as_float((254u << 23) - __float_as_uint(v_unit));  // 1 / v_unit
-#pragma unroll
-                for (int b = 0; b < TB; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) vs[b][h] *= per;
             }
             if (Z::kTwoBursts && ask) fetch(ask_slot, kValues);
-            uint32_t pf[TB][NT][2 * PP];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -882,8 +864,58 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                             float& x = s[b][n][2 * h + i];
                             x = exp2_fast(fmaf(x, qscale[n][i], -base[n][i]));
                             l[n][i] += x;
-                            if constexpr (kScaled) x *= vs[b][h];
                         }
+            if constexpr (kScaled) {
+#pragma unroll
+                for (int b = 0; b < TB; ++b)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[b][n][i] *= vs[b][i >> 1];
+                if (rescale) {
+                    // the next power of two
+                    auto above = [](float x) { return __uint_as_float((min(__float_as_uint(x) >> 23, 252u) + 1) << 23); };
+                    roof = INFINITY;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float most = 0.0f;
+#pragma unroll
+                            for (int b = 0; b < TB; ++b) most = fmaxf(most, fmaxf(fabsf(s[b][n][i]), fabsf(s[b][n][2 + i])));
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                            // (a unit that is much smaller than before could take O out of fp32's range)
+                            const float before = __uint_as_float(__float_as_uint(unit[n][i] * keep[n][i]) & 0xff800000u);
+                            const float now = fmaxf(fmaxf(above(most), fminf(above(most_v), above(most) * Z::kSpread)) * 0x1p-11f,
+                                                    fmaxf(before, Z::kLeastUnit));
+                            if (keep[n][i] > 0.0f) keep[n][i] *= unit[n][i] * inverse(now);
+                            unit[n][i] = now;
+                            roof = fminf(roof, now * 0x1p11f);
+                        }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float per = inverse(unit[n][i & 1]);
+#pragma unroll
+                        for (int b = 0; b < TB; ++b) s[b][n][i] *= per;
+                    }
+            }
+            if constexpr (!Z::kExact) {
+                if (rescale) {
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[d][n][i] *= keep[n][i & 1];
+                }
+            }
+            uint32_t pf[TB][NT][2 * PP];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int b = 0; b < TB; ++b) {
                     if constexpr (CT == MT_F32) {
@@ -1010,7 +1042,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
                     const float exponent = m[n][i] == -INFINITY ? -INFINITY : base[n][i];
                     const int r = quad * 2 + i, row = n * 8 + r;
                     float f = !whole ? 1.0f : none ? 0.0f : 1.0f / sum;
-                    if constexpr (kScaled) f *= v_unit;
+                    if constexpr (kScaled) f *= unit[n][i];
 #pragma unroll
                     for (int d = 0; d < DP / 16; ++d) {
                         const int d0 = 16 * d + (kScaled ? 2 * oct : oct), d1 = d0 + (kScaled ? 1 : 8);

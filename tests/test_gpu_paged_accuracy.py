@@ -8,7 +8,8 @@ That error, with D terms a score, n tokens and A = sum p |v|:
   as multiples of 2^-24 of its largest; a score off by ds moves an output by 2 ds A;
 * exponentials, products and sums: 2 (n + 16) 2^-23 A;
 * probabilities in two pieces, of half a step each: 2^-22 A (fp16), 2^-16 A (bf16), and, of fp16, half
-  the smallest step: 2^-35 of the largest weight that a token has, times the largest V, n times."""
+  the smallest step: 2^-35 of the largest weight that a token has (2^-29 where a weight is a product with a
+  scale of V), times the largest V, n times."""
 
 from __future__ import annotations
 
@@ -54,7 +55,7 @@ def exact(q, k, v, n, k_scale=None, v_scale=None):
     A = torch.einsum("bhgt,bthd->bhgd", p, v.abs())
     weight = (p * vs.transpose(1, 2)[:, :, None, :]).amax(-1, keepdim=True)
     d = A * (piece + 2 * ds + 2 * (n.double()[:, None, None, None] + 16) * 2.0 ** -23)
-    d = d + n[:, None, None, None] * 2.0 ** -35 * weight * codes.abs().amax()
+    d = d + n[:, None, None, None] * 2.0 ** (-35 if v_scale is None else -29) * weight * codes.abs().amax()
     return o.flatten(1, 2), d.flatten(1, 2)
 
 
@@ -102,3 +103,49 @@ def test_long_sums_do_not_drift(q_type, dtype):
     assert abs(float(((got - o.to(q_type).double()) / o).mean())) <= 2.0 ** -15
     half_step = torch.finfo(q_type).eps / 2
     assert float(((got - o) / o).abs().max()) <= half_step + 2.0 ** -13
+
+
+@pytest.mark.parametrize("q_type,dtype", [(F32, I8), (F32, E4M3), (F16, I8), (BF16, E4M3)])
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens", [(8, 2, 64, 512), (16, 1, 128, 8), (24, 1, 256, 3000)])
+def test_scales_far_apart(q_type, dtype, heads, kv_heads, dim, tokens):
+    """Scales of V from 2^-20 to 2^20, and tokens whose scale is 10^8 times as large without any weight: what the
+    others add up to keeps its bits."""
+    batch = 6
+    shape = (batch, -(-tokens // 8) * 8, kv_heads, dim)
+    k, v = codes(shape, dtype), codes(shape, dtype)
+    ks = torch.full(shape[:3], 0.01, device=DEV)
+    vs = 0.01 * torch.exp2(torch.rand(shape[:3], device=DEV) * 40 - 20)
+    vs[0] = vs[1] = 0.01
+    q = torch.randn((batch, heads, dim), device=DEV).to(q_type)
+    # first, last or in the middle: a key so far on the other side of every query that its weight is 0
+    q[:, :, 0] = 16
+    for b, at in ((0, 0), (1, tokens - 1), (2, tokens // 2), (3, 0)):
+        k[b, at] = 0
+        k[b, at, :, 0] = torch.tensor(-100.0).to(dtype)
+        ks[b, at], vs[b, at] = 10, 1e6
+    n = torch.full((batch,), tokens, device=DEV, dtype=torch.int32)
+    out, (want, d) = attend(q, k, v, n, ks, vs), exact(q, k, v, n, ks, vs)
+    check(out, want, d)
+    if q_type is F32:  # errors of either sign
+        assert float(((out - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))).max()) <= 1e-5
+
+
+@pytest.mark.parametrize("q_type,dtype", [(F32, I8), (BF16, E4M3)])
+def test_scales_while_scores_grow(q_type, dtype):
+    """Scores that rise tile by tile, and V's scales that fall or rise with them, far enough for each to be out
+    of the other's range at the end; tokens without scale; all scales 0."""
+    batch, tokens, dim = 5, 640, 64
+    shape = (batch, tokens, 2, dim)
+    k, v = codes(shape, dtype), codes(shape, dtype)
+    t = torch.linspace(0, 1, tokens, device=DEV)[None, :, None].expand(shape[:3])
+    k[..., 0] = torch.tensor(64.0).to(dtype)
+    ks = 0.1 * t
+    vs = torch.stack([torch.exp2(-60 * t[0]), torch.exp2(60 * t[1] - 60), torch.exp2(-60 * t[2]) * (t[2] > 0.5),
+                      torch.zeros_like(t[3]), torch.exp2(40 * torch.rand(t[4].shape, device=DEV) - 20)])
+    q = torch.randn((batch, 8, dim), device=DEV).to(q_type)
+    q[:, :, 0] = 30
+    n = torch.full((batch,), tokens, device=DEV, dtype=torch.int32)
+    out = attend(q, k, v, n, ks, vs)
+    assert not out[3].any()
+    # of a score, the largest term is 30 * 6.4 and the others are small: their sum's error is that of the largest
+    check(out, *exact(q, k, v, n, ks, vs))
