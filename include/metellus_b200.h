@@ -193,7 +193,8 @@ int mt_cache_read(int dev, const mt_paged_cache* cache, const mt_array* slots, c
  * g = h / (heads / kv_heads), for the tokens t in [max(0, n - window), n) (window 0: from
  * 0), n = lengths[b] clamped to the table's width; token t is in page
  * tables[b, t / page_size]. Pages outside [0, pages) count as absent. A sequence without
- * tokens (or whose scores are all -inf) gets zeros. q, out: [batch, heads, head_dim], last stride 1, of one type:
+ * tokens (or whose scores are all -inf) gets zeros. An infinity in q or in a visible row of V may
+ * come out as NaN where the formula has an infinity. q, out: [batch, heads, head_dim], last stride 1, of one type:
  * MT_F32, or the cache's own 16-bit type, or any of the three on an 8-bit cache; an
  * MT_F32 cache takes MT_F32. tables: MT_I32 [batch, width], last stride 1; lengths: MT_I32
  * [batch]; lse (may be NULL): MT_F32 [batch, heads], the natural logarithm of the sum of

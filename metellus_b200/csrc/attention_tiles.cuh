@@ -778,7 +778,9 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if constexpr (!Z::kExact || kPadded) s[b][n][i] += part[n][i];
-                        if constexpr (Z::kExact && (QP > 1 || CT == MT_F32)) s[b][n][i] += small[n][i];
+                        // of an infinite key the largest pieces alone make the score: what is left of an infinity is NaN
+                        if constexpr (Z::kExact && (QP > 1 || CT == MT_F32))
+                            if (fabsf(s[b][n][i]) != INFINITY) s[b][n][i] += small[n][i];
                     }
             }
             if constexpr (kScaled) {

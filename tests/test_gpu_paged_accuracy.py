@@ -149,3 +149,20 @@ def test_scales_while_scores_grow(q_type, dtype):
     assert not out[3].any()
     # of a score, the largest term is 30 * 6.4 and the others are small: their sum's error is that of the largest
     check(out, *exact(q, k, v, n, ks, vs))
+
+
+@pytest.mark.parametrize("q_type,dtype", [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("dim", [64, 80, 36])
+def test_infinite_keys(q_type, dtype, dim):
+    """A key that makes a score -inf has no weight, whatever pieces the product is made of; a sequence of
+    such keys alone gets zeros, and a score of +inf NaN."""
+    k, v = (torch.randn((4, 24, 2, dim), device=DEV).to(dtype) for _ in range(2))
+    q = torch.randn((4, 8, dim), device=DEV).to(q_type)
+    q[:, :, 3] = 1.7
+    n = torch.tensor([20, 7, 17, 20], device=DEV, dtype=torch.int32)
+    k[0, 19, :, 3] = k[1, 6, :, 3] = -torch.inf
+    k[2, :, :, 3] = -torch.inf
+    k[3, 5, :, 3] = torch.inf
+    out = attend(q, k, v, n)
+    check(out[:2], *exact(q[:2], k[:2], v[:2], n[:2] - 1))
+    assert not out[2].any() and bool(out[3].isnan().all())
