@@ -28,7 +28,7 @@ from metellus_b200.api.run import compile_program
 from metellus_b200.orchestrator.builder import Operations
 from metellus_b200.orchestrator.kernel_group import STATUS_KEY
 from metellus_b200.orchestrator.assembly.cache import cache_keys
-from metellus_b200.orchestrator.scheduler import buffer_sizes, check_slots, dispatch_of, scratch_of
+from metellus_b200.orchestrator.scheduler import buffer_sizes, check_slots, dispatch_of, host_dtype, scratch_of
 from metellus_b200.runtime import backend
 from metellus_b200.runtime.buffer import Buffer
 from metellus_b200.runtime.program import BindCache, CheckStatus
@@ -109,6 +109,9 @@ class Executable:
     def __call__(self, inputs: dict[str, np.ndarray] | None = None, out: dict[str, np.ndarray] | None = None, *,
                  wait: bool = True) -> dict[str, np.ndarray]:
         tensors = self.ops.tensors
+        for name, dst in (out or {}).items():
+            if name in tensors and tensors[name].dtype == "int32" and dst.dtype != np.int32:
+                raise ValueError(f"Executable: destination for {name!r} must be int32, got {dst.dtype}")
         for name, arr in (inputs or {}).items():
             if name not in self.input_keys:
                 raise KeyError(f"Executable: {name!r} is not an input of the program")
@@ -133,7 +136,7 @@ class Executable:
             t = tensors[name]
             dst = (out or {}).get(name)
             if dst is None:
-                dst = np.empty(t.shape, dtype=np.float32)
+                dst = np.empty(t.shape, dtype=host_dtype(t))
             if t.buffer_key != t.name:
                 raise ValueError(f"Executable: output {name!r} is a view; request its owner {t.buffer_key!r}")
             if dst.nbytes > self.env[t.buffer_key].nbytes or not dst.flags["C_CONTIGUOUS"]:

@@ -19,7 +19,7 @@ import numpy as np
 from metellus_b200.orchestrator.assembly.cache import cache_keys
 from metellus_b200.orchestrator.builder import Operations
 from metellus_b200.orchestrator.dag import build_dag
-from metellus_b200.orchestrator.ir import CacheWriteOp
+from metellus_b200.orchestrator.ir import CacheWriteOp, Tensor
 from metellus_b200.orchestrator.kernel_group import STATUS_KEY, KernelGroup
 from metellus_b200.runtime.program import (
     Allocate,
@@ -68,6 +68,11 @@ def buffer_sizes(ops: Operations, groups: tuple[KernelGroup, ...]) -> dict[str, 
         for key, nbytes in g.scratch:
             sizes[key] = max(sizes.get(key, 0), nbytes)
     return sizes
+
+
+def host_dtype(t: Tensor) -> type:
+    """What a tensor is on the host."""
+    return np.int32 if t.dtype == "int32" else np.float32
 
 
 def check_slots(ops: Operations, name: str, arr: np.ndarray) -> None:
@@ -144,12 +149,12 @@ def schedule(ops: Operations, groups: tuple[KernelGroup, ...], *, profile: bool 
             names = names_per_key.get(k, ())
             for vn in (n for n in names if n != k):
                 t = tensors[vn]
-                steps.append(Download(name=t.buffer_key, shape=t.shape, dtype=np.float32, into=t.name,
+                steps.append(Download(name=t.buffer_key, shape=t.shape, dtype=host_dtype(t), into=t.name,
                                       row_stride=t.row_stride, col_stride=t.col_stride,
                                       batch_stride=t.batch_stride))
             if k in names:
                 t = tensors[k]
-                steps.append(Download(name=k, shape=t.shape, dtype=np.float32, into=t.name))
+                steps.append(Download(name=k, shape=t.shape, dtype=host_dtype(t), into=t.name))
             else:
                 steps.append(Free(name=k))
             freed.add(k)

@@ -163,3 +163,20 @@ def test_names_of_a_caches_arrays_are_taken():
     ops.cache_write(k="kv.k", v="kv.k", cache="kv", slots="slots", out="kv1")
     with pytest.raises(ValueError, match="'kv.k' has the name of an array of cache 'kv'"):
         schedule(ops, compile_program(ops))
+
+
+def test_views_of_index_tensors_stay_int32():
+    """What a plan downloads of an int32 tensor (its views, as of any other) is int32 on the host."""
+    from metellus_b200.runtime.program import Download
+
+    ops = Operations()
+    ops.cache(PagedCache(4, 16, 2, 64), "kv")
+    ops.from_numpy(f32(6, 128), "k")
+    ops.indices(i32(2, 3), "grid")
+    ops.reshape("grid", (6,), out="slots")
+    ops.transpose("grid", out="turned")
+    ops.reshape("k", (6, 2, 64), out="rows")
+    ops.cache_write(k="k", v="rows", cache="kv", slots="slots", out="kv1")
+    steps = schedule(ops, compile_program(ops)).fragments
+    got = {s.into: np.dtype(s.dtype) for s in steps if isinstance(s, Download)}
+    assert got == {"slots": np.int32, "turned": np.int32, "rows": np.float32}

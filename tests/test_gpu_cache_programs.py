@@ -197,3 +197,35 @@ def test_results_repeat():
     for _ in range(5):
         np.testing.assert_array_equal(exe()["o"], first)
     exe.close()
+
+
+def test_views_of_index_tensors():
+    """Slots that are a view of a matrix: written by, and given back, as int32, by both ways to run."""
+    grid = np.array([[7, 2, 40], [33, 5, -1]], np.int32)
+    rows = np.random.default_rng(1).normal(0, 1, (6, KV, DIM)).astype(np.float32)
+
+    def program(cache):
+        ops = Operations()
+        ops.cache(cache, "kv")
+        ops.from_numpy(rows, "k")
+        ops.indices(grid, "grid")
+        ops.reshape("grid", (6,), out="slots")
+        ops.transpose("grid", out="turned")
+        ops.cache_write(k="k", v="k", cache="kv", slots="slots", out="kv1")
+        ops.cache_read("kv1", "slots", out="K")
+        return ops
+
+    want = np.where((grid.reshape(-1) >= 0)[:, None, None], rows, 0).transpose(1, 0, 2)
+    env = run(program(PagedCache(4, PS, KV, DIM))).env
+    assert env["slots"].dtype == np.int32 and np.array_equal(env["slots"], grid.reshape(-1))
+    assert env["turned"].dtype == np.int32 and np.array_equal(env["turned"], grid.T)
+    assert np.array_equal(env["K"], want)
+
+    exe = Executable(program(PagedCache(4, PS, KV, DIM)), outputs=("K", "grid"))
+    for _ in range(3):
+        got = exe({"grid": grid})
+        assert got["grid"].dtype == np.int32 and np.array_equal(got["grid"], grid)
+        assert np.array_equal(got["K"], want)
+    with pytest.raises(ValueError, match="must be int32"):
+        exe(out={"grid": np.empty((2, 3), np.float32)})
+    exe.close()
