@@ -19,7 +19,8 @@ Arrays are torch CUDA tensors (or another framework's whose type offers DLPack's
 API), all on one device; the last dimension is contiguous, the other
 strides are free. Calls run on torch's current stream of that device without waiting for
 it, allocate only through torch and can be captured into CUDA graphs. What does not fit
-raises ``ValueError`` before anything is launched. What the device alone knows is
+raises ``ValueError`` before anything is launched, tensors that require a gradient (or have a
+tangent) among it: the operators have no derivatives. What the device alone knows is
 handled there: slots and pages outside the cache are skipped, lengths are clamped to the
 table's width.
 
@@ -56,9 +57,22 @@ def _native():
     return _module
 
 
-def _grad_enabled():
-    torch = sys.modules.get("torch")
-    return None if torch is None else torch.is_grad_enabled
+_torch = None   # (forward_ad, what the binding is given, the same within forward-mode differentiation)
+
+
+def _autograd():
+    """torch's tensors, and its functions by which the binding refuses tensors with a gradient or a
+    tangent; None without torch."""
+    global _torch
+    if _torch is None:
+        torch = sys.modules.get("torch")
+        if torch is None:
+            return None
+        forward_ad = torch.autograd.forward_ad
+        hooks = (torch.Tensor, torch.is_grad_enabled)
+        _torch = (forward_ad, hooks + (None,), hooks + (forward_ad.unpack_dual,))
+    forward_ad, plain, dual = _torch
+    return dual if getattr(forward_ad, "_current_level", 0) >= 0 else plain
 
 
 def _dtype_code(dtype) -> int:
@@ -78,7 +92,7 @@ def cache_write(k, v, k_cache, v_cache, slots, *, k_scale=None, v_scale=None) ->
     that holds an infinity or a NaN gets the scale NaN. A slot outside the cache (such as
     -1 for padding) skips its row. Slots must be distinct: a slot given twice is left
     with a mixture of its rows; the others are not affected."""
-    (_module or _native()).cache_write(_grad_enabled(), k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    (_module or _native()).cache_write(_autograd(), k, v, k_cache, v_cache, k_scale, v_scale, slots)
 
 
 def cache_read(k_cache, v_cache, slots, *, k_scale=None, v_scale=None, dtype=None, out=None):
@@ -91,7 +105,7 @@ def cache_read(k_cache, v_cache, slots, *, k_scale=None, v_scale=None, dtype=Non
     if out is not None and dtype is not None:
         raise ValueError("cache_read: dtype and out exclude one another")
     to_k, to_v = (None, None) if out is None else out
-    return (_module or _native()).cache_read(_grad_enabled(), k_cache, v_cache, k_scale, v_scale, slots,
+    return (_module or _native()).cache_read(_autograd(), k_cache, v_cache, k_scale, v_scale, slots,
                                              -1 if dtype is None else _dtype_code(dtype), to_k, to_v)
 
 
@@ -109,5 +123,5 @@ def paged_attention(q, k_cache, v_cache, tables, lengths, *, k_scale=None, v_sca
     the float32 ``[batch, heads]`` natural logarithms of the sums of ``exp(scores)``, by
     which results over parts of a sequence can be joined. A sequence without visible
     tokens gets zeros (and -inf). Scores, sums and accumulators are float32."""
-    return (_module or _native()).paged_attention(_grad_enabled(), q, k_cache, v_cache, k_scale, v_scale, tables, lengths,
+    return (_module or _native()).paged_attention(_autograd(), q, k_cache, v_cache, k_scale, v_scale, tables, lengths,
                                                   scale, window, out, return_lse)

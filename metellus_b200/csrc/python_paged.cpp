@@ -11,6 +11,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/metellus_b200.h"
 
@@ -182,26 +183,51 @@ bool check(int rc) {
     return false;
 }
 
-// The operators have no backward pass: refuse to drop a gradient silently. `grad_enabled`
-// is asked only where an array requires one.
-bool no_grad(PyObject* grad_enabled, PyObject* x, const char* name) {
-    PyObject* r = PyObject_GetAttr(x, g_requires_grad);
-    if (!r) {
-        PyErr_Clear();
+// What the binding asks of a framework that tracks gradients, if one is loaded: its tensors' type,
+// whether it is tracking, and, while forward-mode derivatives are computed (else None), what takes a tensor
+// and its tangent apart.
+struct Autograd {
+    PyObject *type, *grad_enabled, *unpack_dual;
+    bool read(PyObject* x) {
+        type = nullptr;
+        return x == Py_None || PyArg_ParseTuple(x, "OOO", &type, &grad_enabled, &unpack_dual);
+    }
+
+    // The operators have no derivatives: refuse to drop one silently. `grad_enabled` is asked only
+    // where an array requires a gradient.
+    bool allows(PyObject* x, const char* name) {
+        if (!type || x == Py_None || !PyObject_TypeCheck(x, (PyTypeObject*)type)) return true;
+        if (unpack_dual != Py_None) {
+            PyObject* pair = PyObject_CallOneArg(unpack_dual, x);
+            PyObject* tangent = pair ? PySequence_GetItem(pair, 1) : nullptr;
+            Py_XDECREF(pair);
+            if (!tangent) return false;
+            Py_DECREF(tangent);
+            if (tangent != Py_None) {
+                PyErr_Format(PyExc_ValueError, "%s has a tangent; the paged cache's operators have no derivatives", name);
+                return false;
+            }
+        }
+        PyObject* r = PyObject_GetAttr(x, g_requires_grad);
+        if (!r) return false;
+        const int requires_grad = PyObject_IsTrue(r);
+        Py_DECREF(r);
+        if (requires_grad <= 0) return requires_grad == 0;
+        PyObject* e = PyObject_CallNoArgs(grad_enabled);
+        if (!e) return false;
+        const int on = PyObject_IsTrue(e);
+        Py_DECREF(e);
+        if (on > 0)
+            PyErr_Format(PyExc_ValueError,
+                         "%s requires a gradient; the paged cache's operators have none (use torch.no_grad() or detach it)", name);
+        return on == 0;
+    }
+    bool allows(PyObject* const* x, std::initializer_list<const char*> names) {
+        for (const char* name : names)
+            if (!allows(*x++, name)) return false;
         return true;
     }
-    const int requires_grad = PyObject_IsTrue(r);
-    Py_DECREF(r);
-    if (requires_grad <= 0 || grad_enabled == Py_None) return requires_grad >= 0;
-    PyObject* e = PyObject_CallNoArgs(grad_enabled);
-    if (!e) return false;
-    const int on = PyObject_IsTrue(e);
-    Py_DECREF(e);
-    if (on > 0)
-        PyErr_Format(PyExc_ValueError,
-                     "%s requires a gradient; the paged cache's operators have none (use torch.no_grad() or detach it)", name);
-    return on == 0;
-}
+};
 
 bool read_cache(Call& call, PyObject* const* args, mt_paged_cache* c) {
     memset(c, 0, sizeof *c);
@@ -216,32 +242,36 @@ bool count(Py_ssize_t n, Py_ssize_t want) {
     return false;
 }
 
-// (grad_enabled, k, v, k_cache, v_cache, k_scale, v_scale, slots)
+// (autograd, k, v, k_cache, v_cache, k_scale, v_scale, slots)
 PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!count(n, 8)) return nullptr;
     Call call;
+    Autograd autograd;
+    if (!autograd.read(args[0])) return nullptr;
     mt_array k, v, slots;
     mt_paged_cache c;
     void* stream;
     if (!call.array(args[1], "k", &k) || !call.array(args[2], "v", &v) || !read_cache(call, args + 3, &c) ||
         !call.array(args[7], "slots", &slots))
         return nullptr;
-    static const char* const names[] = {"k", "v", "k_cache", "v_cache"};
-    for (int i = 0; i < 4; ++i)
-        if (!no_grad(args[0], args[1 + i], names[i])) return nullptr;
-    if (!call.stream(&stream) || !check(mt_cache_write(call.device.id, &k, &v, &c, &slots, stream))) return nullptr;
+    if (!autograd.allows(args + 1, {"k", "v", "k_cache", "v_cache", "k_scale", "v_scale"})) return nullptr;
+    if (!call.stream(&stream) || !check(mt_cache_write(call.device.id, &k, &v, &c, &slots, stream)))
+        return nullptr;
     Py_RETURN_NONE;
 }
 
-// (grad_enabled, k_cache, v_cache, k_scale, v_scale, slots, dtype code or -1, out_k, out_v) -> (k, v)
+// (autograd, k_cache, v_cache, k_scale, v_scale, slots, dtype code or -1, out_k, out_v) -> (k, v)
 PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!count(n, 9)) return nullptr;
     Call call;
+    Autograd autograd;
+    if (!autograd.read(args[0])) return nullptr;
     mt_array k, v, slots;
     mt_paged_cache c;
     void* stream;
     if (!read_cache(call, args + 1, &c) || !call.array(args[5], "slots", &slots)) return nullptr;
-    if (!no_grad(args[0], args[1], "k_cache") || !no_grad(args[0], args[2], "v_cache")) return nullptr;
+    if (!autograd.allows(args + 1, {"k_cache", "v_cache", "k_scale", "v_scale"}) || !autograd.allows(args + 7, {"out[0]", "out[1]"}))
+        return nullptr;
     long dtype = PyLong_AsLong(args[6]);
     if (dtype == -1 && PyErr_Occurred()) return nullptr;
     PyObject *ok = args[7], *ov = args[8];
@@ -267,19 +297,20 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return result;
 }
 
-// (grad_enabled, q, k_cache, v_cache, k_scale, v_scale, tables, lengths, scale or None, window, out or None, return_lse)
+// (autograd, q, k_cache, v_cache, k_scale, v_scale, tables, lengths, scale or None, window, out or None, return_lse)
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!count(n, 12)) return nullptr;
     Call call;
+    Autograd autograd;
+    if (!autograd.read(args[0])) return nullptr;
     mt_array q, tables, lengths, out, lse;
     mt_paged_cache c;
     void* stream;
     if (!call.array(args[1], "q", &q) || !read_cache(call, args + 2, &c) || !call.array(args[6], "tables", &tables) ||
         !call.array(args[7], "lengths", &lengths))
         return nullptr;
-    static const char* const names[] = {"q", "k_cache", "v_cache"};
-    for (int i = 0; i < 3; ++i)
-        if (!no_grad(args[0], args[1 + i], names[i])) return nullptr;
+    if (!autograd.allows(args + 1, {"q", "k_cache", "v_cache", "k_scale", "v_scale"}) || !autograd.allows(args[10], "out"))
+        return nullptr;
     if (q.ndim != 3) return PyErr_Format(PyExc_ValueError, "paged_attention: q must have 3 dimensions, not %d", q.ndim);
     double scale;
     if (args[8] == Py_None) {
