@@ -20,7 +20,8 @@ API), all on one device; the last dimension is contiguous, the other
 strides are free. Calls run on torch's current stream of that device without waiting for
 it, allocate only through torch and can be captured into CUDA graphs. What does not fit
 raises ``ValueError`` before anything is launched, tensors that require a gradient (or have a
-tangent) among it: the operators have no derivatives. What the device alone knows is
+tangent) among it: the operators have no derivatives. Arrays that are written count as modified in
+place. What the device alone knows is
 handled there: slots and pages outside the cache are skipped, lengths are clamped to the
 table's width.
 
@@ -62,14 +63,14 @@ _torch = None   # (forward_ad, what the binding is given, the same within forwar
 
 def _autograd():
     """torch's tensors, and its functions by which the binding refuses tensors with a gradient or a
-    tangent; None without torch."""
+    tangent and counts writes; None without torch."""
     global _torch
     if _torch is None:
         torch = sys.modules.get("torch")
         if torch is None:
             return None
         forward_ad = torch.autograd.forward_ad
-        hooks = (torch.Tensor, torch.is_grad_enabled)
+        hooks = (torch.Tensor, torch.is_grad_enabled, torch.autograd.graph.increment_version)
         _torch = (forward_ad, hooks + (None,), hooks + (forward_ad.unpack_dual,))
     forward_ad, plain, dual = _torch
     return dual if getattr(forward_ad, "_current_level", 0) >= 0 else plain

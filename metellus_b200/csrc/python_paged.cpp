@@ -184,13 +184,13 @@ bool check(int rc) {
 }
 
 // What the binding asks of a framework that tracks gradients, if one is loaded: its tensors' type,
-// whether it is tracking, and, while forward-mode derivatives are computed (else None), what takes a tensor
-// and its tangent apart.
+// whether it is tracking, a function that counts a tensor's writes, and, while forward-mode derivatives
+// are computed (else None), one that takes a tensor and its tangent apart.
 struct Autograd {
-    PyObject *type, *grad_enabled, *unpack_dual;
+    PyObject *type, *grad_enabled, *count_write, *unpack_dual;
     bool read(PyObject* x) {
         type = nullptr;
-        return x == Py_None || PyArg_ParseTuple(x, "OOO", &type, &grad_enabled, &unpack_dual);
+        return x == Py_None || PyArg_ParseTuple(x, "OOOO", &type, &grad_enabled, &count_write, &unpack_dual);
     }
 
     // The operators have no derivatives: refuse to drop one silently. `grad_enabled` is asked only
@@ -227,6 +227,17 @@ struct Autograd {
             if (!allows(*x++, name)) return false;
         return true;
     }
+
+    // A tensor that something keeps for its own backward pass must not change behind its back.
+    bool written(PyObject* const* x, int n) {
+        for (int i = 0; i < n; ++i) {
+            if (!type || x[i] == Py_None || !PyObject_TypeCheck(x[i], (PyTypeObject*)type)) continue;
+            PyObject* r = PyObject_CallOneArg(count_write, x[i]);
+            if (!r) return false;
+            Py_DECREF(r);
+        }
+        return true;
+    }
 };
 
 bool read_cache(Call& call, PyObject* const* args, mt_paged_cache* c) {
@@ -255,7 +266,8 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
         !call.array(args[7], "slots", &slots))
         return nullptr;
     if (!autograd.allows(args + 1, {"k", "v", "k_cache", "v_cache", "k_scale", "v_scale"})) return nullptr;
-    if (!call.stream(&stream) || !check(mt_cache_write(call.device.id, &k, &v, &c, &slots, stream)))
+    if (!call.stream(&stream) || !check(mt_cache_write(call.device.id, &k, &v, &c, &slots, stream)) ||
+        !autograd.written(args + 3, 4))
         return nullptr;
     Py_RETURN_NONE;
 }
@@ -290,7 +302,7 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     PyObject* result = nullptr;
     if (ok && ov && call.array(ok, "out[0]", &k) && call.array(ov, "out[1]", &v) && call.stream(&stream) &&
-        check(mt_cache_read(call.device.id, &c, &slots, &k, &v, stream)))
+        check(mt_cache_read(call.device.id, &c, &slots, &k, &v, stream)) && autograd.written(args + 7, 2))
         result = PyTuple_Pack(2, ok, ov);
     Py_XDECREF(ok);
     Py_XDECREF(ov);
@@ -343,7 +355,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!call.stream(&stream) ||
         !check(mt_paged_attention(call.device.id, &q, &c, &tables, &lengths, &out, with_lse ? &lse : nullptr, scale, window,
                                   space ? (char*)space->dl_tensor.data + space->dl_tensor.byte_offset : nullptr, bytes,
-                                  stream)))
+                                  stream)) ||
+        !autograd.written(args + 10, 1))
         goto done;
     result = with_lse ? PyTuple_Pack(2, o, z) : Py_NewRef(o);
 done:

@@ -1,4 +1,5 @@
-"""The paged cache's operators beside torch's autograd: no derivative is dropped silently."""
+"""The paged cache's operators beside torch's autograd: no derivative is dropped silently, and what they
+write counts as modified."""
 
 from __future__ import annotations
 
@@ -85,3 +86,20 @@ def test_transforms_are_refused():
                 lambda: torch.func.vmap(f)(a["q"][None])):
         with pytest.raises((ValueError, RuntimeError)):
             run()
+
+
+def test_writes_are_counted():
+    a = arrays()
+    was = {n: x._version for n, x in a.items()}
+    attend(a), write(a), read(a)
+    written = {"out", "k_cache", "v_cache", "k_scale", "v_scale", "out_k", "out_v"}
+    assert {n for n, x in a.items() if x._version > was[n]} == written
+    # what was kept for a backward pass, and written over since, is found out there
+    x = torch.randn((2, 4, 64), device=DEV, requires_grad=True)
+    y = (x * a["out"]).sum()
+    attend(a)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        b = arrays()
+        attend(b), write(b), read(b)
