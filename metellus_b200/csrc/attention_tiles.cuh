@@ -1166,8 +1166,9 @@ __global__ void __launch_bounds__(DP * 2) join_parts(const __grid_constant__ Til
                 if (i + j * sides < count) take(ml[j], y[j]);
         }
     for (int half = sides / 2; half > 0; half /= 2) {
-        // the upper half of a row's teams hands over to the lower one
-        if (side >= half) {
+        // the upper half of a row's teams hands over to the lower one, each in a place of its own, which no
+        // later turn writes
+        if (side >= half && side < 2 * half) {
             sm_o[threadIdx.x] = o;
             if (lane == 0) sm_ml[team] = make_float2(m, l);
         }

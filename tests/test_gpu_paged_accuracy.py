@@ -166,3 +166,20 @@ def test_infinite_keys(q_type, dtype, dim):
     out = attend(q, k, v, n)
     check(out[:2], *exact(q[:2], k[:2], v[:2], n[:2] - 1))
     assert not out[2].any() and bool(out[3].isnan().all())
+
+
+@pytest.mark.parametrize("q_type,dtype,batch,heads,dim", [(F16, F16, 1, 4, 256), (F32, BF16, 2, 16, 128), (BF16, I8, 40, 8, 64),
+                                                          (F32, F32, 1, 1, 32)])
+def test_long_joins_repeat(q_type, dtype, batch, heads, dim):
+    """Sequences in many parts, joined by all teams of a block: the same bits every time, and right."""
+    tokens = 30000 // batch // 8 * 8
+    scaled = dtype is I8
+    k, v = (codes((batch, tokens, 1, dim), dtype) if scaled else torch.randn((batch, tokens, 1, dim), device=DEV).to(dtype)
+            for _ in range(2))
+    z = [0.01 * torch.rand((batch, tokens, 1), device=DEV) if scaled else None for _ in range(2)]
+    q = torch.randn((batch, heads, dim), device=DEV).to(q_type)
+    n = torch.randint(tokens // 2, tokens + 1, (batch,), device=DEV, dtype=torch.int32)
+    out = attend(q, k, v, n, *z)
+    check(out, *exact(q, k, v, n, *z))
+    for _ in range(50):
+        assert torch.equal(attend(q, k, v, n, *z), out)
