@@ -36,6 +36,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "mt_paged_attention.h"
@@ -1236,8 +1237,8 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     t.part_ml = (float2*)workspace;
     t.part_o = (float*)((char*)workspace + ml_bytes);
     auto kernel = t.row_chunks < Z::CPR ? attention_tiles<CT, Q, DP, NT, true> : attention_tiles<CT, Q, DP, NT, false>;
-    static bool ready[2][kMaxDevices] = {};
-    bool& is_ready = ready[t.row_chunks < Z::CPR][dev];
+    static std::atomic<bool> ready[2][kMaxDevices];  // calls of several threads may come first at once
+    std::atomic<bool>& is_ready = ready[t.row_chunks < Z::CPR][dev];
     if (!is_ready) {
         RT_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::SMEM));
         is_ready = true;

@@ -12,6 +12,7 @@
 #include <dlfcn.h>
 #include <nccl.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -139,7 +140,7 @@ int get_func(KernelEntry* k, int dev, CUfunction* f) {
     return 0;
 }
 
-int g_sms[kMaxDev] = {};
+std::atomic<int> g_sms[kMaxDev];  // looked up by whichever thread comes first
 
 }  // namespace
 
@@ -184,7 +185,7 @@ int sm_count(int dev, int* out) {
     if (!g_sms[dev]) {
         int v = 0;
         RT_CHECK(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev));
-        g_sms[dev] = v;  // the same value from every thread
+        g_sms[dev] = v;
     }
     *out = g_sms[dev];
     return 0;
