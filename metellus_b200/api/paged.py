@@ -15,8 +15,8 @@ float32 ``[pages, page_size, kv_heads]``, beside them (value = code * scale). Sl
 is token ``s % page_size`` of page ``s // page_size``; token ``t`` of sequence ``b`` is
 in page ``tables[b, t // page_size]``.
 
-Arrays are torch CUDA tensors (or another framework's whose type offers DLPack's C exchange
-API), all on one device; the last dimension is contiguous, the other
+Arrays are torch CUDA tensors (or another framework's) whose type offers DLPack's C exchange
+API, as torch 2.11's does, all on one device; the last dimension is contiguous, the other
 strides are free. Calls run on torch's current stream of that device without waiting for
 it, allocate only through torch and can be captured into CUDA graphs. What does not fit
 raises ``ValueError`` before anything is launched, tensors that require a gradient (or have a

@@ -72,7 +72,11 @@ const DLPackExchangeAPI* api_of(PyObject* x, const char* name) {
     Py_XDECREF(capsule);
     PyErr_Clear();
     if (!api || api->version.major != 1) {
-        PyErr_Format(PyExc_TypeError, "%s must be a CUDA tensor, not %s", name, Py_TYPE(x)->tp_name);
+        if (PyObject_HasAttrString(x, "__dlpack__"))
+            PyErr_Format(PyExc_TypeError, "%s is a %s, whose type does not offer DLPack's C exchange API, version 1 "
+                         "(__dlpack_c_exchange_api__; torch tensors do as of torch 2.11, perhaps earlier)", name, Py_TYPE(x)->tp_name);
+        else
+            PyErr_Format(PyExc_TypeError, "%s must be a CUDA tensor, not %s", name, Py_TYPE(x)->tp_name);
         return nullptr;
     }
     Py_INCREF(Py_TYPE(x));  // the type stays, and its API with it

@@ -144,3 +144,16 @@ def test_device_arrays_only():
         mt.paged_attention(x, c, c, i[:, None], i)
     with pytest.raises(TypeError, match="must be a CUDA tensor, not list"):
         mt.cache_read([1], c, i)
+
+
+def test_arrays_without_the_exchange_api():
+    """A tensor whose type has no such interface is told so, not that it is no tensor."""
+    pytest.importorskip("torch")
+    import metellus_b200 as mt
+
+    class Tensor:
+        def __dlpack__(self, **_):
+            raise AssertionError("not asked for")
+
+    with pytest.raises(TypeError, match="k_cache is a Tensor, whose type does not offer DLPack's C exchange API"):
+        mt.cache_read(Tensor(), Tensor(), Tensor())
