@@ -183,3 +183,38 @@ def test_long_joins_repeat(q_type, dtype, batch, heads, dim):
     check(out, *exact(q, k, v, n, *z))
     for _ in range(50):
         assert torch.equal(attend(q, k, v, n, *z), out)
+
+
+@pytest.mark.parametrize("q_type,dtype", [(F16, F16), (BF16, BF16), (F16, I8), (BF16, E4M3), (F32, I8), (F32, F32)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (32, 2, 128), (16, 1, 256), (24, 2, 80), (3, 1, 32)])
+def test_long_lines_whose_scores_grow_late(q_type, dtype, heads, kv_heads, dim):
+    """Hundreds of tiles a warp, then scores higher by 6 and scales of V 1000 times as large, by values of the other
+    sign: what was added up before has to be scaled down. The first 256 of 512 tokens are seen 400 times each, so the
+    two halves weigh about the same. Sums are off by 2^-14 A at most (as above, and scores of up to 12 by 2^-20 each), pieces
+    of bf16 by 2^-16 A."""
+    batch, times = 32, 400
+    scaled = dtype in (I8, E4M3)
+    k = (torch.randn((1, 512, kv_heads, dim), device=DEV) * 1.5).round().clamp(-4, 4)
+    k[:, 256:, :, 0] = 64
+    k[:, :256, :, 0] = 0
+    v = torch.randn((1, 512, kv_heads, dim), device=DEV).mul(4).round().clamp(-12, 12) + 40
+    v[:, 256:] *= -1
+    z = [torch.full((1, 512, kv_heads), x, device=DEV) for x in (0.25, 0.01)]
+    z[1][:, 256:] = 10
+    if not scaled:
+        k, v = k * z[0][..., None], v * z[1][..., None]
+        z = [None, None]
+    k, v = k.to(dtype), v.to(dtype)
+    q = torch.randn((batch, heads, dim), device=DEV) * 0.25
+    q[:, :, 0] = 6 / 16 * dim ** 0.5
+    q = q.to(q_type)
+    pages = [None if x is None else x.unflatten(1, (-1, 8)).flatten(0, 1) for x in (k, v, *z)]
+    order = torch.cat([torch.arange(32).repeat(times), torch.arange(32, 64)]).to(DEV, torch.int32)
+    n = torch.full((batch,), len(order) * 8, device=DEV, dtype=torch.int32)
+    got = paged_attention(q, *pages[:2], order.expand(batch, -1), n, k_scale=pages[2], v_scale=pages[3])
+    values = [x.double() if y is None else x.double() * y.double()[..., None] for x, y in ((k, z[0]), (v, z[1]))]
+    s = torch.einsum("bhgd,thd->bhgt", q.double().unflatten(1, (kv_heads, -1)), values[0][0]) * dim ** -0.5
+    s[..., :256] += torch.tensor(float(times)).double().log()
+    p = torch.softmax(s, -1)
+    o, A = (torch.einsum("bhgt,thd->bhgd", p, x).flatten(1, 2) for x in (values[1][0], values[1][0].abs()))
+    check(got, o, A * (2.0 ** -14 + (2.0 ** -16 if dtype is BF16 else 0)))
