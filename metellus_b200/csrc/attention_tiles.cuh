@@ -320,8 +320,8 @@ template <int TW> struct Cuts {
 };
 
 // kPadded: rows are shorter than DP. Only that form looks for their end: with the tests in it, the
-// other would be 5 to 30 % slower (bf16, 16 sequences of 4096 tokens, 8 heads of 256: 88 us, 115);
-// it takes 42 us at 80 dims, 98 of fp32, where products of whole DPs took 47, 157.
+// other would be 5 to 30 % slower (bf16, 16 sequences of 4096 tokens, 8 heads of 256: 91 us, 115);
+// it takes 44 us at 80 dims, 97 of fp32, where products of whole DPs took 47, 157.
 template <int CT, class Q, int DP, int NT, bool kPadded>
 __global__ void __launch_bounds__(Shape<CT, Q, DP, NT>::NW * 32, Shape<CT, Q, DP, NT>::BLOCKS)
 attention_tiles(const __grid_constant__ TileArgs t) {
@@ -1266,14 +1266,15 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
 // Over 8 query heads a key-value head: 16 of them a warp, or 8, so that neighbouring warps read the
 // same rows, which one of them finds in L2. 16 halve what the SMs read, and a warp then has fewer
 // registers left and twice as much to hand over; they win where a warp has many tiles (as far as
-// the tables' width tells). bf16, 2 heads of 128, 32 query heads, us: 16 sequences of 2048 tokens
-// (4 tiles a warp) 20.7, by eights 16.5; of 8192 (14) 38.0, 36.4; of 16384 (28) 56.6, 62.5; 64 of
-// 32768 (221) 322, 436. fp16, 1 head of 256: 7 of 16384 (12) 44.2, 39.8; 32 of 16384 (55) 118, 138.
-// 32-bit rows of over 64 dims leave 16 heads too few registers: 426, by eights 392 at 110 tiles a warp.
+// the tables' width tells). us by sixteens and by eights: bf16, 2 heads of 128, 32 query heads, 16 sequences of
+// 2048 tokens (4 tiles a warp) 21.3, 17.2; of 8192 (14) 40.0, 38.5; of 16384 (28) 58.6, 67.1; 64 of
+// 32768 (221) 326, 465. fp16, 1 head of 256: 7 of 16384 (12) 50.6, 36.8; 32 of 16384 (55) 120, 122.
+// 16 heads of the widest rows leave too few registers where elements are not 16 bits: fp32 over 64 dims 426,
+// 392 at 110 tiles a warp; int8 over 128, float32 queries, 32 of 16384 of 256 dims 178, 142, bfloat16 134, 121.
 template <int CT, class Q, int DP>
 int by_group(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, int dev, cudaStream_t st) {
-    if constexpr (CT != MT_F32 || DP <= 64) {
-        using Z = Shape<CT, Q, DP, 2>;
+    using Z = Shape<CT, Q, DP, 2>;
+    if constexpr (Z::EB == 2 || DP <= (Z::EB == 4 ? 64 : 128)) {
         int sms;
         if (int rc = sm_count(dev, &sms)) return rc;
         const int64_t tiles = (a.max_tokens < a.window ? a.max_tokens : a.window) / Z::TW;
