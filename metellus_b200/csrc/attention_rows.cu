@@ -1,14 +1,14 @@
 // Paged attention for any head_dim and alignment: one warp reads one key row at a time.
 //
 // Softmax in one pass: with the running maximum m of the scores, l = sum exp(s - m) and
-// o = sum exp(s - m) v; a new maximum m' scales l and o by exp(m - m'). Every warp of a
-// block keeps its own (m, l, o) over every eighth token; they are joined at the end.
+// o = sum exp(s - m) v; a new maximum m' scales l and o by exp(m - m'). Every warp of a sequence's
+// blocks keeps its own (m, l, o) over runs of 4 tokens; they are joined at the end.
 //
 // It serves what tiles cannot: rows that are not whole 16-byte pieces, caches whose rows have no 32-bit
 // numbers, scales that are not positive. Instructions bound it (a dot product's 5 exchanges for each
-// query head and token): bf16, 32 query heads on 8 of 100, 64 sequences of 1024 tokens 516 us (32 at the
-// copy rate; heads of 104, in tiles, 48). Few sequences are split over clusters of up to 8 blocks:
-// 1 of 16384 tokens 261 us, 2.6 ms in one block each, a token at a time.
+// query head and token): bf16, 32 query heads on 8 of 100, 64 sequences of 1024 tokens 518 us (32 at the
+// copy rate; heads of 104, in tiles, 50). Few sequences are split over clusters of up to 8 blocks:
+// 1 of 16384 tokens 258 us, 2.6 ms in one block each, a token at a time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

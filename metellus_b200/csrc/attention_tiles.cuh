@@ -19,9 +19,9 @@
 //   its heads in the workspace, and a second kernel joins them; it is launched early and
 //   waits for the first on the device.
 //
-// Measured (bf16, 32 query heads on 8 of 128, pages of 16 in random order): 64 sequences of 4096 to
-// 8192 tokens 243 us = 6.7 TB/s, the copy rate; 16 of 37 to 4001 27 us = 4.5 TB/s; 1 of 120001 82 us =
-// 6.0 TB/s; 1 of 100 7.6 us. The matrix pipe is busy 14 % of the time and a third of the issue slots are
+// Measured (bf16, 32 query heads on 8 of 128, pages of 16 in random order; replayed from graphs, as all
+// times here): 64 sequences of 4096 to 8192 tokens 246 us = 6.6 TB/s, the copy rate; 16 of 37 to 4001 28 us =
+// 4.4 TB/s; 1 of 120001 82 us = 6.0 TB/s; 1 of 100 7.6 us. The matrix pipe is busy 14 % of the time and a third of the issue slots are
 // used, so its 16-row form loses nothing here, and the 128-row form of tcgen05 would cut a line of
 // tiles eight times as coarsely and tie the warps of a block to one another's loads. What is left at
 // short lines are the ends: lengths, then page numbers, then rows have to arrive before the first
@@ -65,7 +65,7 @@ struct TileArgs {
 __device__ inline uint32_t smem_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // kBeyond: a row of 8-bit codes is 128 bytes or less, and the next one is another warp's of the
-// same block: L2 fetches 256 bytes (e4m3, 32 sequences of 8192: 107 us, with 128 bytes 111).
+// same block: L2 fetches 256 bytes (e4m3, 32 sequences of 8192, 64 query heads on 8 of 128: 99.0 us, with 128 bytes 99.8).
 template <bool kBeyond> __device__ inline void copy16(uint32_t dst, const void* src, bool really) {
     if constexpr (kBeyond)
         asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(really ? 16 : 0));
@@ -200,8 +200,8 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     // queries that fp16 may not hold are divided by a power of two per row
     static constexpr bool kNormed = CT != MT_F32 && !kBf16 && (kQ32 || kScaled);
     // A 16-bit cache's next rows are asked for in two bursts a tile, K's before the scores and V's behind
-    // them (64 sequences of 4096 .. 8192, bf16: 249 us, in one burst 257). 8-bit and 32-bit
-    // tiles, whose products take longer, lose by it (int8 44 -> 46, fp32 86 -> 91).
+    // them (64 sequences of 6144, bf16: 248 us, in one burst 253). 8-bit and 32-bit tiles, whose products take
+    // longer, lose by it (e4m3 99 -> 101, fp32 108 -> 110).
     static constexpr bool kTwoBursts = EB == 2;
     // The exponents' base m is raised only when a score passes it by more than kSlack (a factor of
     // 2^4), which after a head's first tiles is rare. fp16 probabilities are held times
@@ -222,7 +222,7 @@ template <int CT, class Q, int DP, int NT> struct Shape {
     static constexpr int warp_bytes(int stages) { return stages * STAGE + Q_BYTES + 128; }
     // stages and resident blocks: 3 blocks an SM (12 warps, 168 registers, enough for O of 64 each;
     // 4 for heads of 32) with 3 stages at least, else 2 blocks, else one. With one warp a scheduler instead of two, bf16
-    // under float32 queries took 79 us for 41 us of bytes.
+    // under float32 queries took 79 us for 41 us of bytes (now 49).
     static constexpr int kMost = 227 * 1024;          // of shared memory a block
     static constexpr bool fits(int warps, int stages, int blocks) {
         return warps * warp_bytes(stages) <= kMost && blocks * (warps * warp_bytes(stages) + 1024) <= 228 * 1024;
@@ -1097,7 +1097,7 @@ attention_tiles(const __grid_constant__ TileArgs t) {
 // middle of, if that ends in it. A block is teams of `lanes` threads, 4 dims each: all of DP, or,
 // for long chains of few rows, a slice of it (blockIdx.z), which leaves more teams. They take
 // `together` rows at a time, and of each row every teams / together-th part (all powers of two).
-// 1 sequence of 30000 tokens, 1 head of 256, 888 parts: 18 us, 47 with 8 teams of whole rows.
+// 1 sequence of 30000 tokens, 1 head of 256, 888 parts: 17 us, 47 with 8 teams of whole rows.
 constexpr int kLeastLanes = 8;
 
 template <class Q, int DP, int ROWS, int TW>
@@ -1214,9 +1214,10 @@ int launch(const AttentionArgs& a, bool run, void* workspace, uint64_t* bytes, i
     // A range a sequence where none has more than a few tiles: that costs less than a join. The more
     // so, the more of the warps that fit the GPU at once the sequences occupy: then a join has many
     // parts, and cutting gives each warp less to gain. Long tiles make up for a join sooner. us, whole
-    // and cut: bf16, 8 heads of 128, 1 sequence of 4 tiles 8.3, 7.3; 40 sequences (a quarter of the
-    // warps) of 6 tiles 10.4, 11.4, of 12 tiles 15.5, 12.5; 110 (three quarters) of 16 tiles 23.1,
-    // 29.7 (of 1 to 16 tiles 21.4, 22.6); fp32, 8 heads of 256, 8 sequences of 2 tiles 18.6, 15.5, of 4 tiles 29.8, 15.5.
+    // and cut: bf16, 8 heads of 128, 1 sequence of 4 tiles 8.3, 7.6; 40 sequences (a quarter of the
+    // warps) of 6 tiles 10.4, 11.6, of 12 tiles 16.5, 13.1; 110 (three quarters) of 16 tiles 22.9,
+    // 29.3 (of 1 to 16 tiles 21.4, 23.8); fp32, 8 heads of 256, 8 sequences of 2 tiles 17.2, 16.0, of 4 tiles 28.1, 15.8.
+    // (Tables that are wider than the sequences hide short ones: those are cut.)
     // Otherwise as many ranges as those warps can take the heads of, or fewer where there cannot be as
     // many tiles.
     const int64_t resident = (int64_t)sms * Z::BLOCKS * Z::NW, used = (int64_t)a.batch * t.items;
